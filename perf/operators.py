@@ -209,9 +209,11 @@ def work(case):
     a = math.erfc(case["sigma"] / math.sqrt(8.0))
     tests = [sum(a ** g for g in range(n)) for n in (range(G + 1) if case["ragged"] else [G])]
     ends = [a ** n if n < P else 0.0 for n in (range(G + 1) if case["ragged"] else [G])]
-    tests, ends = sum(tests) / len(tests), sum(ends) / len(ends)
-    dsize = 4 if case["draft"] == "probs" else size
-    read = tests * V * (size + dsize) + ends * V * size + tests * 16 + 8
+    lost = [1.0 - a ** n for n in (range(G + 1) if case["ragged"] else [G])]
+    tests, ends, lost = (sum(v) / len(v) for v in (tests, ends, lost))
+    # Of a draft given as probabilities a test needs the one of its code, and only a rejection the whole row.
+    dread = V * size * tests if case["draft"] == "logits" else 4 * tests + 4 * V * lost
+    read = V * size * (tests + ends) + dread + tests * 16 + 8
     return {"bytes": int(B * (read + 16)), "flops": int(B * V * (tests * 2 + ends) * 4)}
 
 
