@@ -671,11 +671,16 @@ __global__ __launch_bounds__(WAVES * 64) void vq_argmax_bf16_rot_kernel(
 // the register path does not cover (e.g. the 1024-wide object codebook).
 // Winners found by several waves for one latent (vq_argmin_few_kernel: the code tiles are shared out) meet in idx_out
 // through a 64-bit atomic min on (order-preserving distance bits, code); vq_unpack_key_kernel strips the distance
-// afterwards.  idx_out must have been filled with 0xFF bytes.
+// afterwards.  idx_out must have been filled with ones (vq_fill_key_kernel: a kernel and not a memory-set, because the
+// call may be recorded into a graph).
 __device__ __forceinline__ unsigned long long vq_pack_key(float d, int code) {
     const unsigned b = __builtin_bit_cast(unsigned, d);
     const unsigned ord = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
     return ((unsigned long long)ord << 32) | (unsigned)code;
+}
+__global__ void vq_fill_key_kernel(int64_t* __restrict__ idx, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < n) idx[i] = -1;
 }
 __global__ void vq_unpack_key_kernel(int64_t* __restrict__ idx, int64_t n) {
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -778,7 +783,7 @@ __global__ __launch_bounds__(WAVES * 64) void vq_argmin_generic_kernel(
 // global memory into MFMA operands, PF units requested ahead of the products that use them.  |z|^2 comes from the
 // same fragments (fp32: the lane's half row in ascending order, the very fmaf chain of the generic kernel; bf16: its
 // own pass, the fragments interleave the two halves).  Winners of the tile shares meet in idx_out through vq_pack_key
-// (idx_out filled with 0xFF bytes, vq_unpack_key_kernel afterwards).
+// (idx_out filled by vq_fill_key_kernel, vq_unpack_key_kernel afterwards).
 template <int DT>
 __global__ __launch_bounds__(64) void vq_argmin_few_kernel(
     const typename VqTraits<DT>::elem* __restrict__ z, const char* __restrict__ packed,
@@ -1144,8 +1149,7 @@ static int launch_search(const void* z, const char* ws, const VqPlan& p, int64_t
         int split = (int)((4 * kNumCU + groups - 1) / groups);     // aim at four waves per CU
         if (split > p.n_tiles) split = p.n_tiles;
         if (split > 1) {
-            if (hipMemsetAsync(idx_out, 0xFF, (size_t)n * sizeof(int64_t), st) != hipSuccess)
-                return fail(DVQ_ELAUNCH, "vq_argmin: cannot initialise the index buffer");
+            hipLaunchKernelGGL(vq_fill_key_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, idx_out, n);
             hipLaunchKernelGGL((vq_argmin_few_kernel<DT>), dim3((unsigned)groups, (unsigned)split), dim3(64), 0, st,
                                reinterpret_cast<const typename VqTraits<DT>::elem*>(z), ws, reinterpret_cast<const float*>(ws + p.e2_off),
                                n, D, p.n_tiles, idx_out);
