@@ -50,3 +50,15 @@ def set_compute_dtype(model, dtype):
         if hasattr(m, "compute_dtype"):
             m.compute_dtype = dtype
     return model
+
+
+def set_head_dtype(model, dtype):
+    """Operand type of the MLP heads (`Encoder`, `Decoder`) inside `model` alone: torch.float32, torch.bfloat16, or torch.int8
+    -- 8-bit integers with a scale per activation row and per output channel, sums exact, results fp32 (ops.linear_int8) --
+    for every batch size.  The PointNet encoders and the prior keep theirs; set_compute_dtype sets the heads again."""
+    if dtype not in (torch.float32, torch.bfloat16, torch.int8):
+        raise ValueError("dtype must be torch.float32, torch.bfloat16 or torch.int8")
+    for m in model.modules():
+        if getattr(m, "takes_int8", False):
+            m.compute_dtype = dtype
+    return model

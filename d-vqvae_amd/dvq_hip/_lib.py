@@ -59,6 +59,16 @@ class DvqPriorGather(ctypes.Structure):
     _fields_ = [("table", c_void_p), ("out", c_void_p), ("features", c_int)]
 
 
+class DvqPriorVerify(ctypes.Structure):
+    _fields_ = [("logits", c_void_p), ("logits_b", c_int64), ("logits_p", c_int64), ("logits_v", c_int64),
+                ("draft", c_void_p), ("draft_b", c_int64), ("draft_g", c_int64), ("draft_v", c_int64),
+                ("tokens", c_void_p), ("tokens_b", c_int64), ("tokens_g", c_int64),
+                ("u_accept", c_void_p), ("u_accept_b", c_int64), ("u_accept_g", c_int64),
+                ("u_draw", c_void_p), ("u_draw_b", c_int64), ("lengths", c_void_p), ("lengths_b", c_int64),
+                ("accepted", c_void_p), ("next", c_void_p), ("B", c_int64), ("G", c_int), ("P", c_int), ("V", c_int),
+                ("logits_dtype", c_int), ("draft_dtype", c_int), ("draft_probs", c_int)]
+
+
 # name -> (restype, argtypes); mirrors include/dvq_hip.h one to one
 SIGNATURES = {
     "dvq_version": (c_int, []),
@@ -82,6 +92,11 @@ SIGNATURES = {
                                    c_int, c_int, POINTER(c_void_p), c_int64, c_int, c_void_p]),
     "dvq_to_bf16": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "dvq_linear_bf16": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p]),
+    "dvq_int8_quantize_rows": (c_int, [c_int, POINTER(c_void_p), c_int, c_int64, c_int, c_int, POINTER(c_void_p), c_int64,
+                                       POINTER(c_void_p), c_void_p]),
+    "dvq_linear_int8": (c_int, [c_int, POINTER(c_void_p), POINTER(c_void_p), c_int64, POINTER(c_void_p), POINTER(c_void_p), c_int64,
+                                POINTER(c_void_p), c_int, c_int, c_int, c_int, POINTER(c_void_p), c_int, c_int64, c_void_p]),
+    "dvq_prior_verify": (c_int, [POINTER(DvqPriorVerify), c_void_p]),
     "dvq_prior_packed_bytes": (c_size_t, [c_int, c_int, c_int]),
     "dvq_prior_pack_weight": (c_int, [c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_void_p]),
     "dvq_prior_embed": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),

@@ -12,7 +12,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import DVQ_BF16, DVQ_F32, DvqHandMesh, DvqManoConsts, DvqPointMlp, DvqPriorGather, DvqPriorJob, DvqPriorVRow
+from ._lib import DVQ_BF16, DVQ_F32, DvqHandMesh, DvqManoConsts, DvqPointMlp, DvqPriorGather, DvqPriorJob, DvqPriorVerify, DvqPriorVRow
 
 
 # Optional per-kernel timing with HIP events on the launch stream (used by bench.py for the
@@ -329,6 +329,150 @@ def linear_batched(xs, Ws, bs, relu: bool = False, add_identity3: bool = False, 
     return outs
 
 
+# ------------------------------------------------------- 8-bit integer product
+INT8_MAX_K = (1 << 17) - 1       # longest sum of products of 8-bit codes that 32 bits hold exactly
+
+
+def _launch(fn, name: str, dev: torch.device, *args) -> None:
+    """Call a C entry with `dev` current and torch's stream of that device as the last argument."""
+    st = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        rc = fn(*args, st)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, st)
+    _lib.check(rc, name)
+
+
+def _rows(t: torch.Tensor, what: str, dtypes, dev=None):
+    """Row stride of a 2-D HIP tensor with unit inner stride."""
+    if t.dim() != 2 or t.dtype not in dtypes:
+        raise RuntimeError(f"{what} must be a 2-D tensor of {' or '.join(str(d) for d in dtypes)}, got {tuple(t.shape)} {t.dtype}")
+    if not t.is_cuda:
+        raise RuntimeError("dvq_hip kernels need tensors on a HIP device (got a CPU tensor); there is no CPU fallback")
+    if dev is not None and t.device != dev:
+        raise RuntimeError(f"{what} is on {t.device}, the other operands on {dev}")
+    n, w = t.shape
+    if w > 1 and t.stride(1) != 1:
+        raise RuntimeError(f"{what} must have unit inner stride")
+    return t.stride(0) if n > 1 else max(w, 1)
+
+
+def _vector(t: torch.Tensor, what: str, n: int, dev) -> None:
+    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != dev:
+        raise RuntimeError(f"{what} must be a contiguous float32 [{n}] on {dev}")
+
+
+def _quantize(xs, what: str):
+    """Codes and scales of matrices of one shape, type and row stride, one launch: (list of code pointers, their row
+    stride, list of scale pointers, the buffer that holds them)."""
+    x0 = xs[0]
+    ldx = _rows(x0, what, (torch.float32, torch.bfloat16))
+    M, K = x0.shape
+    for x in xs[1:]:
+        if _rows(x, what, (x0.dtype,), x0.device) != ldx or x.shape != x0.shape:
+            raise RuntimeError(f"{what}: all matrices must have one shape, type and row stride")
+    if not 1 <= K <= INT8_MAX_K:
+        raise RuntimeError(f"{what}: 1..{INT8_MAX_K} features per row, got {K}")
+    n, ldc = len(xs), (K + 63) // 64 * 64
+    each = M * ldc + (M * 4 + 15) // 16 * 16
+    buf = torch.empty(n * each, dtype=torch.uint8, device=x0.device)
+    base = buf.data_ptr()
+    codes = [base + i * each for i in range(n)]
+    scales = [c + M * ldc for c in codes]
+    if M > 0:
+        arr = ctypes.c_void_p * n
+        _launch(_lib.load().dvq_int8_quantize_rows, "dvq_int8_quantize_rows", x0.device, n, arr(*[x.data_ptr() for x in xs]),
+                _dtype_code(x0), ldx, M, K, arr(*codes), ldc, arr(*scales))
+    return codes, ldc, scales, buf
+
+
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(codes int8 [M,K], scale float32 [M]) of the rows of x [M,K] (float32 or bfloat16, unit inner stride): a = max|x|,
+    code = 127 x / a rounded to the nearest whole number (ties to even, of the exact quotient), scale = a / 127.  A row of
+    zeros has codes and scale 0; a row with an infinity or a NaN has codes 0 and scale NaN.  Rows of activations (a scale
+    per token) and of weights [N,K] (a scale per output channel) are quantised alike."""
+    if x.dim() != 2:
+        raise RuntimeError(f"quantize_rows: x must be 2-D, got {tuple(x.shape)}")
+    M, K = x.shape
+    _, ldc, _, buf = _quantize([x], "quantize_rows: x")
+    return buf[:M * ldc].view(torch.int8).view(M, ldc)[:, :K], buf[M * ldc:M * ldc + 4 * M].view(torch.float32)
+
+
+def linear_int8(x, W: torch.Tensor, w_scale: torch.Tensor, b: Optional[torch.Tensor] = None, relu: bool = False,
+                out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """act(x W^T + b) with both operands in 8-bit integers: W int8 [N,K] with w_scale float32 [N] (quantize_rows of the
+    float weight gives both), x float32 or bfloat16 [M,K], quantised row by row in the call, or a pair (codes int8 [M,K],
+    scale float32 [M]) quantised before.  The sums are exact in 32-bit integers; scaling and bias are rounded once to the
+    output's type, float32 or bfloat16.  `out` [M,N] may be a column slice of a wider row-major buffer (not of x's).
+    Inference only: no gradient flows through the codes."""
+    if out is not None:
+        out_dtype = out.dtype
+    return _linear_int8([x], [W], [w_scale], [b], relu, out, out_dtype, "linear_int8")[0]
+
+
+def linear_int8_batched(xs, Ws, w_scales, bs, relu: bool = False, out_dtype: torch.dtype = torch.float32) -> list:
+    """Several linear_int8() calls of one shape -- own x, W, w_scale and b each -- in one launch (up to 8)."""
+    n = len(xs)
+    if not 1 <= n <= 8 or len(Ws) != n or len(w_scales) != n or len(bs) != n:
+        raise RuntimeError("linear_int8_batched: 1..8 products, one x, W, w_scale and b (or None) each")
+    return _linear_int8(list(xs), Ws, w_scales, bs, relu, None, out_dtype, "linear_int8_batched")
+
+
+def _linear_int8(xs, Ws, w_scales, bs, relu, out, out_dtype, what):
+    pairs = isinstance(xs[0], (tuple, list))
+    if any(isinstance(x, (tuple, list)) != pairs for x in xs):
+        raise RuntimeError(f"{what}: either all x are quantised already or none")
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError(f"{what}: output of float32 or bfloat16, not {out_dtype}")
+    first = xs[0][0] if pairs else xs[0]
+    dev = first.device
+    keep = None
+    if pairs:
+        ldx = _rows(first, f"{what}: codes", (torch.int8,))
+        for c, s in xs:
+            if _rows(c, f"{what}: codes", (torch.int8,), dev) != ldx or c.shape != first.shape:
+                raise RuntimeError(f"{what}: all x must have one shape and row stride")
+            _vector(s, f"{what}: the scale of x", first.shape[0], dev)
+    elif first.dim() != 2:
+        raise RuntimeError(f"{what}: x must be 2-D, got {tuple(first.shape)}")
+    M, K = first.shape
+    ldw = _rows(Ws[0], f"{what}: W", (torch.int8,), dev)
+    N = Ws[0].shape[0]
+    for W, s, b in zip(Ws, w_scales, bs):
+        if _rows(W, f"{what}: W", (torch.int8,), dev) != ldw or W.shape != (N, K):
+            raise RuntimeError(f"{what}: W must be int8 [{N},{K}] (all of one row stride), got {tuple(W.shape)}")
+        _vector(s, f"{what}: w_scale", N, dev)
+        if b is not None:
+            _vector(b, f"{what}: b", N, dev)
+    if not 1 <= K <= INT8_MAX_K:
+        raise RuntimeError(f"{what}: 1..{INT8_MAX_K} features per row, got {K}")
+    if out is not None:
+        ldy = _rows(out, f"{what}: out", (torch.float32, torch.bfloat16), dev)
+        if out.shape != (M, N) or ldy < N:
+            raise RuntimeError(f"{what}: out must be [{M},{N}] with rows that do not overlap")
+        if out.untyped_storage().data_ptr() == first.untyped_storage().data_ptr() and M > 0:
+            raise RuntimeError(f"{what}: out must not lie in the memory of x")
+        outs = [out]
+    else:
+        ldy = N
+        outs = [torch.empty(M, N, dtype=out_dtype, device=dev) for _ in xs]
+    if M == 0 or N == 0:
+        return outs
+    n = len(xs)
+    arr = ctypes.c_void_p * n
+    if pairs:
+        codes, scales = [c.data_ptr() for c, _ in xs], [s.data_ptr() for _, s in xs]
+    else:
+        codes, ldx, scales, keep = _quantize(xs, f"{what}: x")
+    _launch(_lib.load().dvq_linear_int8, "dvq_linear_int8", dev, n, arr(*codes), arr(*scales), ldx,
+            arr(*[W.data_ptr() for W in Ws]), arr(*[s.data_ptr() for s in w_scales]), ldw,
+            arr(*[None if b is None else b.data_ptr() for b in bs]), M, K, N, int(relu), arr(*[o.data_ptr() for o in outs]),
+            _dtype_code(outs[0]), ldy)
+    del keep             # (the codes; the allocator hands them out again only to later work of this stream)
+    return outs
+
+
 # ------------------------------------------------------------------- call-site glue
 PRIOR_ORDER_MAX_CLASSES = 1024
 
@@ -544,6 +688,47 @@ def prior_sample(logits: torch.Tensor, u: torch.Tensor, x_out: torch.Tensor, tab
         rc = _lib.load().dvq_prior_sample(_p(logits), n, M, _p(u), u.stride(0), _p(x_out), x_out.stride(0), _p(table),
                                           0 if table is None else table.shape[1], dtype_code, _p(emb_out), _stream(logits))
     _lib.check(rc, "dvq_prior_sample")
+
+
+def prior_verify(logits: torch.Tensor, draft: torch.Tensor, tokens: torch.Tensor, u_accept: torch.Tensor, u_draw: torch.Tensor,
+                 lengths: Optional[torch.Tensor] = None, draft_probs: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Verification of drafted codes.  logits [B,P,V]: the prior's, for the history with the drafts in it, P = G or G + 1;
+    draft [B,G,V]: the logits (draft_probs: the probabilities) the codes were drawn from; float32 or bfloat16 each, any
+    strides (the prior's forward() returns [B,V,cells]).  tokens int64 [B,G]; lengths int64 [B]: how many codes of each row
+    were drafted (None: all G).  With p = softmax(logits) and q the draft's distribution, code g is kept while
+    u_accept[b,g] q(x) < p(x).  Returns (accepted int64 [B]: codes kept; next int64 [B]: at the first rejection a draw from
+    max(p - q, 0) at u_draw[b], after the last kept code a draw from p there if P positions reach it, else -1).
+    u_accept float64 [B,G] and u_draw float64 [B] lie in [0,1).  The codes kept and the code after them are distributed as
+    if drawn from the prior one by one; the results are those of 64-bit arithmetic.  A code outside [0,V) is rejected,
+    lengths are clamped to [0,G]; a distribution that is needed and has no mass (all -inf, or a NaN, +inf or negative
+    probability in it) makes next -1."""
+    for t, what, dim, dtypes in ((logits, "logits", 3, (torch.float32, torch.bfloat16)), (draft, "draft", 3, (torch.float32, torch.bfloat16)),
+                                 (tokens, "tokens", 2, (torch.int64,)), (u_accept, "u_accept", 2, (torch.float64,)),
+                                 (u_draw, "u_draw", 1, (torch.float64,))) + (() if lengths is None else ((lengths, "lengths", 1, (torch.int64,)),)):
+        if t.dim() != dim or t.dtype not in dtypes:
+            raise RuntimeError(f"prior_verify: {what} must be {dim}-D of {' or '.join(str(d) for d in dtypes)}, got {tuple(t.shape)} {t.dtype}")
+        if not t.is_cuda:
+            raise RuntimeError("dvq_hip kernels need tensors on a HIP device (got a CPU tensor); there is no CPU fallback")
+        if t.device != logits.device:
+            raise RuntimeError(f"prior_verify: {what} is on {t.device}, logits on {logits.device}")
+    B, P, V = logits.shape
+    G = draft.shape[1]
+    if draft.shape != (B, G, V) or tokens.shape != (B, G) or u_accept.shape != (B, G) or u_draw.shape != (B,) or (
+            lengths is not None and lengths.shape != (B,)):
+        raise RuntimeError(f"prior_verify: logits [B,P,V] = {tuple(logits.shape)} with draft [B,G,V], tokens and u_accept [B,G], u_draw and "
+                           f"lengths [B]; got {tuple(draft.shape)}, {tuple(tokens.shape)}, {tuple(u_accept.shape)}, {tuple(u_draw.shape)}")
+    if P not in (G, G + 1) or P < 1 or V < 1:
+        raise RuntimeError(f"prior_verify: {P} positions of logits for {G} drafted codes (as many, or one more) of {V}")
+    out = torch.empty(2, B, dtype=torch.int64, device=logits.device)
+    accepted, nxt = out[0], out[1]
+    if B == 0:
+        return accepted, nxt
+    a = DvqPriorVerify(logits.data_ptr(), *logits.stride(), draft.data_ptr(), *draft.stride(), tokens.data_ptr(), *tokens.stride(),
+                       u_accept.data_ptr(), *u_accept.stride(), u_draw.data_ptr(), u_draw.stride(0),
+                       None if lengths is None else lengths.data_ptr(), 0 if lengths is None else lengths.stride(0),
+                       accepted.data_ptr(), nxt.data_ptr(), B, G, P, V, _dtype_code(logits), _dtype_code(draft), int(draft_probs))
+    _launch(_lib.load().dvq_prior_verify, "dvq_prior_verify", logits.device, ctypes.byref(a))
+    return accepted, nxt
 
 
 def prior_uniforms(first_id: int, n: int, n_cells: int, seed: int, device) -> torch.Tensor:

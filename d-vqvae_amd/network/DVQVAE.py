@@ -30,14 +30,40 @@ def _bf16_weight(layer):
     return layer._dvq_bf16
 
 
-def _linear(layer, x, relu=False, out=None, bf16=False):
-    """nn.Linear (+ReLU) on the HIP kernels; with bf16=True large batches run on the bf16 matrix-core kernel."""
+class _Int8Copy:
+    """8-bit copy of a layer's weight and the version it was made of; deep copies and pickles carry an empty one."""
+
+    def __init__(self):
+        self.key = self.codes = self.scale = None
+
+    def __reduce__(self):
+        return _Int8Copy, ()
+
+
+def _int8_weight(layer):
+    """8-bit codes and per-channel scales of an nn.Linear's weight, kept on the layer and refreshed when the weight changes."""
+    W = layer.weight.detach()
+    key = (W.data_ptr(), W._version, dvq_hip.weights_epoch())
+    kept = layer.__dict__.setdefault("_dvq_int8", _Int8Copy())
+    if kept.key != key:
+        kept.codes, kept.scale = ops.quantize_rows(W.float())
+        kept.key = key
+    return kept.codes, kept.scale
+
+
+def _linear(layer, x, relu=False, out=None, bf16=False, int8=False):
+    """nn.Linear (+ReLU) on the HIP kernels; with bf16=True large batches run on the bf16 matrix-core kernel, with
+    int8=True every batch on the 8-bit integer one (activations quantised row by row, weights channel by channel)."""
+    if int8:
+        return ops.linear_int8(x, *_int8_weight(layer), layer.bias.detach(), relu=relu, out=out)
     W = layer.weight.detach()
     Wb = _bf16_weight(layer) if (bf16 and W.is_cuda and x.shape[0] >= ops.LINEAR_BF16_MIN_ROWS) else None
     return ops.linear(x, W, layer.bias.detach(), relu=relu, out=out, W_bf16=Wb)
 
 
 class Encoder(nn.Module):
+    takes_int8 = True               # compute_dtype may be torch.int8 (dvq_hip.set_head_dtype)
+
     def __init__(self, layer_sizes, latent_size):
         super().__init__()
         self.MLP = nn.Sequential()
@@ -50,15 +76,16 @@ class Encoder(nn.Module):
 
     def forward(self, x, out=None):
         x = x.detach()
-        bf16 = self.compute_dtype == torch.bfloat16
+        bf16, int8 = self.compute_dtype == torch.bfloat16, self.compute_dtype == torch.int8
         for m in self.MLP:
             if isinstance(m, nn.Linear):
-                x = _linear(m, x, relu=True, bf16=bf16)
-        return _linear(self.linear_means, x, out=out, bf16=bf16)
+                x = _linear(m, x, relu=True, bf16=bf16, int8=int8)
+        return _linear(self.linear_means, x, out=out, bf16=bf16, int8=int8)
 
 
 class Decoder(dvq_hip.DropsPackedCopies, nn.Module):
     _packed_defaults = {"_heads": dict, "_head_wkey": lambda: None}
+    takes_int8 = True               # compute_dtype may be torch.int8 (dvq_hip.set_head_dtype)
 
     def __init__(self, layer_sizes, latent_size):
         super().__init__()
@@ -77,7 +104,7 @@ class Decoder(dvq_hip.DropsPackedCopies, nn.Module):
         an fp32 [B, d] matrix or a pair (idx int64 [B], table [V, d]) standing for table[idx] (codebook rows).  With
         bf16 operands, three layers and a large batch the two wide layers run as dvq_hip.ops.head_mlp_bf16."""
         layers = [m for m in self.MLP if isinstance(m, nn.Linear)]
-        bf16 = self.compute_dtype == torch.bfloat16
+        bf16, int8 = self.compute_dtype == torch.bfloat16, self.compute_dtype == torch.int8
         first = pieces[0][0] if isinstance(pieces[0], tuple) else pieces[0]
         widths = [(pc[1] if isinstance(pc, tuple) else pc).shape[1] for pc in pieces]
         if (bf16 and first.is_cuda and len(layers) == 3
@@ -107,7 +134,7 @@ class Decoder(dvq_hip.DropsPackedCopies, nn.Module):
                     x[:, col:col + w] = pc.detach()
                 col += w
         for i, m in enumerate(layers):
-            x = _linear(m, x, relu=(i + 1 < len(layers)), bf16=bf16)
+            x = _linear(m, x, relu=(i + 1 < len(layers)), bf16=bf16, int8=int8)
         return x
 
 
@@ -158,8 +185,18 @@ class DVQVAE(dvq_hip.DropsPackedCopies, nn.Module):
         dt = encs[0].compute_dtype
         if hand_xyz.dim() != 3 or hand_xyz.shape[1] != 3:
             raise RuntimeError(f"DVQVAE: hand_xyz must be [B, 3, V], got {tuple(hand_xyz.shape)}")
-        if any(e.compute_dtype != dt for e in encs) or any(h.compute_dtype != dt for h in heads) or not hand_xyz.is_cuda:
+        int8 = all(h.compute_dtype == torch.int8 for h in heads)
+        if any(e.compute_dtype != dt for e in encs) or any(h.compute_dtype != dt and not int8 for h in heads) or not hand_xyz.is_cuda:
             return self.forward_per_part(obj_pc, hand_xyz)
+
+        def head_layer(x, layers, relu):
+            """The layer of one depth of the six heads, one launch for all."""
+            bs = [l.bias.detach() for l in layers]
+            if int8:
+                ws = [_int8_weight(l) for l in layers]
+                return ops.linear_int8_batched(x, [w for w, _ in ws], [s for _, s in ws], bs, relu=relu)
+            return ops.linear_batched(x, [l.weight.detach() for l in layers], bs, relu=relu,
+                                      Ws_bf16=[_bf16_weight(l) for l in layers] if bf16 else None)
         code = DVQ_BF16 if dt == torch.bfloat16 else DVQ_F32
         bf16 = dt == torch.bfloat16
         obj_feat_type, _, _ = self.obj_encoder_type(obj_pc)
@@ -179,11 +216,8 @@ class DVQVAE(dvq_hip.DropsPackedCopies, nn.Module):
         n_mlp = len([m for m in heads[0].MLP if isinstance(m, nn.Linear)])
         for i in range(n_mlp):
             layers = [[m for m in h.MLP if isinstance(m, nn.Linear)][i] for h in heads]
-            x = ops.linear_batched(x, [l.weight.detach() for l in layers], [l.bias.detach() for l in layers], relu=True,
-                                   Ws_bf16=[_bf16_weight(l) for l in layers] if bf16 else None)
-        layers = [h.linear_means for h in heads]
-        lat = ops.linear_batched(x, [l.weight.detach() for l in layers], [l.bias.detach() for l in layers],
-                                 Ws_bf16=[_bf16_weight(l) for l in layers] if bf16 else None)
+            x = head_layer(x, layers, True)
+        lat = head_layer(x, [h.linear_means for h in heads], False)
         vqs = [getattr(self, f"vqvae{k}").vector_quantization for k in range(6)]
         idxs = ops.vq_argmin_batched(lat, [v.embedding.weight.detach() for v in vqs], [v._prepared() for v in vqs])
         idx6, obj_emb = self.vqvae6.inference(obj_feat_type)

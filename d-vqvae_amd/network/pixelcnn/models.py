@@ -168,6 +168,25 @@ class GatedPixelCNN(dvq_hip.DropsPackedCopies, nn.Module):
         self._run_hip(bufs, (H, W), B, None, False, None, forced=x.to(torch.int64).contiguous(), collect=out)
         return out
 
+    @torch.no_grad()
+    def verify(self, x, label, draft, u_accept, u_draw, lengths=None, draft_probs=False):
+        """Verify drafted grids x (int64 [B,H,W], raster order) against this prior: one forward with x as the history, then
+        ops.prior_verify.  draft [B, H*W, input_dim]: the logits (draft_probs: probabilities, as generate(return_probs=True)
+        of a drafting prior returns them) the codes were drawn from; u_accept float64 [B, H*W], u_draw float64 [B];
+        lengths int64 [B]: only the first so many cells of a grid are drafts.  Returns (accepted [B], next [B]): the first
+        accepted cells of a grid and the code after them, where there is a cell for it (-1 where not), are distributed as
+        generate()'s."""
+        if x.dim() != 3:
+            raise RuntimeError(f"GatedPixelCNN.verify: x must be int64 [B,H,W], got {tuple(x.shape)}")
+        B, H, W = x.shape
+        if B == 0:
+            empty = torch.zeros(0, dtype=torch.int64, device=x.device)
+            return empty, empty.clone()
+        if draft.dim() != 3 or draft.shape[:2] != (B, H * W):
+            raise RuntimeError(f"GatedPixelCNN.verify: draft must be [{B},{H * W},codes], got {tuple(draft.shape)}")
+        cells = self.forward(x, label).flatten(2).transpose(1, 2)             # [B, H*W, codes], a view
+        return ops.prior_verify(cells, draft, x.reshape(B, H * W), u_accept, u_draw, lengths, draft_probs)
+
     # ------------------------------------------------------------------ sampling
     def _code(self):
         if self.compute_dtype == torch.bfloat16:

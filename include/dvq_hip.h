@@ -35,7 +35,7 @@ extern "C" {
 #define DVQ_F32 0
 #define DVQ_BF16 1
 
-#define DVQ_VERSION 113   /* major*10000 + minor*100 + patch */
+#define DVQ_VERSION 114   /* major*10000 + minor*100 + patch */
 
 int dvq_version(void);
 const char* dvq_last_error(void);
@@ -359,6 +359,50 @@ int dvq_prior_sample(const float* logits, int n_classes, int M, const double* u,
  * 0x632BE59BD9B4E019 added between the two rounds).  No counterpart in the reference (which draws from torch's global
  * generator, models.py:193); a pure function of (seed, object id, cell), so any sharding of a batch draws the same grids. */
 int dvq_prior_uniforms(int64_t first_id, int64_t n, int n_cells, uint64_t seed, double* out, void* stream);
+
+/* ------------------------------------------------- 8-bit integer product
+ * No counterpart in the reference: the MLP heads (DVQ-VAE/network/DVQVAE.py:161-185) with 8-bit operands.
+ *
+ * dvq_int8_quantize_rows: for every row of x [M,K] (fp32 or bf16 by `dtype`, row stride ldx elements), a = max|x|:
+ *   code = 127 x / a rounded to the nearest whole number, ties to even (of the exact quotient), scale = fl32(a / 127);
+ *   a = 0: codes and scale 0; a row with an infinity or a NaN: codes 0, scale NaN.
+ * codes: int8 [M, ldc], ldc % 16 == 0, K <= ldc; bytes K .. ldc-1 of a row are set to zero.  scale: fp32 [M].
+ *
+ * dvq_linear_int8: y[m,n] = act( (sum_k x[m,k] W[n,k]) xs[m] ws[n] + b[n] ), the sum exact in 32-bit integers, the rest in
+ *   fp32, rounded once to `y_dtype`.  x: int8 [M,K] with row stride ldx, W: int8 [N,K] with row stride ldw (strides in
+ *   bytes, any alignment), b nullable.  K < 2^17.  act: relu keeps a NaN.
+ * Both take host arrays of n_batch (1..8) device pointers: products of ONE shape as one launch. */
+int dvq_int8_quantize_rows(int n_batch, const void* const* x, int dtype, int64_t ldx, int M, int K, void* const* codes,
+                           int64_t ldc, float* const* scale, void* stream);
+int dvq_linear_int8(int n_batch, const void* const* x, const float* const* xs, int64_t ldx, const void* const* W,
+                    const float* const* ws, int64_t ldw, const float* const* b, int M, int K, int N, int relu,
+                    void* const* y, int y_dtype, int64_t ldy, void* stream);
+
+/* ---------------------------------------- verification of drafted codes
+ * What a drafting model proposed for the prior (models.py:161-198): row b brings n = lengths[b] (NULL: G) codes
+ * tokens[b, 0..n-1] drawn from the distributions `draft`, `logits` are the prior's for the same history (P = G or G + 1
+ * positions).  p = softmax(logits[b, g]), q = softmax(draft[b, g]), or draft[b, g] itself with draft_probs != 0.
+ *   code g is kept while  u_accept[b, g] * q(x_g) < p(x_g);  accepted[b] = how many were kept;
+ *   next[b] = at the first rejection g an inverse-CDF draw at u_draw[b] from max(p - q, 0) (from p where that has a mass
+ *   below 2^-40), after n kept codes a draw from p at position n if P > n, else -1.
+ * The draw is the first code whose cumulated mass exceeds u_draw * mass.  Comparison and draw come out as in 64-bit
+ * arithmetic.  A code outside [0, V) has p = q = 0 and is rejected; lengths are clamped to [0, G]; a needed distribution
+ * without mass (all logits -inf; a NaN, +inf, or negative probability in it) makes next[b] = -1, accepted[b] counts what was
+ * kept before it.  Strides in elements, any values (0 for broadcast).  V <= 2^20. */
+typedef struct DvqPriorVerify {
+    const void* logits;  int64_t logits_b, logits_p, logits_v;   /* [B, P, V] */
+    const void* draft;   int64_t draft_b, draft_g, draft_v;      /* [B, G, V] */
+    const int64_t* tokens;  int64_t tokens_b, tokens_g;          /* [B, G] */
+    const double* u_accept; int64_t u_accept_b, u_accept_g;      /* [B, G] in [0, 1) */
+    const double* u_draw;   int64_t u_draw_b;                    /* [B] in [0, 1) */
+    const int64_t* lengths; int64_t lengths_b;                   /* [B] or NULL */
+    int64_t* accepted;                                           /* [B] out */
+    int64_t* next;                                               /* [B] out */
+    int64_t B;
+    int G, P, V;
+    int logits_dtype, draft_dtype, draft_probs;
+} DvqPriorVerify;
+int dvq_prior_verify(const DvqPriorVerify* v, void* stream);
 
 #ifdef __cplusplus
 }

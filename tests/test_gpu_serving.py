@@ -1,0 +1,161 @@
+"""The 8-bit heads and the verification of drafted grids where the models call them, and both together: a drafting head in
+8 bits, its codes drawn from given uniforms, the prior's verification of them."""
+import copy
+import pickle
+
+import numpy as np
+import pytest
+import torch
+
+from dvq_hip import ops, rng, set_compute_dtype, set_head_dtype, synth
+from network.DVQVAE import Decoder, DVQVAE, Encoder
+from network.pixelcnn.models import GatedPixelCNN
+from oracle import serving_oracle as S
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def head(cls, sizes, latent, seed):
+    torch.manual_seed(seed)
+    return cls(sizes, latent).to(DEV).eval()
+
+
+def oracle_mlp(linears, x, relu_last):
+    """The layers one after the other on the oracle's codes, each output rounded to fp32 as the kernel hands it on; the last
+    layer's float64 output."""
+    for i, l in enumerate(linears):
+        W, t = S.int8_codes(l.weight.detach().cpu())
+        c, s = S.int8_codes(x)
+        y = S.linear_int8(c, s, W, t, l.bias.detach().cpu().numpy(), relu_last or i + 1 < len(linears))
+        x = torch.from_numpy(y).float()
+    return y
+
+
+@pytest.mark.parametrize("B", [1, 7, 100, 600])
+def test_heads_in_8_bits_equal_the_layers_one_by_one(B):
+    """The same fp32 hand-over between layers: the oracle's rounding of a 64-bit value and the kernel's are the same one,
+    so codes agree and the last output is off by its own rounding (2^-24) at most."""
+    x = torch.randn(B, 1024, generator=torch.Generator().manual_seed(B))
+    e = set_head_dtype(head(Encoder, [1024, 512], 256, 0), torch.int8)
+    y = e(x.to(DEV)).cpu().double().numpy()
+    ref = oracle_mlp([m for m in e.MLP if isinstance(m, torch.nn.Linear)] + [e.linear_means], x, False)
+    assert np.all(np.abs(y - ref) <= 2.0 ** -24 * np.abs(ref) * (1 + 1e-6) + 2.0 ** -50)
+    d = set_head_dtype(head(Decoder, [1024, 128, 6], 1024, 1), torch.int8)
+    ref = oracle_mlp([m for m in d.MLP if isinstance(m, torch.nn.Linear)], x, False)
+    assert np.all(np.abs(d(x.to(DEV)).cpu().double().numpy() - ref) <= 2.0 ** -24 * np.abs(ref) * (1 + 1e-6) + 2.0 ** -50)
+
+
+def test_decoder_takes_its_input_in_pieces():
+    d = set_head_dtype(head(Decoder, [1024, 128, 6], 2048, 2), torch.int8)
+    g = torch.Generator().manual_seed(0)
+    table, idx, f = torch.randn(128, 1024, generator=g).to(DEV), torch.randint(0, 128, (40,), generator=g).to(DEV), torch.randn(40, 1024, generator=g).to(DEV)
+    assert torch.equal(d.forward_pieces([(idx, table), f]), d(torch.cat([table[idx], f], 1)))
+
+
+def test_8_bit_heads_follow_their_weights_and_stay_out_of_copies():
+    e = set_head_dtype(head(Encoder, [64, 32], 16, 3), torch.int8)
+    x = torch.randn(5, 64, generator=torch.Generator().manual_seed(1)).to(DEV)
+    a = e(x)
+    twin, loaded = copy.deepcopy(e), pickle.loads(pickle.dumps(e))
+    assert torch.equal(twin(x), a) and torch.equal(loaded.to(DEV)(x), a)
+    with torch.no_grad():
+        e.linear_means.weight.mul_(2.0)
+        e.linear_means.bias.mul_(2.0)
+    assert torch.allclose(e(x), 2 * a, rtol=1e-6) and torch.equal(twin(x), a)
+    set_compute_dtype(e, torch.float32)
+    assert not torch.equal(e(x), 2 * a)
+
+
+def test_error_of_8_bit_heads_is_that_of_their_rounding():
+    """Against fp32: every layer's operands are off by at most half a code, |x| and |w| by max/254.  For the first layer that
+    bounds an output by sum |w| a/254 + |x| a_w/254 + a a_w/254^2; here on the layer itself."""
+    torch.manual_seed(4)
+    l = torch.nn.Linear(1024, 512).to(DEV)
+    x = torch.randn(300, 1024, device=DEV)
+    y = ops.linear_int8(x, *ops.quantize_rows(l.weight.detach()), l.bias.detach()).double()
+    ref = x.double() @ l.weight.detach().double().T + l.bias.detach().double()
+    a, aw = x.abs().amax(1).double()[:, None], l.weight.detach().abs().amax(1).double()[None, :]
+    lim = l.weight.detach().abs().double().sum(1)[None, :] * a / 254 + x.abs().double().sum(1)[:, None] * aw / 254 + 1024 * a * aw / 254 ** 2
+    assert ((y - ref).abs() <= lim * (1 + 1e-6)).all()
+
+
+def test_hand_encoder_with_8_bit_heads_equals_its_parts_one_by_one():
+    torch.manual_seed(5)
+    m = DVQVAE(obj_inchannel=4).to(DEV).eval()
+    obj, hand = synth.object_clouds(3, 200, seed=1).to(DEV), torch.randn(3, 3, 778, generator=torch.Generator().manual_seed(2)).to(DEV)
+    set_head_dtype(m, torch.int8)
+    idx, emb = m(obj, hand)
+    idx1, emb1 = m.forward_per_part(obj, hand)
+    assert torch.equal(idx, idx1) and torch.equal(emb, emb1)
+
+
+def test_generation_with_8_bit_heads_runs_and_stays_near_fp32():
+    from dvq_hip.pipeline import GraspGenerator
+    gen = GraspGenerator.synthetic(torch.device(DEV), seed=0, with_prior=True)
+    objs = synth.object_clouds(3, 300, seed=4).to(DEV)
+    xt = torch.randint(0, 128, (3, 3, 3), generator=torch.Generator().manual_seed(0)).to(DEV)
+    ref = gen.generate(objs, x_tilde=xt)["vertices"]
+    set_head_dtype(gen.model, torch.int8)
+    out = gen.generate(objs, x_tilde=xt)["vertices"]
+    assert torch.isfinite(out).all() and out.shape == ref.shape and not torch.equal(out, ref)
+
+
+def prior(seed, layers=3, codes=128, dim=128):
+    torch.manual_seed(seed)
+    p = GatedPixelCNN(codes, dim, layers, n_classes=16).to(DEV).eval()
+    with torch.no_grad():
+        p.output_conv[2].weight.mul_(4.0)
+    return p
+
+
+@pytest.mark.parametrize("B", [1, 30])
+def test_a_drafting_prior_is_verified_by_another(B):
+    target, draft = prior(0), prior(1)
+    g = torch.Generator().manual_seed(2)
+    label = torch.randint(0, 16, (B,), generator=g).to(DEV)
+    u = lambda *s: torch.rand(*s, generator=g, dtype=torch.float64).to(DEV)
+    x, q = draft.generate(None, label, batch_size=B, uniforms=u(B, 9), return_probs=True)
+    ua, ud = u(B, 9), u(B)
+    lengths = torch.randint(0, 10, (B,), generator=g).to(DEV)
+    for n in (None, lengths):
+        acc, nxt = target.verify(x, label, q, ua, ud, lengths=n, draft_probs=True)
+        with torch.no_grad():
+            cells = target(x, label).flatten(2).transpose(1, 2)
+        ra, rn = S.verify(cells, q, x.reshape(B, 9), ua, ud, n, True)
+        assert np.array_equal(acc.cpu().numpy(), ra) and np.array_equal(nxt.cpu().numpy(), rn)
+    acc, nxt = target.verify(x, label, cells, ua, ud)                 # drafted by itself: all kept, no cell behind the last
+    assert (acc == 9).all() and (nxt == -1).all()
+    with pytest.raises(RuntimeError):
+        target.verify(x, label, q[:, :8], ua, ud, draft_probs=True)
+    with pytest.raises(RuntimeError):
+        target.verify(x.reshape(B, 9), label, q, ua, ud, draft_probs=True)
+    empty = target.verify(x[:0], label[:0], q[:0], ua[:0], ud[:0], draft_probs=True)
+    assert empty[0].shape == (0,) and empty[1].shape == (0,)
+
+
+def test_8_bit_drafting_head_and_verification_together():
+    """Object feature -> 9 x 128 draft logits in 8 bits (two products), codes drawn at given uniforms, one forward of the prior
+    with them as the history, verification; against the same steps on the oracle from the feature and the prior's logits on."""
+    B, V = 50, 128
+    target = prior(3)
+    h = set_head_dtype(head(Encoder, [1024, 256], 9 * V, 6), torch.int8)
+    g = torch.Generator().manual_seed(7)
+    feat = torch.randn(B, 1024, generator=g)
+    label = torch.randint(0, 16, (B,), generator=g).to(DEV)
+    u = rng.uniforms(torch.arange(B, device=DEV), 9, seed=1)
+    ua, ud = rng.uniforms(torch.arange(B, device=DEV), 9, seed=2), rng.uniforms(torch.arange(B, device=DEV), 1, seed=3)[:, 0]
+
+    d = h(feat.to(DEV)).view(B, 9, V)
+    x = torch.empty(B, 9, dtype=torch.int64, device=DEV)
+    ops.prior_sample(d.view(B * 9, V), u.reshape(-1), x.view(-1))
+    acc, nxt = target.verify(x.view(B, 3, 3), label, d, ua, ud)
+
+    lin = [m for m in h.MLP if isinstance(m, torch.nn.Linear)] + [h.linear_means]
+    ref = oracle_mlp(lin, feat, False)
+    assert np.all(np.abs(d.view(B, -1).cpu().double().numpy() - ref) <= 2.0 ** -24 * np.abs(ref) * (1 + 1e-6) + 2.0 ** -50)
+    with torch.no_grad():
+        cells = target(x.view(B, 3, 3), label).flatten(2).transpose(1, 2)
+    ra, rn = S.verify(cells, d, x, ua, ud)
+    assert np.array_equal(acc.cpu().numpy(), ra) and np.array_equal(nxt.cpu().numpy(), rn)
+    assert 0 < acc.sum() < 9 * B

@@ -1,0 +1,124 @@
+"""The oracles of the 8-bit product and of the verification against independent arithmetic, and what the entry points refuse.
+Nothing here needs a GPU: the C entries refuse before they launch."""
+import ctypes
+from fractions import Fraction
+
+import numpy as np
+import pytest
+import torch
+
+from dvq_hip import _lib, ops, set_head_dtype
+from oracle import serving_oracle as S
+
+VP = ctypes.c_void_p
+
+
+def test_codes_of_the_oracle_are_the_nearest_whole_numbers_of_exact_quotients():
+    g = torch.Generator().manual_seed(0)
+    x = torch.cat([torch.randn(40, 24, generator=g), torch.randn(40, 24, generator=g).to(torch.bfloat16).float(),
+                   torch.randint(-254, 255, (40, 24), generator=g).float() * 0.5])
+    x[80:, 0] = 127.0                          # halves: 127 x / a = x, ties throughout
+    codes, scale = S.int8_codes(x)
+    for m in range(x.shape[0]):
+        a = max(Fraction(float(v)) for v in x[m].abs())
+        for k in range(x.shape[1]):
+            assert codes[m, k] == round(127 * Fraction(float(x[m, k])) / a)          # Fraction rounds halves to even
+    assert codes.max() == 127 and codes.min() >= -127
+    assert np.array_equal(scale, (x.abs().amax(1).double() / 127).float().numpy())
+
+
+def test_codes_of_the_oracle_in_special_rows():
+    x = torch.zeros(5, 4)
+    x[1, 2] = float("inf")
+    x[2, 0] = float("nan")
+    x[3] = torch.tensor([1e-45, -1e-45, 0.0, 0.0])
+    x[4] = torch.tensor([3.4e38, -1.7e38, 1.0, 0.0])
+    codes, scale = S.int8_codes(x)
+    assert not codes[:3].any() and scale[0] == 0 and np.isnan(scale[1:3]).all()
+    assert codes[3].tolist() == [127, -127, 0, 0] and codes[4, 0] == 127 and np.isfinite(scale[4])
+
+
+def test_verification_oracle_keeps_the_target_distribution():
+    """Summed over drafted code and accept/reject, the first emitted code has probability p exactly: over all codes x,
+    q(x) min(1, p(x)/q(x)) + P(reject) (p - q)+ / mass = p(x).  Here by counting: 20000 rows."""
+    g = torch.Generator().manual_seed(1)
+    V, B = 6, 20000
+    t, d = torch.randn(V, generator=g), torch.randn(V, generator=g)
+    q = torch.softmax(d.double(), 0)
+    x = torch.multinomial(q.expand(B, V), 1, generator=g)
+    acc, nxt = S.verify(t.expand(B, 1, V), d.expand(B, 1, V), x, torch.rand(B, 1, generator=g, dtype=torch.float64),
+                        torch.rand(B, generator=g, dtype=torch.float64))
+    first = np.where(acc == 1, x[:, 0].numpy(), nxt)
+    p = torch.softmax(t.double(), 0).numpy()
+    # binomial deviation of a count of 20000: five of them
+    assert np.all(np.abs(np.bincount(first, minlength=V) / B - p) <= 5 * np.sqrt(p * (1 - p) / B))
+
+
+def _quantize(lib, n=1, M=4, K=16, ldc=16, dtype=0, ldx=16, ptr=16):
+    arr = (VP * 8)(*[ptr] * 8)
+    return lib.dvq_int8_quantize_rows(n, arr, dtype, ldx, M, K, arr, ldc, arr, None)
+
+
+def _product(lib, n=1, M=4, K=16, N=4, ldx=16, ldw=16, ldy=4, y_dtype=0, ptr=16):
+    arr = (VP * 8)(*[ptr] * 8)
+    return lib.dvq_linear_int8(n, arr, arr, ldx, arr, arr, ldw, None, M, K, N, 0, arr, y_dtype, ldy, None)
+
+
+@pytest.mark.parametrize("bad", [dict(n=0), dict(n=9), dict(K=0), dict(K=1 << 17, ldc=1 << 17), dict(ldc=24), dict(K=17), dict(M=-1),
+                                 dict(dtype=2), dict(ptr=None), dict(ldx=-1)])
+def test_quantize_refusals(bad):
+    lib = _lib.load()
+    assert _quantize(lib, **bad) == -1 and lib.dvq_last_error()
+
+
+@pytest.mark.parametrize("bad", [dict(n=0), dict(n=9), dict(K=0), dict(K=1 << 17), dict(M=-1), dict(N=0), dict(y_dtype=3), dict(ldy=3),
+                                 dict(ldx=-1), dict(ldw=-1), dict(ptr=None)])
+def test_product_refusals(bad):
+    lib = _lib.load()
+    assert _product(lib, **bad) == -1 and lib.dvq_last_error()
+
+
+def _verify_args(**kw):
+    a = _lib.DvqPriorVerify()
+    for f in ("logits", "draft", "tokens", "u_accept", "u_draw", "accepted", "next"):
+        setattr(a, f, 16)
+    a.B, a.G, a.P, a.V = 2, 3, 4, 8
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("bad", [dict(B=-1), dict(V=0), dict(V=(1 << 20) + 1), dict(P=2), dict(P=5), dict(G=0, P=0), dict(G=-1), dict(logits_dtype=2),
+                                 dict(draft_dtype=-1), dict(logits=None), dict(draft=None), dict(tokens=None), dict(u_accept=None),
+                                 dict(u_draw=None), dict(accepted=None), dict(next=None)])
+def test_verify_refusals(bad):
+    lib = _lib.load()
+    assert lib.dvq_prior_verify(ctypes.byref(_verify_args(**bad)), None) == -1 and lib.dvq_last_error()
+    assert lib.dvq_prior_verify(None, None) == -1
+
+
+def test_empty_calls_return_without_a_launch():
+    lib = _lib.load()
+    assert _quantize(lib, M=0) == 0 and _product(lib, M=0) == 0
+    assert lib.dvq_prior_verify(ctypes.byref(_verify_args(B=0)), None) == 0
+
+
+def test_cpu_tensors_and_wrong_types_are_refused():
+    x, W, s = torch.zeros(2, 16), torch.zeros(4, 16, dtype=torch.int8), torch.zeros(4)
+    for call in (lambda: ops.quantize_rows(x), lambda: ops.linear_int8(x, W, s), lambda: ops.linear_int8((W, s), W, s),
+                 lambda: ops.linear_int8(x.double(), W, s), lambda: ops.linear_int8(x, W, s, out_dtype=torch.float16),
+                 lambda: ops.linear_int8_batched([], [], [], []), lambda: ops.linear_int8_batched([x, (W, s)], [W, W], [s, s], [None, None])):
+        with pytest.raises(RuntimeError):
+            call()
+    lg, tok, u = torch.zeros(2, 3, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3, dtype=torch.float64)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        ops.prior_verify(lg, lg, tok, u, u[:, 0])
+
+
+def test_head_dtype_is_set_on_the_heads_alone():
+    from network.gen_net import GenNet
+    m = set_head_dtype(GenNet(), torch.int8)
+    assert m.decoder.compute_dtype == torch.int8 and m.pos_decoder.compute_dtype == torch.int8
+    assert m.obj_encoder_type.compute_dtype == torch.float32 and m.GatedPixelCNN.compute_dtype == torch.float32
+    with pytest.raises(ValueError):
+        set_head_dtype(m, torch.float16)
