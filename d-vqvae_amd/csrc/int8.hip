@@ -13,22 +13,23 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kInt8MaxBatch = 8;
-struct QuantBatch {
+// Fewer 64 x 64 tiles than this leave CUs without work: the kernel that splits k runs instead.
+constexpr int kInt8SplitBelow = 128;
+struct Int8Prepare {
     const void* x[kInt8MaxBatch];
+    const int8_t* W[kInt8MaxBatch];
     int8_t* codes[kInt8MaxBatch];
+    int8_t* w_codes[kInt8MaxBatch];
     float* scale[kInt8MaxBatch];
 };
 struct Int8Batch {
-    const int8_t* x[kInt8MaxBatch];
+    const void* x[kInt8MaxBatch];
     const float* xs[kInt8MaxBatch];
     const int8_t* W[kInt8MaxBatch];
     const float* ws[kInt8MaxBatch];
     const float* b[kInt8MaxBatch];
     void* y[kInt8MaxBatch];
 };
-
-__device__ __forceinline__ float int8_load(const float* p) { return *p; }
-__device__ __forceinline__ float int8_load(const unsigned short* p) { return bf16_bits_to_f32(*p); }
 
 // Code of x in a row whose factor is inv = 127 / a in 64 bits: the nearest whole number to the EXACT quotient 127 x / a,
 // ties to even.  x * inv is off by at most 2^-46 (|quotient| <= 127).  A quotient that is not a half differs from every
@@ -40,36 +41,7 @@ __device__ __forceinline__ int int8_code(float x, double inv) {
     return (int)rint(t);
 }
 
-// One workgroup per row: |x| as bit patterns orders like the values and puts infinities and NaN on top.
-template <typename T>
-__global__ __launch_bounds__(256) void int8_quantize_kernel(QuantBatch p, int64_t ldx, int K, int64_t ldc) {
-    __shared__ unsigned top[4];
-    const int64_t m = blockIdx.x;
-    const int tid = threadIdx.x;
-    const T* x = reinterpret_cast<const T*>(p.x[blockIdx.y]) + m * ldx;
-    int8_t* c = p.codes[blockIdx.y] + m * ldc;
-    unsigned a = 0;
-    for (int k = tid; k < K; k += 256) {
-        const unsigned bits = __builtin_bit_cast(unsigned, int8_load(x + k)) & 0x7FFFFFFFu;
-        a = bits > a ? bits : a;
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const unsigned other = __shfl_xor(a, o, 64);
-        a = other > a ? other : a;
-    }
-    if ((tid & 63) == 0) top[tid >> 6] = a;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 4; ++w) a = top[w] > a ? top[w] : a;
-    const bool finite = a < 0x7F800000u;
-    const double amax = (double)__builtin_bit_cast(float, a);
-    const double inv = finite && a > 0 ? 127.0 / amax : 0.0;
-    for (int k = tid; k < ldc; k += 256) c[k] = (k < K && inv > 0.0) ? (int8_t)int8_code(int8_load(x + k), inv) : (int8_t)0;
-    if (tid == 0) p.scale[blockIdx.y][m] = finite ? (float)(amax / 127.0) : __builtin_nanf("");
-}
-
-// 16 bytes of a row from byte k on, zeros behind the row's end; never reads outside the row.
+// 16 bytes of a row from byte k on, zeros behind the row's end; any alignment, never reads outside the row.
 __device__ __forceinline__ i32x4 int8_chunk(const int8_t* row, int k, int K) {
     i32x4 v = {0, 0, 0, 0};
     if (k + 16 <= K) __builtin_memcpy(&v, row + k, 16);
@@ -81,6 +53,117 @@ __device__ __forceinline__ i32x4 int8_chunk(const int8_t* row, int k, int K) {
     return v;
 }
 
+// Four elements of a row from element k on (k % 4 == 0), zeros behind the row's end.  `wide`: rows start at multiples of
+// four elements' bytes.
+__device__ __forceinline__ f32x4 int8_load4(const float* x, int k, int K, bool wide) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (wide && k + 4 <= K) return *reinterpret_cast<const f32x4*>(x + k);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (k + j < K) v[j] = x[k + j];
+    return v;
+}
+__device__ __forceinline__ f32x4 int8_load4(const unsigned short* x, int k, int K, bool wide) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (wide && k + 4 <= K) {
+        const uint2 u = *reinterpret_cast<const uint2*>(x + k);
+        v[0] = __builtin_bit_cast(float, u.x << 16); v[1] = __builtin_bit_cast(float, u.x & 0xFFFF0000u);
+        v[2] = __builtin_bit_cast(float, u.y << 16); v[3] = __builtin_bit_cast(float, u.y & 0xFFFF0000u);
+        return v;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (k + j < K) v[j] = bf16_bits_to_f32(x[k + j]);
+    return v;
+}
+
+// |x| as bit patterns orders like the values and puts infinities and NaN on top.
+__device__ __forceinline__ unsigned int8_top(unsigned a, f32x4 v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float f = v[j];                   // (a bit cast of the vector's element itself reads element 0)
+        const unsigned bits = __builtin_bit_cast(unsigned, f) & 0x7FFFFFFFu;
+        a = bits > a ? bits : a;
+    }
+    return a;
+}
+__device__ __forceinline__ unsigned wave_top(unsigned a) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const unsigned other = __shfl_xor(a, o, 64);
+        a = other > a ? other : a;
+    }
+    return a;
+}
+// Factor of the codes and scale of a row whose largest |x| has the bit pattern `top`.
+__device__ __forceinline__ double int8_inv(unsigned top, float& scale) {
+    const bool finite = top < 0x7F800000u;
+    const double amax = (double)__builtin_bit_cast(float, top);
+    scale = finite ? (float)(amax / 127.0) : __builtin_nanf("");
+    return finite && top > 0 ? 127.0 / amax : 0.0;
+}
+__device__ __forceinline__ unsigned int8_codes4(f32x4 v, double inv) {
+    if (!(inv > 0.0)) return 0;
+    unsigned c = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c |= (unsigned)(int8_code(v[j], inv) & 0xFF) << (8 * j);
+    return c;
+}
+
+// One wave per row; rows of up to kInt8Held features are read once and stay in registers between the maximum and the codes.
+constexpr int kInt8Held = 4096;
+template <typename T>
+__device__ __forceinline__ void int8_quantize_row(const T* x, int K, bool wide, int8_t* c, int ldc, float* scale) {
+    const int lane = threadIdx.x & 63;
+    f32x4 v[kInt8Held / 256];
+    unsigned a = 0;
+    if (K <= kInt8Held) {
+#pragma unroll
+        for (int i = 0; i < kInt8Held / 256; ++i)
+            if (i * 256 < K) { v[i] = int8_load4(x, i * 256 + lane * 4, K, wide); }
+#pragma unroll
+        for (int i = 0; i < kInt8Held / 256; ++i)
+            if (i * 256 < K) a = int8_top(a, v[i]);
+    } else {
+#pragma unroll 4
+        for (int k = lane * 4; k < K; k += 256) a = int8_top(a, int8_load4(x, k, K, wide));
+    }
+    float s;
+    const double inv = int8_inv(wave_top(a), s);
+    if (K <= kInt8Held) {
+#pragma unroll
+        for (int i = 0; i < kInt8Held / 256; ++i) {
+            const int k = i * 256 + lane * 4;
+            if (i * 256 < K && k < ldc) *reinterpret_cast<unsigned*>(c + k) = int8_codes4(v[i], inv);
+        }
+        for (int k = (K + 255) / 256 * 256 + lane * 4; k < ldc; k += 256) *reinterpret_cast<unsigned*>(c + k) = 0;
+    } else {
+#pragma unroll 4
+        for (int k = lane * 4; k < ldc; k += 256) *reinterpret_cast<unsigned*>(c + k) = int8_codes4(int8_load4(x, k, K, wide), inv);
+    }
+    if (lane == 0) *scale = s;
+}
+
+// Rows 0 .. M-1 of every matrix of the batch are quantised; T = int8_t: copied to rows that start at multiples of 16 bytes.
+// The N rows behind them (if any) are weights, copied alike.  One wave per row.
+template <typename T>
+__global__ __launch_bounds__(64) void int8_prepare_kernel(Int8Prepare p, int64_t ldx, int64_t ldw, int M, int K, int64_t ldc) {
+    const int bz = blockIdx.y;
+    const bool weight = (int)blockIdx.x >= M;
+    const int64_t m = weight ? (int)blockIdx.x - M : (int)blockIdx.x;
+    if (weight || sizeof(T) == 1) {
+        const int8_t* from = weight ? p.W[bz] + m * ldw : reinterpret_cast<const int8_t*>(p.x[bz]) + m * ldx;
+        int8_t* to = (weight ? p.w_codes[bz] : p.codes[bz]) + m * ldc;
+        for (int k = (int)threadIdx.x * 16; k < ldc; k += 1024) *reinterpret_cast<i32x4*>(to + k) = int8_chunk(from, k, K);
+        return;
+    }
+    if constexpr (sizeof(T) != 1) {
+        const T* x = reinterpret_cast<const T*>(p.x[bz]) + m * ldx;
+        const bool wide = (reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T))) == 0;
+        int8_quantize_row<T>(x, K, wide, p.codes[bz] + m * ldc, (int)ldc, p.scale[bz] + m);
+    }
+}
+
 // Scaled in 64 bits, rounded once: no intermediate leaves the range of 32 bits where the result does not (s is up to 2^121,
 // the sum up to 2^31), at four 64-bit instructions per output.
 __device__ __forceinline__ float int8_scale(int acc, float s, float t, float b, int relu) {
@@ -90,93 +173,337 @@ __device__ __forceinline__ float int8_scale(int acc, float s, float t, float b, 
 __device__ __forceinline__ void int8_store(float* y, float v) { *y = v; }
 __device__ __forceinline__ void int8_store(unsigned short* y, float v) { *y = f32_to_bf16_bits(v); }
 
-// Any strides and alignments: 64 x 64 outputs per workgroup, 64 k per step, operands through registers into LDS.
-template <typename Y>
-__global__ __launch_bounds__(256) void int8_any_kernel(Int8Batch p, int64_t ldx, int64_t ldw, int M, int K, int N, int relu,
-                                                       int64_t ldy) {
-    constexpr int LD = 80;                       // bytes per LDS row: 64 + 16, so that rows start 20 banks apart
-    __shared__ __align__(16) int8_t sa[64 * LD], sb[64 * LD];
-    const int bz = blockIdx.y;
+// Few rows: a workgroup takes 16 output channels of up to 16 rows over the whole of k, split among its eight waves, and
+// adds the waves' sums in LDS.  Every weight byte is read once, straight into the operand registers of the 16x16x64
+// instruction, and is requested before the rows are quantised -- by every workgroup for itself into LDS (16-byte pieces
+// of row r at piece ^ (r & 7), so that the eight rows of a read phase lie in different banks): the whole layer is one
+// launch.  K <= kInt8Held.
+template <typename T, typename Y>
+__global__ __launch_bounds__(512) void int8_rows16_kernel(Int8Batch p, int64_t ldx, int64_t ldw, int M, int K, int N, int relu, int64_t ldy) {
+    extern __shared__ __align__(16) int8_t smem[];
+    __shared__ float sc[16];
+    const int bz = blockIdx.y, n0 = (int)blockIdx.x * 16;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int nt = (N + 63) / 64;
-    const int m0 = (int)(blockIdx.x / nt) * 64, n0 = (int)(blockIdx.x % nt) * 64;
-    const int row = tid >> 2, ch = (tid & 3) * 16;
-    const int ma = m0 + row < M ? m0 + row : M - 1, nb = n0 + row < N ? n0 + row : N - 1;
-    const int8_t* pa = p.x[bz] + (int64_t)ma * ldx;
-    const int8_t* pb = p.W[bz] + (int64_t)nb * ldw;
-    const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
-    const int r = lane & 31, h = lane >> 5;
-    i32x16 acc;
+    const int Kp = (K + 127) / 128 * 128, steps = Kp / 64;
+    const int wr = n0 + (lane & 15) < N ? n0 + (lane & 15) : N - 1;
+    const int8_t* w = p.W[bz] + (int64_t)wr * ldw;
+    i32x4 wf[kInt8Held / 512];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e] = 0;
-    for (int k0 = 0; k0 < K; k0 += 64) {
-        const i32x4 va = int8_chunk(pa, k0 + ch, K), vb = int8_chunk(pb, k0 + ch, K);
-        __syncthreads();
-        *reinterpret_cast<i32x4*>(sa + row * LD + ch) = va;
-        *reinterpret_cast<i32x4*>(sb + row * LD + ch) = vb;
-        __syncthreads();
+    for (int i = 0; i < kInt8Held / 512; ++i)
+        if (wave + 8 * i < steps) wf[i] = int8_chunk(w, 64 * (wave + 8 * i) + 16 * (lane >> 4), K);
+    for (int r = wave; r < M; r += 8) {
+        const T* x = reinterpret_cast<const T*>(p.x[bz]) + r * ldx;
+        const bool wide = (reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T))) == 0;
+        f32x4 v[kInt8Held / 256];
+        unsigned a = 0;
 #pragma unroll
-        for (int kk = 0; kk < 64; kk += 32) {
-            const i32x4 fa = *reinterpret_cast<const i32x4*>(sa + (wm + r) * LD + kk + 16 * h);
-            const i32x4 fb = *reinterpret_cast<const i32x4*>(sb + (wn + r) * LD + kk + 16 * h);
-            acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa, fb, acc, 0, 0, 0);
+        for (int i = 0; i < kInt8Held / 256; ++i)
+            if (i * 256 < K) v[i] = int8_load4(x, i * 256 + lane * 4, K, wide);
+#pragma unroll
+        for (int i = 0; i < kInt8Held / 256; ++i)
+            if (i * 256 < K) a = int8_top(a, v[i]);
+        float s;
+        const double inv = int8_inv(wave_top(a), s);
+        if (lane == 0) sc[r] = s;
+#pragma unroll
+        for (int i = 0; i < kInt8Held / 256; ++i) {
+            const int k = i * 256 + lane * 4;
+            if (i * 256 < K && k < Kp) *reinterpret_cast<unsigned*>(smem + r * Kp + (((k >> 4) ^ (r & 7)) << 4) + (k & 15)) = int8_codes4(v[i], inv);
         }
     }
-    const int n = n0 + wn + r;
-    if (n >= N) return;
-    const float t = p.ws[bz][n], bias = p.b[bz] ? p.b[bz][n] : 0.f;
-    Y* y = reinterpret_cast<Y*>(p.y[bz]);
+    __syncthreads();
+    i32x4 acc = {0, 0, 0, 0};
+    const int r = lane & 15;                    // (rows beyond M hold whatever was there: they reach outputs beyond M only)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const int m = m0 + wm + (e & 3) + 8 * (e >> 2) + 4 * h;
-        if (m < M) int8_store(y + (int64_t)m * ldy + n, int8_scale(acc[e], p.xs[bz][m], t, bias, relu));
+    for (int i = 0; i < kInt8Held / 512; ++i)
+        if (wave + 8 * i < steps) {
+            const int piece = 4 * (wave + 8 * i) + (lane >> 4);
+            const i32x4 xf = *reinterpret_cast<const i32x4*>(smem + r * Kp + ((piece ^ (r & 7)) << 4));
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[i], xf, acc, 0, 0, 0);
+        }
+    __syncthreads();
+    int* red = reinterpret_cast<int*>(smem);
+    *reinterpret_cast<i32x4*>(red + wave * 256 + lane * 4) = acc;
+    __syncthreads();
+    if (tid >= 256) return;
+    const int m = tid >> 4, n = tid & 15;
+    if (m >= M || n0 + n >= N) return;
+    int sum = 0;
+#pragma unroll
+    for (int g = 0; g < 8; ++g) sum += red[g * 256 + (m + 16 * (n >> 2)) * 4 + (n & 3)];
+    int8_store(reinterpret_cast<Y*>(p.y[bz]) + m * ldy + n0 + n,
+               int8_scale(sum, sc[m], p.ws[bz][n0 + n], p.b[bz] ? p.b[bz][n0 + n] : 0.f, relu));
+}
+
+// Rows quantised before, few tiles: 16 channels x 16 RM rows per workgroup over the whole of k, split among eight waves; both
+// operands go from memory (rows: L2) straight into operand registers.  Any strides and alignments.
+template <int RM, typename Y>
+__global__ __launch_bounds__(512) void int8_split_kernel(Int8Batch p, int64_t ldx, int64_t ldw, int M, int K, int N, int relu, int64_t ldy) {
+    __shared__ __align__(16) int red[8 * RM * 256];
+    const int bz = blockIdx.z, n0 = (int)blockIdx.x * 16, m0 = (int)blockIdx.y * 16 * RM;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int wr = n0 + (lane & 15) < N ? n0 + (lane & 15) : N - 1;
+    const int8_t* w = p.W[bz] + (int64_t)wr * ldw;
+    const int8_t* x[RM];
+    i32x4 acc[RM];
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+        const int m = m0 + 16 * i + (lane & 15) < M ? m0 + 16 * i + (lane & 15) : M - 1;
+        x[i] = reinterpret_cast<const int8_t*>(p.x[bz]) + (int64_t)m * ldx;
+        acc[i] = i32x4{0, 0, 0, 0};
+    }
+#pragma unroll 4
+    for (int k = 64 * wave + 16 * (lane >> 4); k - 16 * (lane >> 4) < K; k += 512) {
+        const i32x4 wf = int8_chunk(w, k, K);
+#pragma unroll
+        for (int i = 0; i < RM; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf, int8_chunk(x[i], k, K), acc[i], 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < RM; ++i) *reinterpret_cast<i32x4*>(red + (wave * RM + i) * 256 + lane * 4) = acc[i];
+    __syncthreads();
+    for (int o = tid; o < RM * 256; o += 512) {
+        const int i = o >> 8, m = (o >> 4) & 15, n = o & 15;
+        const int row = m0 + 16 * i + m;
+        if (row >= M || n0 + n >= N) continue;
+        int sum = 0;
+#pragma unroll
+        for (int g = 0; g < 8; ++g) sum += red[(g * RM + i) * 256 + (m + 16 * (n >> 2)) * 4 + (n & 3)];
+        int8_store(reinterpret_cast<Y*>(p.y[bz]) + (int64_t)row * ldy + n0 + n,
+                   int8_scale(sum, p.xs[bz][row], p.ws[bz][n0 + n], p.b[bz] ? p.b[bz][n0 + n] : 0.f, relu));
     }
 }
+
+__device__ __forceinline__ void int8_glds16(const void* gsrc_lane, void* lds_wave_base) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)gsrc_lane,
+                                     (__attribute__((address_space(3))) void*)lds_wave_base, 16, 0, 0);
+}
+
+__device__ __attribute__((aligned(16))) const int int8_zeros[4] = {0, 0, 0, 0};
+
+// Tiles of BM x BN outputs, WVM x WVN waves, k in stages of 128 bytes through two LDS buffers: the copies of a stage go
+// straight from memory into LDS while the products of the one before run, one barrier a stage.  Rows of both operands
+// start at multiples of 16 bytes and K is a multiple of 16 (zeros behind the features).  A row's 128 bytes of a stage
+// lie in LDS with 16-byte piece c at place c ^ (row & 7): copies stay linear in LDS (each lane picks its source), and the
+// eight rows of a fragment's read phase lie in different banks.
+template <int BM, int BN, int WVM, int WVN, typename Y>
+__global__ __launch_bounds__(WVM * WVN * 64) void int8_tile_kernel(Int8Batch p, int64_t ldx, int64_t ldw, int M, int K, int N, int relu, int64_t ldy) {
+    constexpr int WV = WVM * WVN, TM = BM / WVM / 32, TN = BN / WVN / 32;
+    constexpr int UA = BM / 8, UB = BN / 8, PER = (UA + UB) / WV;      // units of 8 rows x 128 bytes
+    constexpr int STAGE = (BM + BN) * 128;
+    static_assert(TM >= 1 && TN >= 1 && (UA + UB) % WV == 0, "tile");
+    extern __shared__ __align__(16) int8_t smem[];
+    const int bz = blockIdx.y;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int nx = (N + BN - 1) / BN, ny = (M + BM - 1) / BM;
+    int tx, ty;
+    xcd_tile((int)blockIdx.x, nx, ny, tx, ty);
+    const int m0 = ty * BM, n0 = tx * BN;
+
+    const int8_t* src[PER];
+    const int piece = (lane & 7) ^ (lane >> 3);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int u = wave + WV * i;
+        const int row = (u < UA ? m0 + u * 8 : n0 + (u - UA) * 8) + (lane >> 3);
+        src[i] = u < UA ? reinterpret_cast<const int8_t*>(p.x[bz]) + (int64_t)(row < M ? row : M - 1) * ldx + piece * 16
+                        : p.W[bz] + (int64_t)(row < N ? row : N - 1) * ldw + piece * 16;
+    }
+    auto issue = [&](int st) {
+        int8_t* dst = smem + (st & 1) * STAGE + wave * 1024;
+        const int k0 = st * 128;
+        if (k0 + 128 <= K) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) int8_glds16(src[i] + k0, dst + i * WV * 1024);
+        } else {
+            const bool in = k0 + piece * 16 < K;
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                int8_glds16(in ? static_cast<const void*>(src[i] + k0) : static_cast<const void*>(int8_zeros), dst + i * WV * 1024);
+        }
+    };
+
+    const int wm = (wave / WVN) * (BM / WVM), wn = (wave % WVN) * (BN / WVN);
+    const int r = lane & 31, h = lane >> 5;
+    i32x16 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+    const int stages = (K + 127) / 128;
+    issue(0);
+    for (int st = 0; st < stages; ++st) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // own copies of this stage have landed
+        __syncthreads();                                     // everyone's have, and everyone is done with the other buffer
+        if (st + 1 < stages) issue(st + 1);
+        const int8_t* sa = smem + (st & 1) * STAGE + (wm + r) * 128;
+        const int8_t* sb = smem + (st & 1) * STAGE + (BM + wn + r) * 128;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            const int at = ((2 * kk + h) ^ (r & 7)) << 4;
+            i32x4 fa[TM], fb[TN];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) fa[i] = *reinterpret_cast<const i32x4*>(sa + i * 32 * 128 + at);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) fb[j] = *reinterpret_cast<const i32x4*>(sb + j * 32 * 128 + at);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fb[j], acc[i][j], 0, 0, 0);
+        }
+    }
+    Y* y = reinterpret_cast<Y*>(p.y[bz]);
+    const float* xs = p.xs[bz];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int n = n0 + wn + 32 * j + r;
+        if (n >= N) continue;
+        const float t = p.ws[bz][n], bias = p.b[bz] ? p.b[bz][n] : 0.f;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int m = m0 + wm + 32 * i + (e & 3) + 8 * (e >> 2) + 4 * h;
+                if (m < M) int8_store(y + (int64_t)m * ldy + n, int8_scale(acc[i][j][e], xs[m], t, bias, relu));
+            }
+    }
+}
+
+template <int BM, int BN, int WVM, int WVN, typename Y>
+static int int8_tiles(const Int8Batch& p, int n_batch, int64_t ldx, int64_t ldw, int M, int K, int N, int relu, int64_t ldy, hipStream_t st) {
+    auto kern = int8_tile_kernel<BM, BN, WVM, WVN, Y>;
+    const size_t lds = 2 * (BM + BN) * 128;
+    if (int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), lds, "linear_int8")) return rc;
+    const int64_t tiles = (int64_t)((M + BM - 1) / BM) * ((N + BN - 1) / BN);
+    if (tiles > 0x7FFFFFFF) return fail(DVQ_EINVAL, "linear_int8: M x N too large");
+    hipLaunchKernelGGL(kern, dim3((unsigned)tiles, (unsigned)n_batch), dim3(WVM * WVN * 64), lds, st, p, ldx, ldw, M, K, N, relu, ldy);
+    return check_launch("linear_int8");
+}
+
+static inline int64_t tile_count(int M, int N, int b, int n_batch) { return (int64_t)((M + b - 1) / b) * ((N + b - 1) / b) * n_batch; }
+
+// The product of rows that are codes already (p.x); `aligned`: rows of both operands at multiples of 16 bytes, K % 16 == 0.
+template <typename Y>
+static int int8_product(const Int8Batch& p, int n_batch, int64_t ldx, int64_t ldw, int M, int K, int N, int relu, int64_t ldy, bool aligned,
+                        hipStream_t st) {
+    if (!aligned || tile_count(M, N, 64, n_batch) < kInt8SplitBelow) {
+        const dim3 blk(512);
+        const unsigned gx = (unsigned)((N + 15) / 16);
+        if (M <= 16) hipLaunchKernelGGL((int8_split_kernel<1, Y>), dim3(gx, 1, n_batch), blk, 0, st, p, ldx, ldw, M, K, N, relu, ldy);
+        else if (M <= 32) hipLaunchKernelGGL((int8_split_kernel<2, Y>), dim3(gx, 1, n_batch), blk, 0, st, p, ldx, ldw, M, K, N, relu, ldy);
+        else hipLaunchKernelGGL((int8_split_kernel<4, Y>), dim3(gx, (M + 63) / 64, n_batch), blk, 0, st, p, ldx, ldw, M, K, N, relu, ldy);
+        return check_launch("linear_int8");
+    }
+    if (tile_count(M, N, 256, n_batch) >= 224) return int8_tiles<256, 256, 2, 4, Y>(p, n_batch, ldx, ldw, M, K, N, relu, ldy, st);
+    if (tile_count(M, N, 128, n_batch) >= 192) return int8_tiles<128, 128, 2, 2, Y>(p, n_batch, ldx, ldw, M, K, N, relu, ldy, st);
+    return int8_tiles<64, 64, 2, 2, Y>(p, n_batch, ldx, ldw, M, K, N, relu, ldy, st);
+}
+
+static bool aligned16(const void* const* ptrs, int n, int64_t ld) {
+    if (ld % 16) return false;
+    for (int i = 0; i < n; ++i)
+        if (reinterpret_cast<uintptr_t>(ptrs[i]) % 16) return false;
+    return true;
+}
+
+static inline int64_t int8_ld(int K) { return (K + 63) / 64 * 64; }
+static inline int64_t int8_each(int rows, int K) { return rows * int8_ld(K) + (rows * (int64_t)4 + 15) / 16 * 16; }
 
 }  // namespace dvq
 
 using namespace dvq;
 
-extern "C" int dvq_int8_quantize_rows(int n_batch, const void* const* x, int dtype, int64_t ldx, int M, int K, void* const* codes,
-                                      int64_t ldc, float* const* scale, void* stream) {
-    if (n_batch < 1 || n_batch > kInt8MaxBatch) return fail(DVQ_EINVAL, "int8_quantize_rows: 1..%d matrices per launch", kInt8MaxBatch);
+// Rows of a float matrix at a time quantised by each workgroup for itself: no workspace, one launch.
+static bool int8_one_launch(int M, int K) { return M <= 16 && K <= kInt8Held; }
+
+extern "C" size_t dvq_linear_int8_workspace_bytes(int n_batch, int M, int K, int N) {
+    if (n_batch < 1 || M < 1 || K < 1 || N < 1) return 0;
+    return (size_t)n_batch * (size_t)(int8_each(M, K) + (int64_t)N * int8_ld(K));
+}
+
+extern "C" int dvq_int8_quantize_rows(const void* x, int dtype, int64_t ldx, int M, int K, void* codes, int64_t ldc, float* scale, void* stream) {
     if (dtype != DVQ_F32 && dtype != DVQ_BF16) return fail(DVQ_EINVAL, "int8_quantize_rows: dtype must be DVQ_F32 or DVQ_BF16");
-    if (M < 0 || K < 1 || K >= (1 << 17) || ldx < 0 || ldc < K || (ldc % 16) != 0)
+    if (M < 0 || K < 1 || K >= (1 << 17) || ldx < 0 || ldc < K || (ldc % 16) != 0 || ldc > (1 << 30))
         return fail(DVQ_EINVAL, "int8_quantize_rows: M >= 0, 1 <= K < 2^17, ldc >= K a multiple of 16 (got M = %d, K = %d, ldc = %lld)", M, K, (long long)ldc);
     if (M == 0) return DVQ_OK;
-    if (!x || !codes || !scale) return fail(DVQ_EINVAL, "int8_quantize_rows: null pointer");
-    QuantBatch p;
-    for (int i = 0; i < n_batch; ++i) {
-        if (!x[i] || !codes[i] || !scale[i]) return fail(DVQ_EINVAL, "int8_quantize_rows: null pointer");
-        p.x[i] = x[i]; p.codes[i] = reinterpret_cast<int8_t*>(codes[i]); p.scale[i] = scale[i];
-    }
-    const dim3 grid((unsigned)M, (unsigned)n_batch);
-    if (dtype == DVQ_F32) hipLaunchKernelGGL(int8_quantize_kernel<float>, grid, dim3(256), 0, as_stream(stream), p, ldx, K, ldc);
-    else hipLaunchKernelGGL(int8_quantize_kernel<unsigned short>, grid, dim3(256), 0, as_stream(stream), p, ldx, K, ldc);
+    if (!x || !codes || !scale || reinterpret_cast<uintptr_t>(codes) % 16) return fail(DVQ_EINVAL, "int8_quantize_rows: null or unaligned pointer");
+    Int8Prepare p = {};
+    p.x[0] = x; p.codes[0] = reinterpret_cast<int8_t*>(codes); p.scale[0] = scale;
+    if (dtype == DVQ_F32) hipLaunchKernelGGL(int8_prepare_kernel<float>, dim3((unsigned)M, 1), dim3(64), 0, as_stream(stream), p, ldx, 0, M, K, ldc);
+    else hipLaunchKernelGGL(int8_prepare_kernel<unsigned short>, dim3((unsigned)M, 1), dim3(64), 0, as_stream(stream), p, ldx, 0, M, K, ldc);
     return check_launch("int8_quantize_rows");
 }
 
-extern "C" int dvq_linear_int8(int n_batch, const void* const* x, const float* const* xs, int64_t ldx, const void* const* W,
+extern "C" int dvq_linear_int8(int n_batch, const void* const* x, int x_dtype, const float* const* xs, int64_t ldx, const void* const* W,
                                const float* const* ws, int64_t ldw, const float* const* b, int M, int K, int N, int relu,
-                               void* const* y, int y_dtype, int64_t ldy, void* stream) {
+                               void* const* y, int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
     if (n_batch < 1 || n_batch > kInt8MaxBatch) return fail(DVQ_EINVAL, "linear_int8: 1..%d products per launch", kInt8MaxBatch);
+    if (x_dtype != DVQ_F32 && x_dtype != DVQ_BF16 && x_dtype != DVQ_I8) return fail(DVQ_EINVAL, "linear_int8: x_dtype must be DVQ_F32, DVQ_BF16 or DVQ_I8");
     if (y_dtype != DVQ_F32 && y_dtype != DVQ_BF16) return fail(DVQ_EINVAL, "linear_int8: y_dtype must be DVQ_F32 or DVQ_BF16");
     if (M < 0 || N < 1 || K < 1 || K >= (1 << 17)) return fail(DVQ_EINVAL, "linear_int8: M >= 0, N >= 1, 1 <= K < 2^17 (got M = %d, N = %d, K = %d)", M, N, K);
     if (ldx < 0 || ldw < 0 || ldy < N) return fail(DVQ_EINVAL, "linear_int8: bad row stride");
+    if (M > 0x7FFFFFFF - N) return fail(DVQ_EINVAL, "linear_int8: M + N must stay below 2^31");
     if (M == 0) return DVQ_OK;
-    if (!x || !xs || !W || !ws || !y) return fail(DVQ_EINVAL, "linear_int8: null pointer");
-    Int8Batch p;
+    const bool codes = x_dtype == DVQ_I8;
+    if (!x || !W || !ws || !y || (codes && !xs)) return fail(DVQ_EINVAL, "linear_int8: null pointer");
+    for (int i = 0; i < n_batch; ++i)
+        if (!x[i] || !W[i] || !ws[i] || !y[i] || (codes && !xs[i])) return fail(DVQ_EINVAL, "linear_int8: null pointer");
+    Int8Batch p = {};
     for (int i = 0; i < n_batch; ++i) {
-        if (!x[i] || !xs[i] || !W[i] || !ws[i] || !y[i]) return fail(DVQ_EINVAL, "linear_int8: null pointer");
-        p.x[i] = reinterpret_cast<const int8_t*>(x[i]); p.xs[i] = xs[i];
+        p.x[i] = x[i]; p.xs[i] = codes ? xs[i] : nullptr;
         p.W[i] = reinterpret_cast<const int8_t*>(W[i]); p.ws[i] = ws[i];
         p.b[i] = b ? b[i] : nullptr;
         p.y[i] = y[i];
     }
-    const int64_t tiles = (int64_t)((M + 63) / 64) * ((N + 63) / 64);
-    if (tiles > 0x7FFFFFFF) return fail(DVQ_EINVAL, "linear_int8: M x N too large");
-    const dim3 grid((unsigned)tiles, (unsigned)n_batch);
-    if (y_dtype == DVQ_F32) hipLaunchKernelGGL(int8_any_kernel<float>, grid, dim3(256), 0, as_stream(stream), p, ldx, ldw, M, K, N, relu, ldy);
-    else hipLaunchKernelGGL(int8_any_kernel<unsigned short>, grid, dim3(256), 0, as_stream(stream), p, ldx, ldw, M, K, N, relu, ldy);
-    return check_launch("linear_int8");
+    hipStream_t st = as_stream(stream);
+    const bool f32 = y_dtype == DVQ_F32;
+    if (!codes && int8_one_launch(M, K)) {
+        const int Kp = (K + 127) / 128 * 128;
+        const size_t lds = (size_t)16 * Kp > 8192 ? (size_t)16 * Kp : 8192;      // <= 64 KiB
+        const dim3 grid((unsigned)((N + 15) / 16), (unsigned)n_batch), blk(512);
+        if (x_dtype == DVQ_F32) {
+            if (f32) hipLaunchKernelGGL((int8_rows16_kernel<float, float>), grid, blk, lds, st, p, ldx, ldw, M, K, N, relu, ldy);
+            else hipLaunchKernelGGL((int8_rows16_kernel<float, unsigned short>), grid, blk, lds, st, p, ldx, ldw, M, K, N, relu, ldy);
+        } else {
+            if (f32) hipLaunchKernelGGL((int8_rows16_kernel<unsigned short, float>), grid, blk, lds, st, p, ldx, ldw, M, K, N, relu, ldy);
+            else hipLaunchKernelGGL((int8_rows16_kernel<unsigned short, unsigned short>), grid, blk, lds, st, p, ldx, ldw, M, K, N, relu, ldy);
+        }
+        return check_launch("linear_int8");
+    }
+    // What the tiles cannot read in place -- features to quantise, rows that do not start at multiples of 16 bytes -- is
+    // laid out in the workspace by one launch.
+    const bool tiles = tile_count(M, N, 64, n_batch) >= kInt8SplitBelow;
+    const bool wide = K % 16 == 0;
+    const bool copy_w = tiles && !(wide && aligned16(W, n_batch, ldw));
+    const bool copy_x = !codes || (tiles && !(wide && aligned16(x, n_batch, ldx)));
+    int Kt = K;
+    if (copy_w || copy_x) {
+        const size_t need = dvq_linear_int8_workspace_bytes(n_batch, M, K, N);
+        if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
+            return fail(DVQ_EINVAL, "linear_int8: needs a 16-byte aligned workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : 0);
+        Int8Prepare q = {};
+        int8_t* base = reinterpret_cast<int8_t*>(workspace);
+        const int64_t ldc = int8_ld(K);
+        for (int i = 0; i < n_batch; ++i) {
+            q.x[i] = p.x[i]; q.W[i] = p.W[i];
+            q.codes[i] = base; q.scale[i] = reinterpret_cast<float*>(base + M * ldc);
+            base += int8_each(M, K);
+            q.w_codes[i] = base;
+            base += N * ldc;
+            if (copy_x) { p.x[i] = q.codes[i]; if (!codes) p.xs[i] = q.scale[i]; }
+            if (copy_w) p.W[i] = q.w_codes[i];
+        }
+        const int rows = copy_x ? M : 0;
+        const dim3 grid((unsigned)(rows + (copy_w ? N : 0)), (unsigned)n_batch);
+        if (x_dtype == DVQ_F32) hipLaunchKernelGGL(int8_prepare_kernel<float>, grid, dim3(64), 0, st, q, ldx, ldw, rows, K, ldc);
+        else if (x_dtype == DVQ_BF16) hipLaunchKernelGGL(int8_prepare_kernel<unsigned short>, grid, dim3(64), 0, st, q, ldx, ldw, rows, K, ldc);
+        else hipLaunchKernelGGL(int8_prepare_kernel<int8_t>, grid, dim3(64), 0, st, q, ldx, ldw, rows, K, ldc);
+        if (int rc = check_launch("linear_int8")) return rc;
+        if (copy_x) ldx = ldc;
+        if (copy_w) ldw = ldc;
+        if (tiles) Kt = (K + 15) / 16 * 16;             // (zeros behind the features)
+    }
+    return f32 ? int8_product<float>(p, n_batch, ldx, ldw, M, Kt, N, relu, ldy, tiles, st)
+               : int8_product<unsigned short>(p, n_batch, ldx, ldw, M, Kt, N, relu, ldy, tiles, st);
 }

@@ -15,6 +15,7 @@ LIB_PATH = os.environ.get("DVQ_HIP_LIB") or os.path.join(os.path.dirname(_HERE),
 
 DVQ_F32 = 0
 DVQ_BF16 = 1
+DVQ_I8 = 2
 
 
 class DvqPointMlp(ctypes.Structure):
@@ -92,10 +93,11 @@ SIGNATURES = {
                                    c_int, c_int, POINTER(c_void_p), c_int64, c_int, c_void_p]),
     "dvq_to_bf16": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "dvq_linear_bf16": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p]),
-    "dvq_int8_quantize_rows": (c_int, [c_int, POINTER(c_void_p), c_int, c_int64, c_int, c_int, POINTER(c_void_p), c_int64,
-                                       POINTER(c_void_p), c_void_p]),
-    "dvq_linear_int8": (c_int, [c_int, POINTER(c_void_p), POINTER(c_void_p), c_int64, POINTER(c_void_p), POINTER(c_void_p), c_int64,
-                                POINTER(c_void_p), c_int, c_int, c_int, c_int, POINTER(c_void_p), c_int, c_int64, c_void_p]),
+    "dvq_int8_quantize_rows": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p]),
+    "dvq_linear_int8_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "dvq_linear_int8": (c_int, [c_int, POINTER(c_void_p), c_int, POINTER(c_void_p), c_int64, POINTER(c_void_p), POINTER(c_void_p), c_int64,
+                                POINTER(c_void_p), c_int, c_int, c_int, c_int, POINTER(c_void_p), c_int, c_int64, c_void_p, c_size_t,
+                                c_void_p]),
     "dvq_prior_verify": (c_int, [POINTER(DvqPriorVerify), c_void_p]),
     "dvq_prior_packed_bytes": (c_size_t, [c_int, c_int, c_int]),
     "dvq_prior_pack_weight": (c_int, [c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_void_p]),

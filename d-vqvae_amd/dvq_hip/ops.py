@@ -12,7 +12,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import DVQ_BF16, DVQ_F32, DvqHandMesh, DvqManoConsts, DvqPointMlp, DvqPriorGather, DvqPriorJob, DvqPriorVerify, DvqPriorVRow
+from ._lib import DVQ_BF16, DVQ_F32, DVQ_I8, DvqHandMesh, DvqManoConsts, DvqPointMlp, DvqPriorGather, DvqPriorJob, DvqPriorVerify, DvqPriorVRow
 
 
 # Optional per-kernel timing with HIP events on the launch stream (used by bench.py for the
@@ -363,40 +363,23 @@ def _vector(t: torch.Tensor, what: str, n: int, dev) -> None:
         raise RuntimeError(f"{what} must be a contiguous float32 [{n}] on {dev}")
 
 
-def _quantize(xs, what: str):
-    """Codes and scales of matrices of one shape, type and row stride, one launch: (list of code pointers, their row
-    stride, list of scale pointers, the buffer that holds them)."""
-    x0 = xs[0]
-    ldx = _rows(x0, what, (torch.float32, torch.bfloat16))
-    M, K = x0.shape
-    for x in xs[1:]:
-        if _rows(x, what, (x0.dtype,), x0.device) != ldx or x.shape != x0.shape:
-            raise RuntimeError(f"{what}: all matrices must have one shape, type and row stride")
-    if not 1 <= K <= INT8_MAX_K:
-        raise RuntimeError(f"{what}: 1..{INT8_MAX_K} features per row, got {K}")
-    n, ldc = len(xs), (K + 63) // 64 * 64
-    each = M * ldc + (M * 4 + 15) // 16 * 16
-    buf = torch.empty(n * each, dtype=torch.uint8, device=x0.device)
-    base = buf.data_ptr()
-    codes = [base + i * each for i in range(n)]
-    scales = [c + M * ldc for c in codes]
-    if M > 0:
-        arr = ctypes.c_void_p * n
-        _launch(_lib.load().dvq_int8_quantize_rows, "dvq_int8_quantize_rows", x0.device, n, arr(*[x.data_ptr() for x in xs]),
-                _dtype_code(x0), ldx, M, K, arr(*codes), ldc, arr(*scales))
-    return codes, ldc, scales, buf
-
-
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """(codes int8 [M,K], scale float32 [M]) of the rows of x [M,K] (float32 or bfloat16, unit inner stride): a = max|x|,
     code = 127 x / a rounded to the nearest whole number (ties to even, of the exact quotient), scale = a / 127.  A row of
     zeros has codes and scale 0; a row with an infinity or a NaN has codes 0 and scale NaN.  Rows of activations (a scale
-    per token) and of weights [N,K] (a scale per output channel) are quantised alike."""
-    if x.dim() != 2:
-        raise RuntimeError(f"quantize_rows: x must be 2-D, got {tuple(x.shape)}")
+    per token) and of weights [N,K] (a scale per output channel) are quantised alike.  The rows of the codes start at
+    multiples of 64 bytes, where linear_int8 reads them in place."""
+    ldx = _rows(x, "quantize_rows: x", (torch.float32, torch.bfloat16))
     M, K = x.shape
-    _, ldc, _, buf = _quantize([x], "quantize_rows: x")
-    return buf[:M * ldc].view(torch.int8).view(M, ldc)[:, :K], buf[M * ldc:M * ldc + 4 * M].view(torch.float32)
+    if not 1 <= K <= INT8_MAX_K:
+        raise RuntimeError(f"quantize_rows: 1..{INT8_MAX_K} features per row, got {K}")
+    ldc = (K + 63) // 64 * 64
+    codes = torch.empty(M, ldc, dtype=torch.int8, device=x.device)
+    scale = torch.empty(M, dtype=torch.float32, device=x.device)
+    if M > 0:
+        _launch(_lib.load().dvq_int8_quantize_rows, "dvq_int8_quantize_rows", x.device, x.data_ptr(), _dtype_code(x), ldx, M, K,
+                codes.data_ptr(), ldc, scale.data_ptr())
+    return codes[:, :K], scale
 
 
 def linear_int8(x, W: torch.Tensor, w_scale: torch.Tensor, b: Optional[torch.Tensor] = None, relu: bool = False,
@@ -425,28 +408,25 @@ def _linear_int8(xs, Ws, w_scales, bs, relu, out, out_dtype, what):
         raise RuntimeError(f"{what}: either all x are quantised already or none")
     if out_dtype not in (torch.float32, torch.bfloat16):
         raise RuntimeError(f"{what}: output of float32 or bfloat16, not {out_dtype}")
-    first = xs[0][0] if pairs else xs[0]
-    dev = first.device
-    keep = None
-    if pairs:
-        ldx = _rows(first, f"{what}: codes", (torch.int8,))
-        for c, s in xs:
-            if _rows(c, f"{what}: codes", (torch.int8,), dev) != ldx or c.shape != first.shape:
-                raise RuntimeError(f"{what}: all x must have one shape and row stride")
-            _vector(s, f"{what}: the scale of x", first.shape[0], dev)
-    elif first.dim() != 2:
-        raise RuntimeError(f"{what}: x must be 2-D, got {tuple(first.shape)}")
+    feats, scales = [x[0] for x in xs] if pairs else xs, [x[1] for x in xs] if pairs else [None] * len(xs)
+    first = feats[0]
+    ldx = _rows(first, f"{what}: x", (torch.int8,) if pairs else (torch.float32, torch.bfloat16))
     M, K = first.shape
-    ldw = _rows(Ws[0], f"{what}: W", (torch.int8,), dev)
-    N = Ws[0].shape[0]
-    for W, s, b in zip(Ws, w_scales, bs):
-        if _rows(W, f"{what}: W", (torch.int8,), dev) != ldw or W.shape != (N, K):
-            raise RuntimeError(f"{what}: W must be int8 [{N},{K}] (all of one row stride), got {tuple(W.shape)}")
-        _vector(s, f"{what}: w_scale", N, dev)
-        if b is not None:
-            _vector(b, f"{what}: b", N, dev)
+    dev = first.device
     if not 1 <= K <= INT8_MAX_K:
         raise RuntimeError(f"{what}: 1..{INT8_MAX_K} features per row, got {K}")
+    ldw = _rows(Ws[0], f"{what}: W", (torch.int8,), dev)
+    N = Ws[0].shape[0]
+    for x, sx, W, sw, b in zip(feats, scales, Ws, w_scales, bs):
+        if x is not first and (_rows(x, f"{what}: x", (first.dtype,), dev) != ldx or x.shape != first.shape):
+            raise RuntimeError(f"{what}: all x must have one shape, type and row stride")
+        if sx is not None:
+            _vector(sx, f"{what}: the scale of x", M, dev)
+        if _rows(W, f"{what}: W", (torch.int8,), dev) != ldw or W.shape != (N, K):
+            raise RuntimeError(f"{what}: W must be int8 [{N},{K}] (all of one row stride), got {tuple(W.shape)}")
+        _vector(sw, f"{what}: w_scale", N, dev)
+        if b is not None:
+            _vector(b, f"{what}: b", N, dev)
     if out is not None:
         ldy = _rows(out, f"{what}: out", (torch.float32, torch.bfloat16), dev)
         if out.shape != (M, N) or ldy < N:
@@ -461,15 +441,15 @@ def _linear_int8(xs, Ws, w_scales, bs, relu, out, out_dtype, what):
         return outs
     n = len(xs)
     arr = ctypes.c_void_p * n
-    if pairs:
-        codes, scales = [c.data_ptr() for c, _ in xs], [s.data_ptr() for _, s in xs]
-    else:
-        codes, ldx, scales, keep = _quantize(xs, f"{what}: x")
-    _launch(_lib.load().dvq_linear_int8, "dvq_linear_int8", dev, n, arr(*codes), arr(*scales), ldx,
-            arr(*[W.data_ptr() for W in Ws]), arr(*[s.data_ptr() for s in w_scales]), ldw,
-            arr(*[None if b is None else b.data_ptr() for b in bs]), M, K, N, int(relu), arr(*[o.data_ptr() for o in outs]),
-            _dtype_code(outs[0]), ldy)
-    del keep             # (the codes; the allocator hands them out again only to later work of this stream)
+    lib = _lib.load()
+    ws, nbytes = None, 0
+    if pairs or M > 16 or K > 4096:          # (few rows of floats: one launch without a workspace)
+        nbytes = lib.dvq_linear_int8_workspace_bytes(n, M, K, N)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch(lib.dvq_linear_int8, "dvq_linear_int8", dev, n, arr(*[x.data_ptr() for x in feats]), DVQ_I8 if pairs else _dtype_code(first),
+            arr(*[s.data_ptr() for s in scales]) if pairs else None, ldx, arr(*[W.data_ptr() for W in Ws]),
+            arr(*[s.data_ptr() for s in w_scales]), ldw, arr(*[None if b is None else b.data_ptr() for b in bs]), M, K, N, int(relu),
+            arr(*[o.data_ptr() for o in outs]), _dtype_code(outs[0]), ldy, _p(ws), nbytes)
     return outs
 
 

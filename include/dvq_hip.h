@@ -34,6 +34,7 @@ extern "C" {
 
 #define DVQ_F32 0
 #define DVQ_BF16 1
+#define DVQ_I8 2      /* 8-bit codes with a scale per row (dvq_linear_int8) */
 
 #define DVQ_VERSION 114   /* major*10000 + minor*100 + patch */
 
@@ -368,15 +369,18 @@ int dvq_prior_uniforms(int64_t first_id, int64_t n, int n_cells, uint64_t seed, 
  *   a = 0: codes and scale 0; a row with an infinity or a NaN: codes 0, scale NaN.
  * codes: int8 [M, ldc], ldc % 16 == 0, K <= ldc; bytes K .. ldc-1 of a row are set to zero.  scale: fp32 [M].
  *
- * dvq_linear_int8: y[m,n] = act( (sum_k x[m,k] W[n,k]) xs[m] ws[n] + b[n] ), the sum exact in 32-bit integers, the rest in
- *   fp32, rounded once to `y_dtype`.  x: int8 [M,K] with row stride ldx, W: int8 [N,K] with row stride ldw (strides in
- *   bytes, any alignment), b nullable.  K < 2^17.  act: relu keeps a NaN.
- * Both take host arrays of n_batch (1..8) device pointers: products of ONE shape as one launch. */
-int dvq_int8_quantize_rows(int n_batch, const void* const* x, int dtype, int64_t ldx, int M, int K, void* const* codes,
-                           int64_t ldc, float* const* scale, void* stream);
-int dvq_linear_int8(int n_batch, const void* const* x, const float* const* xs, int64_t ldx, const void* const* W,
+ * dvq_linear_int8: y[m,n] = act( (sum_k c[m,k] W[n,k]) s[m] ws[n] + b[n] ), the sum exact in 32-bit integers, scaled in 64
+ *   bits and rounded once to `y_dtype`.  x: [M,K] of x_dtype DVQ_F32 or DVQ_BF16 (c, s: as above, made in the call; xs is
+ *   ignored) or DVQ_I8 (c = x, s = xs); row strides in elements, any alignment of the element.  W: int8 [N,K], b nullable.
+ *   K < 2^17.  act: relu keeps a NaN.  y must not overlap x.
+ *   x, xs, W, ws, b, y: host arrays of n_batch (1..8) device pointers, products of ONE shape in the same launches.
+ *   workspace: dvq_linear_int8_workspace_bytes() bytes, 16-byte aligned; not touched (may be NULL) for M <= 16 rows of floats
+ *   with K <= 4096, and for DVQ_I8 with rows of x and W at multiples of 16 bytes and K % 16 == 0. */
+int dvq_int8_quantize_rows(const void* x, int dtype, int64_t ldx, int M, int K, void* codes, int64_t ldc, float* scale, void* stream);
+size_t dvq_linear_int8_workspace_bytes(int n_batch, int M, int K, int N);
+int dvq_linear_int8(int n_batch, const void* const* x, int x_dtype, const float* const* xs, int64_t ldx, const void* const* W,
                     const float* const* ws, int64_t ldw, const float* const* b, int M, int K, int N, int relu,
-                    void* const* y, int y_dtype, int64_t ldy, void* stream);
+                    void* const* y, int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------- verification of drafted codes
  * What a drafting model proposed for the prior (models.py:161-198): row b brings n = lengths[b] (NULL: G) codes

@@ -54,28 +54,36 @@ def test_verification_oracle_keeps_the_target_distribution():
     assert np.all(np.abs(np.bincount(first, minlength=V) / B - p) <= 5 * np.sqrt(p * (1 - p) / B))
 
 
-def _quantize(lib, n=1, M=4, K=16, ldc=16, dtype=0, ldx=16, ptr=16):
+def _quantize(lib, M=4, K=16, ldc=16, dtype=0, ldx=16, ptr=16, codes=16):
+    return lib.dvq_int8_quantize_rows(ptr, dtype, ldx, M, K, codes, ldc, ptr, None)
+
+
+def _product(lib, n=1, M=4, K=16, N=4, ldx=16, ldw=16, ldy=4, x_dtype=0, y_dtype=0, ptr=16, xs=True, ws=16, nbytes=1 << 40):
     arr = (VP * 8)(*[ptr] * 8)
-    return lib.dvq_int8_quantize_rows(n, arr, dtype, ldx, M, K, arr, ldc, arr, None)
+    return lib.dvq_linear_int8(n, arr, x_dtype, arr if xs else None, ldx, arr, arr, ldw, None, M, K, N, 0, arr, y_dtype, ldy, ws, nbytes, None)
 
 
-def _product(lib, n=1, M=4, K=16, N=4, ldx=16, ldw=16, ldy=4, y_dtype=0, ptr=16):
-    arr = (VP * 8)(*[ptr] * 8)
-    return lib.dvq_linear_int8(n, arr, arr, ldx, arr, arr, ldw, None, M, K, N, 0, arr, y_dtype, ldy, None)
-
-
-@pytest.mark.parametrize("bad", [dict(n=0), dict(n=9), dict(K=0), dict(K=1 << 17, ldc=1 << 17), dict(ldc=24), dict(K=17), dict(M=-1),
-                                 dict(dtype=2), dict(ptr=None), dict(ldx=-1)])
+@pytest.mark.parametrize("bad", [dict(K=0), dict(K=1 << 17, ldc=1 << 17), dict(ldc=24), dict(K=17), dict(M=-1), dict(dtype=2), dict(ptr=None),
+                                 dict(codes=8), dict(ldx=-1)])
 def test_quantize_refusals(bad):
     lib = _lib.load()
     assert _quantize(lib, **bad) == -1 and lib.dvq_last_error()
 
 
-@pytest.mark.parametrize("bad", [dict(n=0), dict(n=9), dict(K=0), dict(K=1 << 17), dict(M=-1), dict(N=0), dict(y_dtype=3), dict(ldy=3),
-                                 dict(ldx=-1), dict(ldw=-1), dict(ptr=None)])
+@pytest.mark.parametrize("bad", [dict(n=0), dict(n=9), dict(K=0), dict(K=1 << 17), dict(M=-1), dict(N=0), dict(x_dtype=3), dict(y_dtype=2), dict(ldy=3),
+                                 dict(ldx=-1), dict(ldw=-1), dict(ptr=None), dict(x_dtype=2, xs=False), dict(M=0x7FFFFFFF),
+                                 dict(M=20, ws=None), dict(M=20, ws=8), dict(M=20, nbytes=20 * 64 + 80 + 4 * 64 - 1), dict(K=4097, ws=None),
+                                 dict(n=2, M=20, nbytes=20 * 64 + 80 + 4 * 64)])
 def test_product_refusals(bad):
     lib = _lib.load()
     assert _product(lib, **bad) == -1 and lib.dvq_last_error()
+
+
+def test_workspace_of_the_product():
+    size = _lib.load().dvq_linear_int8_workspace_bytes
+    assert size(1, 20, 16, 4) == 20 * 64 + 80 + 4 * 64 and size(3, 20, 16, 4) == 3 * size(1, 20, 16, 4)
+    assert size(1, 0, 16, 4) == 0 and size(0, 20, 16, 4) == 0
+    assert size(8, 1 << 20, 1 << 16, 1 << 16) == 8 * ((1 << 36) + (1 << 22) + (1 << 32))
 
 
 def _verify_args(**kw):
