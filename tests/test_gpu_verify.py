@@ -184,7 +184,7 @@ def test_first_and_last_uniforms(V):
     check(c)
 
 
-@pytest.mark.parametrize("V", [70, 512, 5000])
+@pytest.mark.parametrize("V", [70, 512, 900, 5000, 20000])
 def test_strides(V):
     """The prior's [B, V, cells] layout, slices, every second row, broadcast uniforms and drafts, columns of wider buffers."""
     c = make(14, 4, 5, V, seed=3)
@@ -201,7 +201,12 @@ def test_strides(V):
         wide = torch.full((2 * v.shape[0], *v.shape[1:]), 1, dtype=v.dtype, device=DEV)
         wide[::2] = v
         return wide[::2]
-    for place in (cells, inside, spread):
+    def target_cells(k, v):
+        return cells(k, v) if k == "logits" else v
+
+    def draft_cells(k, v):
+        return cells(k, v) if k == "draft" else v
+    for place in (cells, inside, spread, target_cells, draft_cells):
         check(c, place=place)
         check(c, lengths=torch.arange(14) % 5, place=place)
     one = make(1, 4, 5, V, seed=8)
