@@ -10,11 +10,14 @@
 //   Tests: one pass over the row in 32-bit exponentials, the sums of few of them collected in 64 bits.  Their error is
 //     bounded (kVerifyMargin); a test that clears the bound is decided, one within it -- one in ten thousand -- has its
 //     sums taken again in 64 bits.
-//   Draw: one position per row, 64-bit exponentials.  The row is cut into tiles of 512 codes, one wave each; the masses
-//     of the tiles find the tile, a scan inside it the code.
+//   Draw: one position per row, 64-bit exponentials, in one pass although the weights e_p - k e_q (k = S_p / S_q) need the
+//     pass's own sums: k is known to kVerifyMargin from the test, which settles the sign of all weights but those next to
+//     zero, and with the signs settled a tile's mass is sum e_p - k sum e_q over its positive codes.  Tiles that hold a code
+//     next to zero are done again once k is known.  A tile is 512 codes, one wave; the tiles' masses find the tile, a scan
+//     inside it the code.
 // Three forms: rows of up to 1024 codes stay in the registers of one wave per position; longer rows have a workgroup per
-// row that stops at the first rejection; few long rows, and long rows whose positions lie interleaved in memory, are cut
-// among workgroups (three launches).
+// row that stops at the first rejection; few long rows, and long rows whose codes do not lie side by side, are cut among
+// workgroups (three launches).
 #include "common.h"
 
 namespace dvq {
@@ -45,38 +48,86 @@ struct VerifyArgs {
 __device__ __forceinline__ float verify_load(const float* p) { return *p; }
 __device__ __forceinline__ float verify_load(const unsigned short* p) { return bf16_bits_to_f32(*p); }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+// One step of a wave reduction: the value of the lane that the DPP control names, `none` where there is no such lane.
+template <int CTRL>
+__device__ __forceinline__ float verify_dpp(float v, float none) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+}
+template <int CTRL>
+__device__ __forceinline__ double verify_dpp(double v) {
+    const long long b = __builtin_bit_cast(long long, v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, 0xF, 0xF, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, ((long long)hi << 32) | (unsigned)lo);
+}
+__device__ __forceinline__ double verify_lane(double v, int lane) {
+    const long long b = __builtin_bit_cast(long long, v);
+    const int lo = __builtin_amdgcn_readlane((int)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
+    return __builtin_bit_cast(double, ((long long)hi << 32) | (unsigned)lo);
+}
+// Sums of the lanes up to each: inside rows of 16 lanes (shifts by 1, 2, 4, 8), then the row before (0x142), then the lower
+// half (0x143) into the rows behind.
+__device__ __forceinline__ double wave_scan(double v) {
+    v += verify_dpp<0x111>(v);
+    v += verify_dpp<0x112>(v);
+    v += verify_dpp<0x114>(v);
+    v += verify_dpp<0x118>(v);
+    const int row = (threadIdx.x & 63) >> 4;
+    const double t = verify_dpp<0x142>(v);
+    if (row & 1) v += t;
+    const double h = verify_dpp<0x143>(v);
+    if (row & 2) v += h;
     return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {            // (only lane 63 has to be right: no row is spared)
+    v += verify_dpp<0x111>(v);
+    v += verify_dpp<0x112>(v);
+    v += verify_dpp<0x114>(v);
+    v += verify_dpp<0x118>(v);
+    v += verify_dpp<0x142>(v);
+    v += verify_dpp<0x143>(v);
+    return verify_lane(v, 63);
 }
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+    const float none = -__builtin_inff();
+    v = fmaxf(v, verify_dpp<0x111>(v, none));
+    v = fmaxf(v, verify_dpp<0x112>(v, none));
+    v = fmaxf(v, verify_dpp<0x114>(v, none));
+    v = fmaxf(v, verify_dpp<0x118>(v, none));
+    v = fmaxf(v, verify_dpp<0x142>(v, none));
+    v = fmaxf(v, verify_dpp<0x143>(v, none));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
-// exp(d) in 64 bits: d = k ln 2 + f with |f| <= ln 2 / 2 (ln 2 in two parts), the Taylor polynomial of degree 13 (its rest
-// is below f^14 / 14! = 4e-18), scaled by 2^k.  NaN stays NaN, below -746 the result is 0.
-__device__ __forceinline__ double verify_exp(double d) {
-    const double k = rint(d * 1.4426950408889634);
-    double f = __builtin_fma(-k, 0.6931471805599453, d);
-    f = __builtin_fma(-k, 2.3190468138462996e-17, f);
-    double s = 1.0 / 6227020800.0;
-    s = __builtin_fma(s, f, 1.0 / 479001600.0);
-    s = __builtin_fma(s, f, 1.0 / 39916800.0);
-    s = __builtin_fma(s, f, 1.0 / 3628800.0);
-    s = __builtin_fma(s, f, 1.0 / 362880.0);
-    s = __builtin_fma(s, f, 1.0 / 40320.0);
-    s = __builtin_fma(s, f, 1.0 / 5040.0);
-    s = __builtin_fma(s, f, 1.0 / 720.0);
-    s = __builtin_fma(s, f, 1.0 / 120.0);
-    s = __builtin_fma(s, f, 1.0 / 24.0);
-    s = __builtin_fma(s, f, 1.0 / 6.0);
-    s = __builtin_fma(s, f, 0.5);
-    s = __builtin_fma(s, f, 1.0);
-    s = __builtin_fma(s, f, 1.0);
-    return d < -746.0 ? 0.0 : __builtin_ldexp(s, (int)k);
+// exp(d), d <= 700 and not NaN, in 64 bits: d = k ln 2 / 16 + f with |f| <= ln 2 / 32, the Taylor polynomial of degree 6 (its
+// rest is below f^7 / 7! = 5e-16) times 2^(k / 16), the sixteenths from a table in LDS (16 entries of 8 bytes: every lane's
+// read is in a bank of its own or shared).  Adding 1.5 * 2^52 leaves k in the low bits.  Below -746 the result is 0.
+__device__ __constant__ const double kVerifySixteenths[16] = {
+    1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916,
+    1.189207115002721, 1.241857812073484, 1.2968395546510096, 1.3542555469368927,
+    1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543,
+    1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+struct Exp {
+    const double* tab;
+    __device__ __forceinline__ double operator()(double d) const {
+        d = fmax(d, -746.0);
+        const double t = __builtin_fma(d, 23.083120654223414, 6755399441055744.0);
+        const int k = (int)__builtin_bit_cast(long long, t);
+        const double f = __builtin_fma(t - 6755399441055744.0, -0.043321698784996584, d);
+        double s = __builtin_fma(f, 1.0 / 720.0, 1.0 / 120.0);
+        s = __builtin_fma(s, f, 1.0 / 24.0);
+        s = __builtin_fma(s, f, 1.0 / 6.0);
+        s = __builtin_fma(s, f, 0.5);
+        s = __builtin_fma(s, f, 1.0);
+        s = __builtin_fma(s, f, 1.0);
+        return __builtin_ldexp(s * tab[k & 15], k >> 4);
+    }
+};
+// The table in LDS; every thread of the workgroup calls it once.
+__device__ __forceinline__ Exp verify_table(double* lds) {
+    if (threadIdx.x < 16) lds[threadIdx.x] = kVerifySixteenths[threadIdx.x];
+    __syncthreads();
+    return Exp{lds};
 }
 
 // exp(x - ref) in 32 bits for the tests.
@@ -117,15 +168,18 @@ __device__ __forceinline__ void verify_tile(const T* row, int64_t sv, bool unit,
 // Reference point and sum of exp(x - ref) of logits seen so far; no distribution: ref = -inf, or s not a number (a NaN or
 // +inf among the logits makes it one).
 struct Sum { float ref; double s; };
-__device__ __forceinline__ bool sum_ok(const Sum& a) { return a.ref > -__builtin_inff() && a.s == a.s; }
+__device__ __forceinline__ bool sum_ok(const Sum& a) { return a.ref > -__builtin_inff() && a.ref < __builtin_inff() && a.s == a.s; }
+__device__ __forceinline__ double sum_moved(const Exp& ex, const Sum& a, float ref) {        // a.s for reference point ref >= a.ref
+    return a.ref > -__builtin_inff() && a.ref < ref ? a.s * ex((double)a.ref - (double)ref) : a.s;
+}
 
 // The reference moves up only where the next eight exceed it by more than kVerifySlack, and then exactly.
-__device__ __forceinline__ void sum_add(Sum& a, const float (&x)[8]) {
+__device__ __forceinline__ void sum_add(const Exp& ex, Sum& a, const float (&x)[8]) {
     float m = x[0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) m = fmaxf(m, x[j]);
     if (m > a.ref + kVerifySlack) {
-        a.s *= verify_exp((double)a.ref - (double)m);
+        a.s = sum_moved(ex, a, m);
         a.ref = m;
     }
     const float ref = a.ref > -__builtin_inff() ? a.ref : 0.f;       // (nothing but -inf and NaN so far)
@@ -134,21 +188,14 @@ __device__ __forceinline__ void sum_add(Sum& a, const float (&x)[8]) {
     for (int j = 0; j < 8; ++j) f += verify_exp32(x[j] - ref);
     a.s += (double)f;
 }
-__device__ __forceinline__ Sum sum_wave(Sum a) {
+__device__ __forceinline__ Sum sum_wave(const Exp& ex, const Sum& a) {
     const float top = wave_max(a.ref);
-    a.s = wave_sum(a.ref > -__builtin_inff() ? a.s * verify_exp((double)a.ref - (double)top) : a.s);
-    a.ref = top;
-    return a;
+    return Sum{top, wave_sum(sum_moved(ex, a, top))};
 }
 template <int N>
-__device__ __forceinline__ Sum sum_join(const Sum* parts) {         // the same for every thread that calls it
-    Sum a = parts[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) a.ref = fmaxf(a.ref, parts[i].ref);
-    a.s = 0.0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) a.s += parts[i].ref > -__builtin_inff() ? parts[i].s * verify_exp((double)parts[i].ref - (double)a.ref) : parts[i].s;
-    return a;
+__device__ __forceinline__ Sum sum_join(const Exp& ex, const Sum* parts) {         // every wave for itself, all the same
+    const int lane = threadIdx.x & 63;
+    return sum_wave(ex, lane < N ? parts[lane] : Sum{-__builtin_inff(), 0.0});
 }
 
 enum { VERIFY_KEEP = 0, VERIFY_REJECT = 1, VERIFY_BAD = 2, VERIFY_UNSURE = 3 };
@@ -156,15 +203,15 @@ enum { VERIFY_KEEP = 0, VERIFY_REJECT = 1, VERIFY_BAD = 2, VERIFY_UNSURE = 3 };
 // The test of one drafted code; p, q: sums of the position's logits (q unused with PROBS).  `exact`: the sums were taken
 // in 64 bits.
 template <typename T, typename D, bool PROBS>
-__device__ __forceinline__ int verify_test(const VerifyArgs& a, int64_t b, int g, const Sum& p, const Sum& q, bool exact) {
+__device__ __forceinline__ int verify_test(const Exp& ex, const VerifyArgs& a, int64_t b, int g, const Sum& p, const Sum& q, bool exact) {
     if (!sum_ok(p) || (!PROBS && !sum_ok(q))) return VERIFY_BAD;
     const int64_t x = a.tokens[b * a.tb + g * a.tg];
     if (x < 0 || x >= a.V) return VERIFY_REJECT;
     const float t = verify_load(reinterpret_cast<const T*>(a.logits) + b * a.lb + g * a.lp + x * a.lv);
     const float d = verify_load(reinterpret_cast<const D*>(a.draft) + b * a.db + g * a.dg + x * a.dv);
     if (PROBS && !(d >= 0.f && d < __builtin_inff())) return VERIFY_BAD;
-    const double px = verify_exp((double)t - (double)p.ref) / p.s;
-    const double lhs = a.u[b * a.ub + g * a.ug] * (PROBS ? (double)d : verify_exp((double)d - (double)q.ref) / q.s);
+    const double px = ex((double)t - (double)p.ref) / p.s;
+    const double lhs = a.u[b * a.ub + g * a.ug] * (PROBS ? (double)d : ex((double)d - (double)q.ref) / q.s);
     if (!exact && px > 0.0 && lhs > 0.0 && !(fabs(lhs - px) > kVerifyMargin * px)) return VERIFY_UNSURE;
     return lhs < px ? VERIFY_KEEP : VERIFY_REJECT;
 }
@@ -175,44 +222,77 @@ __device__ __forceinline__ int verify_length(const VerifyArgs& a, int64_t b) {
     return n < 0 ? 0 : n > a.G ? a.G : (int)n;
 }
 
-// What the draw needs: reference points and reciprocal sums (64 bits) of p and q, and whether q is taken off.
-struct Draw { double p_ref, p_inv, q_ref, q_inv; bool residual; };
+// Weights of a position's codes: e_p - k e_q where positive (residual), else e_p, with e_p = exp(t - p_ref) and e_q = exp(q -
+// q_ref), or q itself where probabilities are given (k = S_p then).
+struct Weights { double p_ref, q_ref, k; bool residual; };
 
-// Mass of this lane's eight codes of a tile; a given probability that is none makes it NaN.
+// e_p and e_q of this lane's eight codes of a tile; a given probability that is none makes its e_q NaN.
 template <typename T, typename D, bool PROBS>
-__device__ __forceinline__ void verify_mass(const Draw& d, const float (&t)[8], const float (&q)[8], double (&w)[8]) {
+__device__ __forceinline__ void verify_terms(const Exp& ex, const VerifyArgs& a, const T* lr, const D* dr, const Weights& w, bool unit, int v0,
+                                             int lane, double (&ep)[8], double (&eq)[8]) {
+    float t[8], q[8];
+    verify_tile(lr, a.lv, unit, v0, a.V, lane, -__builtin_inff(), t);
+    if (w.residual) verify_tile(dr, a.dv, unit, v0, a.V, lane, PROBS ? 0.f : -__builtin_inff(), q);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        w[j] = verify_exp((double)t[j] - d.p_ref) * d.p_inv;
-        if (d.residual) {
-            const double e = PROBS ? (double)q[j] : verify_exp((double)q[j] - d.q_ref) * d.q_inv;
-            const bool bad = PROBS && !(q[j] >= 0.f && q[j] < __builtin_inff());
-            w[j] = bad ? __builtin_nan("") : fmax(w[j] - e, 0.0);
-        }
+        ep[j] = ex((double)t[j] - w.p_ref);
+        eq[j] = 0.0;
+        if (w.residual) eq[j] = !PROBS ? ex((double)q[j] - w.q_ref) : (q[j] >= 0.f && q[j] < __builtin_inff()) ? (double)q[j] : __builtin_nan("");
+        if (j & 1) __builtin_amdgcn_sched_barrier(0);            // (all eight at once do not fit the registers of four waves)
     }
 }
-template <typename T, typename D, bool PROBS>
-__device__ __forceinline__ void verify_tile_mass(const VerifyArgs& a, const T* lr, const D* dr, const Draw& d, int v0, int lane, double (&w)[8]) {
-    float t[8], q[8];
-    verify_tile(lr, a.lv, a.unit, v0, a.V, lane, -__builtin_inff(), t);
-    if (d.residual) verify_tile(dr, a.dv, a.unit, v0, a.V, lane, PROBS ? 0.f : -__builtin_inff(), q);
-    verify_mass<T, D, PROBS>(d, t, q, w);
+__device__ __forceinline__ double verify_weight(const Weights& w, double ep, double eq) {
+    if (!w.residual) return ep;
+    const double d = __builtin_fma(-w.k, eq, ep);
+    return d > 0.0 || d != d ? d : 0.0;
 }
 __device__ __forceinline__ double verify_sum8(const double (&w)[8]) {
     return ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
 }
 
-// One wave: the first code of the tile at v0 whose cumulated mass (with `before` in front of it) exceeds thr, the last code
-// with mass if none does (the tile's own sum was taken in another order) or if `over`.  w: the masses as verify_tile lays
-// them out; lds: 8 x 72 doubles of this wave's own.
+// What the one pass over a tile leaves (the same in every lane): sums over its codes and over its positive ones.
+struct Tile { double sp, sq, a, c; bool near; };
+
+// One wave.  w.k is within kVerifyMargin / 4 of the true one.
+template <typename T, typename D, bool PROBS>
+__device__ __forceinline__ Tile verify_pass(const Exp& ex, const VerifyArgs& a, const T* lr, const D* dr, const Weights& w, bool unit, int v0, int lane) {
+    double ep[8], eq[8], pa = 0.0, pc = 0.0;
+    verify_terms<T, D, PROBS>(ex, a, lr, dr, w, unit, v0, lane, ep, eq);
+    bool near = false;
+    if (w.residual) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const double kq = w.k * eq[j], d = ep[j] - kq;
+            near |= fabs(d) < kVerifyMargin * kq;
+            if (d > 0.0) { pa += ep[j]; pc += eq[j]; }
+        }
+    }
+    Tile t;
+    t.sp = wave_sum(verify_sum8(ep));
+    t.sq = t.a = t.c = 0.0;
+    if (w.residual) { t.sq = wave_sum(verify_sum8(eq)); t.a = wave_sum(pa); t.c = wave_sum(pc); }
+    t.near = __any(near);
+    return t;
+}
+// Mass of a tile with the weights known exactly; one wave.
+template <typename T, typename D, bool PROBS>
+__device__ __forceinline__ double verify_tile_mass(const Exp& ex, const VerifyArgs& a, const T* lr, const D* dr, const Weights& w, bool unit, int v0, int lane) {
+    double ep[8], eq[8];
+    verify_terms<T, D, PROBS>(ex, a, lr, dr, w, unit, v0, lane, ep, eq);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ep[j] = verify_weight(w, ep[j], eq[j]);
+    return wave_sum(verify_sum8(ep));
+}
+
+// One wave: the first code of the tile at v0 whose cumulated weight (with `before` in front of it) exceeds thr, the last code
+// with weight if none does (the tile's own sum was taken in another order) or if `over`.  w: the weights as verify_tile
+// lays them out; lds: 576 doubles.
 __device__ __forceinline__ int verify_locate(const double (&w)[8], bool unit, int v0, double before, double thr, bool over, double* lds) {
     const int lane = threadIdx.x & 63;
     double c[8];
-    if (unit) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) c[j] = w[j];
-    } else {
-        // from 64 j + lane to 8 lane + j
+    for (int j = 0; j < 8; ++j) c[j] = w[j];
+    if (!unit) {                                                 // from 64 j + lane to 8 lane + j
 #pragma unroll
         for (int j = 0; j < 8; ++j) { const int at = 64 * j + lane; lds[at + (at >> 3)] = w[j]; }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -224,12 +304,7 @@ __device__ __forceinline__ int verify_locate(const double (&w)[8], bool unit, in
     int last = -1;
 #pragma unroll
     for (int j = 0; j < 8; ++j) { own += c[j]; if (c[j] > 0.0) last = j; }
-    double incl = own;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double t = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += t;
-    }
+    const double incl = wave_scan(own);
     const unsigned long long some = __ballot(last >= 0), hit = __ballot(!over && last >= 0 && before + incl > thr);
     const int l = hit ? __ffsll(hit) - 1 : some ? 63 - __clzll(some) : 0;
     int at = last;
@@ -242,7 +317,7 @@ __device__ __forceinline__ int verify_locate(const double (&w)[8], bool unit, in
             if (!found && c[j] > 0.0 && cum > thr) { found = true; at = j; }
         }
     }
-    return v0 + 8 * l + __shfl(at, l, 64);
+    return v0 + 8 * l + __builtin_amdgcn_readlane(at, l);
 }
 
 // The tile that holds the draw, from the masses of all tiles (one wave): returns its number, `before` = mass in front of it;
@@ -253,44 +328,49 @@ __device__ __forceinline__ int verify_pick(const double* mass, int tiles, double
     int last = 0;
     for (int base = 0; base < tiles; base += 64) {
         const double m = base + lane < tiles ? mass[base + lane] : 0.0;
-        double incl = m;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double t = __shfl_up(incl, o, 64);
-            if (lane >= o) incl += t;
-        }
+        const double incl = wave_scan(m);
         const unsigned long long some = __ballot(m > 0.0), hit = __ballot(m > 0.0 && before + incl > thr);
         if (hit) {
             const int l = __ffsll(hit) - 1;
-            before += __shfl(incl - m, l, 64);
+            before += verify_lane(incl - m, l);
             over = false;
             return base + l;
         }
         if (some) last = base + 63 - __clzll(some);
-        before += __shfl(incl, 63, 64);
+        before += verify_lane(incl, 63);
     }
     over = true;
     return last;
 }
-// Sum of the masses of all tiles in the order that verify_pick takes (one wave).
-__device__ __forceinline__ double verify_total(const double* mass, int tiles) {
+// Sum of n values in the order that verify_pick takes (one wave).
+__device__ __forceinline__ double verify_total(const double* v, int n) {
     const int lane = threadIdx.x & 63;
     double total = 0.0;
-    for (int base = 0; base < tiles; base += 64) total += wave_sum(base + lane < tiles ? mass[base + lane] : 0.0);
+    for (int base = 0; base < n; base += 64) total += wave_sum(base + lane < n ? v[base + lane] : 0.0);
     return total;
 }
 
-// Sum of exp(x - ref) of a whole row in 64 bits, codes dealt to `waves` waves tile by tile; this wave's share.
+// Sum of exp(x - ref) of a whole row in 64 bits by the whole workgroup, for the tests too near to tell.
 template <typename T>
-__device__ __forceinline__ double verify_sum64(const T* row, int64_t sv, bool unit, int V, double ref, int first, int step, int lane) {
+__device__ __noinline__ double verify_row_sum64(Exp ex, const T* row, int64_t sv, bool unit, int V, double ref, double* parts) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     double s = 0.0;
-    for (int v0 = first * kTile; v0 < V; v0 += step * kTile) {
+    for (int v0 = wave * kTile; v0 < V; v0 += waves * kTile) {
         float x[8];
         verify_tile(row, sv, unit, v0, V, lane, -__builtin_inff(), x);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s += verify_exp((double)x[j] - ref);
+        for (int j = 0; j < 8; ++j) {
+            s += ex((double)x[j] - ref);
+            if (j & 1) __builtin_amdgcn_sched_barrier(0);
+        }
     }
-    return wave_sum(s);
+    s = wave_sum(s);
+    __syncthreads();
+    if (lane == 0) parts[wave] = s;
+    __syncthreads();
+    double all = 0.0;
+    for (int w = 0; w < waves; ++w) all += parts[w];
+    return all;
 }
 
 // ------------------------------------------------------------------------------------------------ rows of up to 1024 codes
@@ -299,7 +379,8 @@ __device__ __forceinline__ double verify_sum64(const T* row, int64_t sv, bool un
 template <int TILES, typename T, typename D, bool PROBS>
 __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
     __shared__ int state[16];
-    __shared__ double lds[kTile + kTile / 8];
+    __shared__ double lds[kTile + kTile / 8], table[16];
+    const Exp ex = verify_table(table);
     const int64_t b = blockIdx.x;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     const int V = a.V;
@@ -311,7 +392,7 @@ __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
         const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)g * a.lp;
         const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
         Sum p = {none, 0.0}, s = {none, 0.0};
-        int st = g > n ? VERIFY_KEEP : g == n ? VERIFY_REJECT : VERIFY_KEEP;
+        int st = g == n ? VERIFY_REJECT : VERIFY_KEEP;           // (behind n: not looked at)
         if (g <= n && g < a.P) {
 #pragma unroll
             for (int i = 0; i < TILES; ++i) verify_tile(lr, a.lv, a.unit, i * kTile, V, lane, none, t[i]);
@@ -319,36 +400,33 @@ __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
 #pragma unroll
                 for (int i = 0; i < TILES; ++i) verify_tile(dr, a.dv, a.unit, i * kTile, V, lane, none, q[i]);
 #pragma unroll
-            for (int i = 0; i < TILES; ++i) sum_add(p, t[i]);
-            p = sum_wave(p);
+            for (int i = 0; i < TILES; ++i) sum_add(ex, p, t[i]);
+            p = sum_wave(ex, p);
             if (g < n) {
                 if (!PROBS) {
 #pragma unroll
-                    for (int i = 0; i < TILES; ++i) sum_add(s, q[i]);
-                    s = sum_wave(s);
+                    for (int i = 0; i < TILES; ++i) sum_add(ex, s, q[i]);
+                    s = sum_wave(ex, s);
                 }
-                st = verify_test<T, D, PROBS>(a, b, g, p, s, false);
+                st = verify_test<T, D, PROBS>(ex, a, b, g, p, s, false);
+                if (st == VERIFY_UNSURE) {
+                    double e = 0.0;
+#pragma unroll
+                    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) e += ex((double)t[i][j] - (double)p.ref);
+                    p.s = wave_sum(e);
+                    if (!PROBS) {
+                        e = 0.0;
+#pragma unroll
+                        for (int i = 0; i < TILES; ++i)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) e += ex((double)q[i][j] - (double)s.ref);
+                        s.s = wave_sum(e);
+                    }
+                    st = verify_test<T, D, PROBS>(ex, a, b, g, p, s, true);
+                }
             } else if (!sum_ok(p)) st = VERIFY_BAD;
-        }
-        // sums in 64 bits: of the position that may stop the row, and of one too near to tell
-        if (st == VERIFY_REJECT || st == VERIFY_UNSURE) {
-            if (g < a.P && sum_ok(p)) {
-                double e = 0.0;
-#pragma unroll
-                for (int i = 0; i < TILES; ++i)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) e += verify_exp((double)t[i][j] - (double)p.ref);
-                p.s = wave_sum(e);
-            }
-            if (!PROBS && g < n) {
-                double e = 0.0;
-#pragma unroll
-                for (int i = 0; i < TILES; ++i)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) e += verify_exp((double)q[i][j] - (double)s.ref);
-                s.s = wave_sum(e);
-            }
-            if (st == VERIFY_UNSURE) st = verify_test<T, D, PROBS>(a, b, g, p, s, true);
         }
         int stop = st == VERIFY_KEEP ? waves : 0;                // first wave of this round whose position stops the row
         if (waves > 1) {
@@ -364,20 +442,46 @@ __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
             if (lane == 0) a.next[b] = -1;
             return;
         }
-        Draw d = {(double)p.ref, 1.0 / p.s, (double)s.ref, 1.0 / s.s, g < n};
-        if (PROBS && g < n)
+        const bool residual = g < n;
+        if (PROBS && residual)
 #pragma unroll
             for (int i = 0; i < TILES; ++i) verify_tile(dr, a.dv, a.unit, i * kTile, V, lane, 0.f, q[i]);
-        double w[TILES][8], mass[TILES], total = 0.0;
-        for (int pass = 0; pass < 2; ++pass) {
-            total = 0.0;
+        // all terms stay in registers: sums first, weights from them
+        double w[TILES][8], eq[TILES][8], mass[TILES], sp = 0.0, sq = 0.0, total = 0.0;
+#pragma unroll
+        for (int i = 0; i < TILES; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                w[i][j] = ex((double)t[i][j] - (double)p.ref);
+                eq[i][j] = 0.0;
+                if (residual) {
+                    const float v = q[i][j];
+                    eq[i][j] = !PROBS ? ex((double)v - (double)s.ref) : (v >= 0.f && v < __builtin_inff()) ? (double)v : __builtin_nan("");
+                }
+                sp += w[i][j];
+                sq += eq[i][j];
+                if (j & 1) __builtin_amdgcn_sched_barrier(0);
+            }
+        sp = wave_sum(sp);
+        if (!PROBS && residual) sq = wave_sum(sq);
+        Weights k = {(double)p.ref, (double)s.ref, PROBS ? sp : sp / sq, residual};
+        if (residual) {
+            double d[TILES];
 #pragma unroll
             for (int i = 0; i < TILES; ++i) {
-                verify_mass<T, D, PROBS>(d, t[i], q[i], w[i]);
-                total += mass[i] = wave_sum(verify_sum8(w[i]));
+                double x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = verify_weight(k, w[i][j], eq[i][j]);
+                total += d[i] = wave_sum(verify_sum8(x));
             }
-            if (!d.residual || !(total <= kVerifyNoMass)) break;
-            d.residual = false;                                  // nothing left over: from p
+            k.residual = !(total <= kVerifyNoMass * sp);         // nothing left over: from p
+        }
+        total = 0.0;
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[i][j] = verify_weight(k, w[i][j], eq[i][j]);
+            total += mass[i] = wave_sum(verify_sum8(w[i]));
         }
         if (total != total) {
             if (lane == 0) a.next[b] = -1;
@@ -397,114 +501,306 @@ __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
 }
 
 // --------------------------------------------------------------------------------- longer rows, one workgroup per row
+// The draw of a row whose tiles have been passed over: a[i], c[i] and near[i] of every tile in (LDS or other) memory, sp and sq
+// their sums.  Leaves a[i] = mass; every wave calls it.
+template <typename T, typename D, bool PROBS>
+__device__ __forceinline__ void verify_finish(const Exp& ex, const VerifyArgs& args, int64_t b, const T* lr, const D* dr, Weights w, bool unit, double sp,
+                                              double sq, double* a, const double* c, const unsigned char* near, int tiles, double* lds) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    double total = 0.0;
+    if (w.residual) {
+        w.k = PROBS ? sp : sp / sq;
+        for (int i = threadIdx.x; i < tiles; i += blockDim.x)
+            if (!near[i]) a[i] = __builtin_fma(-w.k, c[i], a[i]);
+        int turn = 0;                                            // tiles to do again are dealt to the waves one by one
+        for (int base = 0; base < tiles; base += 64)
+            for (unsigned long long m = __ballot(base + lane < tiles && near[base + lane]); m; m &= m - 1) {
+                if (turn == wave) {
+                    const int i = base + __ffsll(m) - 1;
+                    const double mass = verify_tile_mass<T, D, PROBS>(ex, args, lr, dr, w, unit, i * kTile, lane);
+                    if (lane == 0) a[i] = mass;
+                }
+                turn = turn + 1 == waves ? 0 : turn + 1;
+            }
+        __syncthreads();
+        total = verify_total(a, tiles);                          // every wave for itself, in one order
+        if (total <= kVerifyNoMass * sp) {                       // nothing left over: from p
+            __syncthreads();
+            w.residual = false;
+            for (int i = wave; i < tiles; i += waves) {
+                const double m = verify_tile_mass<T, D, PROBS>(ex, args, lr, dr, w, unit, i * kTile, lane);
+                if (lane == 0) a[i] = m;
+            }
+            __syncthreads();
+            total = verify_total(a, tiles);
+        }
+    } else total = verify_total(a, tiles);
+    if (wave != 0) return;
+    if (total != total || sq != sq) {                            // (sq: a given probability that is none)
+        if (lane == 0) args.next[b] = -1;
+        return;
+    }
+    const double thr = args.r[b * args.rb] * total;
+    double before, ep[8], eq[8];
+    bool over;
+    const int i = verify_pick(a, tiles, thr, before, over);
+    verify_terms<T, D, PROBS>(ex, args, lr, dr, w, unit, i * kTile, lane, ep, eq);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ep[j] = verify_weight(w, ep[j], eq[j]);
+    const int at = verify_locate(ep, unit, i * kTile, before, thr, over, lds);
+    if (lane == 0) args.next[b] = at;
+}
+
 template <int WAVES, typename T>
-__device__ __forceinline__ Sum verify_row_sum(const T* row, int64_t sv, bool unit, int V, Sum* parts) {
+__device__ __forceinline__ Sum verify_row_sum(const Exp& ex, const T* row, int V, Sum* parts) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     Sum a = {-__builtin_inff(), 0.0};
-#pragma unroll 4
+#pragma unroll 2
     for (int v0 = wave * kTile; v0 < V; v0 += WAVES * kTile) {
         float x[8];
-        verify_tile(row, sv, unit, v0, V, lane, -__builtin_inff(), x);
-        sum_add(a, x);
+        verify_tile(row, 1, true, v0, V, lane, -__builtin_inff(), x);
+        sum_add(ex, a, x);
     }
-    a = sum_wave(a);
+    a = sum_wave(ex, a);
     __syncthreads();
     if (lane == 0) parts[wave] = a;
     __syncthreads();
-    return sum_join<WAVES>(parts);
-}
-template <int WAVES, typename T>
-__device__ __forceinline__ double verify_row_sum64(const T* row, int64_t sv, bool unit, int V, double ref, double* parts) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const double s = verify_sum64(row, sv, unit, V, ref, wave, WAVES, lane);
-    __syncthreads();
-    if (lane == 0) parts[wave] = s;
-    __syncthreads();
-    double all = 0.0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) all += parts[w];
-    return all;
+    return sum_join<WAVES>(ex, parts);
 }
 
+// Codes side by side (a.unit).
 template <int WAVES, typename T, typename D, bool PROBS>
-__global__ __launch_bounds__(WAVES * 64) void verify_row_kernel(VerifyArgs a) {
-    extern __shared__ double mass[];                             // one per tile of the row
-    __shared__ Sum parts[WAVES];
-    __shared__ double parts64[WAVES];
-    __shared__ double lds[kTile + kTile / 8];
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(4))) void verify_row_kernel(VerifyArgs a) {
+    extern __shared__ double tile_a[];                           // per tile of the row: a, c, near
+    __shared__ Sum parts[2][WAVES];
+    __shared__ double parts64[2][WAVES], lds[kTile + kTile / 8], table[16];
+    const Exp ex = verify_table(table);
     const int64_t b = blockIdx.x;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int V = a.V, tiles = (V + kTile - 1) / kTile;
+    double* tile_c = tile_a + tiles;
+    unsigned char* tile_near = reinterpret_cast<unsigned char*>(tile_c + tiles);
     const int n = verify_length(a, b);
     const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb;
     const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db;
     Sum p = {0.f, 1.0}, q = {0.f, 1.0};
     int g = 0, st = VERIFY_KEEP;
-    bool exact = false;
-    for (; g < n; ++g, lr += a.lp, dr += a.dg) {
-        p = verify_row_sum<WAVES>(lr, a.lv, a.unit, V, parts);
-        if (!PROBS) q = verify_row_sum<WAVES>(dr, a.dv, a.unit, V, parts);
-        st = verify_test<T, D, PROBS>(a, b, g, p, q, false);     // (the same for every thread: one code's values)
-        exact = false;
+    for (; g < a.P; ++g, lr += a.lp, dr += a.dg) {
+        if (g > n) break;
+        p = verify_row_sum<WAVES>(ex, lr, V, parts[0]);
+        if (g == n) {                                            // every draft kept: one more code
+            st = sum_ok(p) ? VERIFY_REJECT : VERIFY_BAD;
+            break;
+        }
+        if (!PROBS) q = verify_row_sum<WAVES>(ex, dr, V, parts[1]);
+        st = verify_test<T, D, PROBS>(ex, a, b, g, p, q, false); // (the same for every thread: one code's values)
         if (st == VERIFY_UNSURE) {
-            p.s = verify_row_sum64<WAVES>(lr, a.lv, a.unit, V, (double)p.ref, parts64);
-            if (!PROBS) q.s = verify_row_sum64<WAVES>(dr, a.dv, a.unit, V, (double)q.ref, parts64);
-            st = verify_test<T, D, PROBS>(a, b, g, p, q, true);
-            exact = true;
+            p.s = verify_row_sum64(ex, lr, 1, true, V, (double)p.ref, parts64[0]);
+            if (!PROBS) q.s = verify_row_sum64(ex, dr, 1, true, V, (double)q.ref, parts64[1]);
+            st = verify_test<T, D, PROBS>(ex, a, b, g, p, q, true);
         }
         if (st != VERIFY_KEEP) break;
     }
     if (threadIdx.x == 0) a.accepted[b] = g;
-    if (st == VERIFY_KEEP && g < a.P) {                          // every draft kept: one more code
-        p = verify_row_sum<WAVES>(lr, a.lv, a.unit, V, parts);
-        st = sum_ok(p) ? VERIFY_REJECT : VERIFY_BAD;
-        exact = false;
-    }
     if (st != VERIFY_REJECT) {
         if (threadIdx.x == 0) a.next[b] = -1;
         return;
     }
-    const bool residual = g < n;
-    if (!exact) {
-        p.s = verify_row_sum64<WAVES>(lr, a.lv, a.unit, V, (double)p.ref, parts64);
-        if (!PROBS && residual) q.s = verify_row_sum64<WAVES>(dr, a.dv, a.unit, V, (double)q.ref, parts64);
-    }
-    // (a code outside the table is rejected before its draft's sums are needed: they are there all the same)
-    Draw d = {(double)p.ref, 1.0 / p.s, (double)q.ref, 1.0 / q.s, residual};
-    double total = 0.0;
-    for (int pass = 0; pass < 2; ++pass) {
-        for (int i = wave; i < tiles; i += WAVES) {
-            double w[8];
-            verify_tile_mass<T, D, PROBS>(a, lr, dr, d, i * kTile, lane, w);
-            const double m = wave_sum(verify_sum8(w));
-            if (lane == 0) mass[i] = m;
+    const Weights w = {(double)p.ref, (double)q.ref, PROBS ? p.s : p.s / q.s, g < n};
+    double sp = 0.0, sq = 0.0;
+    for (int i = wave; i < tiles; i += WAVES) {
+        const Tile t = verify_pass<T, D, PROBS>(ex, a, lr, dr, w, true, i * kTile, lane);
+        sp += t.sp;
+        sq += t.sq;
+        if (lane == 0) {
+            tile_a[i] = w.residual ? t.a : t.sp;
+            tile_c[i] = t.c;
+            tile_near[i] = t.near;
         }
-        __syncthreads();
-        total = verify_total(mass, tiles);                       // every wave for itself, in one order
-        if (!d.residual || !(total <= kVerifyNoMass)) break;
-        d.residual = false;                                      // nothing left over: from p
-        __syncthreads();
     }
-    if (wave != 0) return;
-    if (total != total) {
-        if (lane == 0) a.next[b] = -1;
-        return;
-    }
-    const double thr = a.r[b * a.rb] * total;
-    double before, w[8];
-    bool over;
-    const int i = verify_pick(mass, tiles, thr, before, over);
-    verify_tile_mass<T, D, PROBS>(a, lr, dr, d, i * kTile, lane, w);
-    const int at = verify_locate(w, a.unit, i * kTile, before, thr, over, lds);
-    if (lane == 0) a.next[b] = at;
+    __syncthreads();
+    if (lane == 0) { parts64[0][wave] = sp; parts64[1][wave] = sq; }
+    __syncthreads();
+    sp = sq = 0.0;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) { sp += parts64[0][i]; sq += parts64[1][i]; }
+    verify_finish<T, D, PROBS>(ex, a, b, lr, dr, w, true, sp, sq, tile_a, tile_c, tile_near, tiles, lds);
 }
 
+// ------------------------------------------------------------- long rows cut among workgroups: three launches
+constexpr int kSplitWaves = 4;
+constexpr int kChunk = 8;                                        // tiles whose test sums one workgroup takes
+// Workspace of one row: test sums of every position's chunks (target, then draft), the decision, what the pass leaves of
+// every tile.
+struct Decision { double k; float p_ref, q_ref; int g, st; };
+struct SplitRow {
+    Sum* p; Sum* q; Decision* d;
+    double *sp, *sq, *a, *c; unsigned char* near;
+};
+__host__ __device__ inline int64_t split_bytes(int P, int G, int V) {
+    const int64_t tiles = (V + kTile - 1) / kTile, chunks = (tiles + kChunk - 1) / kChunk;
+    return (P + G) * chunks * (int64_t)sizeof(Sum) + (int64_t)sizeof(Decision) + 4 * tiles * 8 + (tiles + 15) / 16 * 16 + 8;
+}
+__device__ __forceinline__ SplitRow split_row(char* ws, const VerifyArgs& a, int64_t b) {
+    const int64_t tiles = (a.V + kTile - 1) / kTile, chunks = (tiles + kChunk - 1) / kChunk;
+    char* at = ws + b * ((split_bytes(a.P, a.G, a.V) + 15) / 16 * 16);
+    SplitRow r;
+    r.p = reinterpret_cast<Sum*>(at);
+    r.q = r.p + a.P * chunks;
+    r.d = reinterpret_cast<Decision*>(r.q + a.G * chunks);
+    r.sp = reinterpret_cast<double*>(r.d + 1);
+    r.sq = r.sp + tiles;
+    r.a = r.sq + tiles;
+    r.c = r.a + tiles;
+    r.near = reinterpret_cast<unsigned char*>(r.c + tiles);
+    return r;
+}
+
+// Test sums of one chunk: of one position, or, where codes lie apart and a chunk's positions share cache lines, of all of
+// them one after the other.  All positions are summed: which ones the row needs is not known yet.
 template <typename T, typename D, bool PROBS>
-static int verify_launch(const VerifyArgs& a, hipStream_t st) {
+__global__ __launch_bounds__(kSplitWaves * 64) void verify_stats_kernel(VerifyArgs a, char* ws, int chunks, int groups) {
+    __shared__ Sum parts[2][kSplitWaves];
+    __shared__ double table[16];
+    const Exp ex = verify_table(table);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t id = blockIdx.x;
+    const int chunk = (int)(id % chunks), group = (int)(id / chunks % groups);
+    const int64_t b = id / chunks / groups;
+    const int n = verify_length(a, b);
+    const SplitRow row = split_row(ws, a, b);
+    const int first = groups == 1 ? 0 : group, end = groups == 1 ? a.P : group + 1;
+    for (int g = first; g < end && g <= n; ++g) {
+        const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)g * a.lp;
+        const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
+        const bool both = !PROBS && g < n;
+        Sum p = {-__builtin_inff(), 0.0}, q = p;
+        for (int i = chunk * kChunk + wave; i < (chunk + 1) * kChunk && i * kTile < a.V; i += kSplitWaves) {
+            float x[8];
+            verify_tile(lr, a.lv, a.unit, i * kTile, a.V, lane, -__builtin_inff(), x);
+            sum_add(ex, p, x);
+            if (both) {
+                verify_tile(dr, a.dv, a.unit, i * kTile, a.V, lane, -__builtin_inff(), x);
+                sum_add(ex, q, x);
+            }
+        }
+        p = sum_wave(ex, p);
+        if (both) q = sum_wave(ex, q);
+        __syncthreads();
+        if (lane == 0) { parts[0][wave] = p; parts[1][wave] = q; }
+        __syncthreads();
+        if (wave == 0) {
+            p = sum_join<kSplitWaves>(ex, parts[0]);
+            q = sum_join<kSplitWaves>(ex, parts[1]);
+            if (lane == 0) {
+                row.p[g * chunks + chunk] = p;
+                if (both) row.q[g * chunks + chunk] = q;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ Sum split_join(const Exp& ex, const Sum* parts, int chunks, int lane) {       // one wave
+    Sum a = {-__builtin_inff(), 0.0};
+    for (int i = lane; i < chunks; i += 64) {
+        const Sum t = parts[i];
+        const float top = fmaxf(a.ref, t.ref);
+        a.s = sum_moved(ex, a, top) + sum_moved(ex, t, top);
+        a.ref = top;
+    }
+    return sum_wave(ex, a);
+}
+
+// One tile per wave of the position that stops the row.  Every workgroup finds that position for itself from the chunks' sums,
+// one wave per position; the first of a row writes it down.
+template <typename T, typename D, bool PROBS>
+__global__ __launch_bounds__(kSplitWaves * 64) void verify_pass_kernel(VerifyArgs a, char* ws, int chunks, int groups) {
+    __shared__ Sum sums[2][kSplitWaves];
+    __shared__ int state[kSplitWaves];
+    __shared__ double parts64[kSplitWaves], table[16];
+    const Exp ex = verify_table(table);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t b = (int64_t)blockIdx.x / groups;
+    const int first = (int)((int64_t)blockIdx.x % groups);
+    const int n = verify_length(a, b);
+    const SplitRow row = split_row(ws, a, b);
+    Sum p = {0.f, 1.0}, q = {0.f, 1.0};
+    int st = VERIFY_KEEP, g = 0;
+    for (int base = 0; st == VERIFY_KEEP; base += kSplitWaves) {
+        const int mine = base + wave;
+        int s = mine == n ? (n < a.P ? VERIFY_REJECT : VERIFY_BAD) : VERIFY_KEEP;
+        if (mine <= n && mine < a.P) {
+            p = split_join(ex, row.p + mine * chunks, chunks, lane);
+            if (mine < n) {
+                if (!PROBS) q = split_join(ex, row.q + mine * chunks, chunks, lane);
+                s = verify_test<T, D, PROBS>(ex, a, b, mine, p, q, false);
+            } else if (!sum_ok(p)) s = VERIFY_BAD;
+        }
+        __syncthreads();
+        if (lane == 0) { sums[0][wave] = p; sums[1][wave] = q; state[wave] = s; }
+        __syncthreads();
+        for (int i = 0; i < kSplitWaves && st == VERIFY_KEEP; ++i) {     // (position n always stops: the loop ends)
+            st = state[i];
+            g = base + i;
+            if (st == VERIFY_KEEP) continue;
+            p = sums[0][i];
+            q = sums[1][i];
+            if (st == VERIFY_UNSURE) {
+                const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)g * a.lp;
+                const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
+                p.s = verify_row_sum64(ex, lr, a.lv, a.unit, a.V, (double)p.ref, parts64);
+                if (!PROBS) q.s = verify_row_sum64(ex, dr, a.dv, a.unit, a.V, (double)q.ref, parts64);
+                st = verify_test<T, D, PROBS>(ex, a, b, g, p, q, true);
+            }
+        }
+    }
+    const Weights w = {(double)p.ref, (double)q.ref, PROBS ? p.s : p.s / q.s, g < n};
+    if (first == 0 && threadIdx.x == 0) {
+        a.accepted[b] = g;
+        *row.d = Decision{w.k, p.ref, q.ref, g, st};
+        if (st != VERIFY_REJECT) a.next[b] = -1;
+    }
+    const int i = first * kSplitWaves + wave;
+    if (st != VERIFY_REJECT || i * kTile >= a.V) return;
+    const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)g * a.lp;
+    const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
+    const Tile t = verify_pass<T, D, PROBS>(ex, a, lr, dr, w, a.unit, i * kTile, lane);
+    if (lane == 0) {
+        row.sp[i] = t.sp;
+        row.sq[i] = t.sq;
+        row.a[i] = w.residual ? t.a : t.sp;
+        row.c[i] = t.c;
+        row.near[i] = t.near;
+    }
+}
+
+// One workgroup per row: the draw.
+template <typename T, typename D, bool PROBS>
+__global__ __launch_bounds__(kSplitWaves * 64) void verify_draw_kernel(VerifyArgs a, char* ws) {
+    __shared__ double lds[kTile + kTile / 8], table[16];
+    const Exp ex = verify_table(table);
+    const int64_t b = blockIdx.x;
+    const SplitRow row = split_row(ws, a, b);
+    const Decision d = *row.d;
+    if (d.st != VERIFY_REJECT) return;
+    const int tiles = (a.V + kTile - 1) / kTile;
+    const Weights w = {(double)d.p_ref, (double)d.q_ref, d.k, d.g < verify_length(a, b)};
+    const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)d.g * a.lp;
+    const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)d.g * a.dg;
+    const double sp = verify_total(row.sp, tiles), sq = verify_total(row.sq, tiles);
+    verify_finish<T, D, PROBS>(ex, a, b, lr, dr, w, a.unit, sp, sq, row.a, row.c, row.near, tiles, lds);
+}
+
+// Rows that the workgroup-per-row form takes; fewer, or codes that do not lie side by side, are cut among workgroups.
+constexpr int kRowsMin = 192;
+static bool verify_split(int64_t B, int V, bool unit) { return V > 2 * kTile && (!unit || B < kRowsMin); }
+
+template <typename T, typename D, bool PROBS>
+static int verify_launch(const VerifyArgs& a, char* ws, hipStream_t st) {
     const dim3 grid((unsigned)a.B);
     if (a.V <= 2 * kTile) {
         // positions at a time: all at once for few rows, one after the other where the rows alone fill the card
-        int64_t waves = 8192 / (a.B > 0 ? a.B : 1);
+        int64_t waves = 8192 / a.B;
         if (waves > a.G + 1) waves = a.G + 1;
         if (waves > 16) waves = 16;
         if (waves < 1) waves = 1;
@@ -513,9 +809,18 @@ static int verify_launch(const VerifyArgs& a, hipStream_t st) {
         else hipLaunchKernelGGL((verify_short_kernel<2, T, D, PROBS>), grid, blk, 0, st, a);
         return check_launch("prior_verify");
     }
-    const size_t lds = (size_t)((a.V + kTile - 1) / kTile) * sizeof(double);
-    if (a.B >= 768) hipLaunchKernelGGL((verify_row_kernel<4, T, D, PROBS>), grid, dim3(256), lds, st, a);
-    else hipLaunchKernelGGL((verify_row_kernel<8, T, D, PROBS>), grid, dim3(512), lds, st, a);
+    const int tiles = (a.V + kTile - 1) / kTile;
+    if (verify_split(a.B, a.V, a.unit)) {
+        const int chunks = (tiles + kChunk - 1) / kChunk, groups = a.unit ? a.P : 1, per = (tiles + kSplitWaves - 1) / kSplitWaves;
+        const dim3 blk(kSplitWaves * 64);
+        hipLaunchKernelGGL((verify_stats_kernel<T, D, PROBS>), dim3((unsigned)(a.B * groups * chunks)), blk, 0, st, a, ws, chunks, groups);
+        hipLaunchKernelGGL((verify_pass_kernel<T, D, PROBS>), dim3((unsigned)(a.B * per)), blk, 0, st, a, ws, chunks, per);
+        hipLaunchKernelGGL((verify_draw_kernel<T, D, PROBS>), grid, blk, 0, st, a, ws);
+        return check_launch("prior_verify");
+    }
+    const size_t lds = (size_t)tiles * 17;
+    if (a.B >= 768) hipLaunchKernelGGL((verify_row_kernel<8, T, D, PROBS>), grid, dim3(512), lds, st, a);
+    else hipLaunchKernelGGL((verify_row_kernel<16, T, D, PROBS>), grid, dim3(1024), lds, st, a);
     return check_launch("prior_verify");
 }
 
@@ -523,7 +828,13 @@ static int verify_launch(const VerifyArgs& a, hipStream_t st) {
 
 using namespace dvq;
 
-extern "C" int dvq_prior_verify(const DvqPriorVerify* v, void* stream) {
+extern "C" size_t dvq_prior_verify_workspace_bytes(const DvqPriorVerify* v) {
+    if (!v || v->B < 1 || v->V < 1 || v->P < 1 || v->G < 0) return 0;
+    if (!verify_split(v->B, v->V, v->logits_v == 1 && (v->draft_v == 1 || v->G == 0))) return 0;
+    return (size_t)v->B * (size_t)((split_bytes(v->P, v->G, v->V) + 15) / 16 * 16);
+}
+
+extern "C" int dvq_prior_verify(const DvqPriorVerify* v, void* workspace, size_t workspace_bytes, void* stream) {
     if (!v) return fail(DVQ_EINVAL, "prior_verify: null arguments");
     if (v->B < 0 || v->B > 0x7FFFFFFF || v->V < 1 || v->V > (1 << 20)) return fail(DVQ_EINVAL, "prior_verify: 0 <= B < 2^31, 1 <= V <= 2^20");
     if (v->G < 0 || v->G > 65535 || (v->P != v->G && v->P != v->G + 1) || v->P < 1)
@@ -533,6 +844,12 @@ extern "C" int dvq_prior_verify(const DvqPriorVerify* v, void* stream) {
     if (v->B == 0) return DVQ_OK;
     if (!v->logits || !v->u_draw || !v->accepted || !v->next || (v->G > 0 && (!v->draft || !v->tokens || !v->u_accept)))
         return fail(DVQ_EINVAL, "prior_verify: null pointer");
+    // (workgroups of the largest launch: one per row, position and chunk)
+    const int64_t chunks = (v->V + kTile * kChunk - 1) / (kTile * kChunk), per = (v->V + kTile * kSplitWaves - 1) / (kTile * kSplitWaves);
+    if (v->B * (v->P * chunks > per ? v->P * chunks : per) > 0x7FFFFFFF) return fail(DVQ_EINVAL, "prior_verify: B x P x V too large");
+    const size_t need = dvq_prior_verify_workspace_bytes(v);
+    if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+        return fail(DVQ_EINVAL, "prior_verify: needs a 16-byte aligned workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : 0);
     VerifyArgs a;
     a.logits = v->logits; a.lb = v->logits_b; a.lp = v->logits_p; a.lv = v->logits_v;
     a.draft = v->draft; a.db = v->draft_b; a.dg = v->draft_g; a.dv = v->draft_v;
@@ -543,13 +860,14 @@ extern "C" int dvq_prior_verify(const DvqPriorVerify* v, void* stream) {
     a.accepted = v->accepted; a.next = v->next;
     a.B = v->B; a.G = v->G; a.P = v->P; a.V = v->V;
     a.unit = a.lv == 1 && (a.dv == 1 || a.G == 0);
+    char* ws = reinterpret_cast<char*>(workspace);
     hipStream_t st = as_stream(stream);
     const bool tf = v->logits_dtype == DVQ_F32, df = v->draft_dtype == DVQ_F32;
     typedef unsigned short u16;
     if (v->draft_probs) {
-        if (tf) return df ? verify_launch<float, float, true>(a, st) : verify_launch<float, u16, true>(a, st);
-        return df ? verify_launch<u16, float, true>(a, st) : verify_launch<u16, u16, true>(a, st);
+        if (tf) return df ? verify_launch<float, float, true>(a, ws, st) : verify_launch<float, u16, true>(a, ws, st);
+        return df ? verify_launch<u16, float, true>(a, ws, st) : verify_launch<u16, u16, true>(a, ws, st);
     }
-    if (tf) return df ? verify_launch<float, float, false>(a, st) : verify_launch<float, u16, false>(a, st);
-    return df ? verify_launch<u16, float, false>(a, st) : verify_launch<u16, u16, false>(a, st);
+    if (tf) return df ? verify_launch<float, float, false>(a, ws, st) : verify_launch<float, u16, false>(a, ws, st);
+    return df ? verify_launch<u16, float, false>(a, ws, st) : verify_launch<u16, u16, false>(a, ws, st);
 }

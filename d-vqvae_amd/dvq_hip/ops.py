@@ -707,7 +707,10 @@ def prior_verify(logits: torch.Tensor, draft: torch.Tensor, tokens: torch.Tensor
                        u_accept.data_ptr(), *u_accept.stride(), u_draw.data_ptr(), u_draw.stride(0),
                        None if lengths is None else lengths.data_ptr(), 0 if lengths is None else lengths.stride(0),
                        accepted.data_ptr(), nxt.data_ptr(), B, G, P, V, _dtype_code(logits), _dtype_code(draft), int(draft_probs))
-    _launch(_lib.load().dvq_prior_verify, "dvq_prior_verify", logits.device, ctypes.byref(a))
+    lib, ref = _lib.load(), ctypes.byref(a)
+    nbytes = lib.dvq_prior_verify_workspace_bytes(ref)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
+    _launch(lib.dvq_prior_verify, "dvq_prior_verify", logits.device, ref, _p(ws), nbytes)
     return accepted, nxt
 
 

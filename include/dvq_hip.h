@@ -406,7 +406,9 @@ typedef struct DvqPriorVerify {
     int G, P, V;
     int logits_dtype, draft_dtype, draft_probs;
 } DvqPriorVerify;
-int dvq_prior_verify(const DvqPriorVerify* v, void* stream);
+/* workspace: dvq_prior_verify_workspace_bytes(v) bytes (0 for most shapes: NULL then), 16-byte aligned. */
+size_t dvq_prior_verify_workspace_bytes(const DvqPriorVerify* v);
+int dvq_prior_verify(const DvqPriorVerify* v, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

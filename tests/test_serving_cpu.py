@@ -96,19 +96,32 @@ def _verify_args(**kw):
     return a
 
 
-@pytest.mark.parametrize("bad", [dict(B=-1), dict(V=0), dict(V=(1 << 20) + 1), dict(P=2), dict(P=5), dict(G=0, P=0), dict(G=-1), dict(logits_dtype=2),
+@pytest.mark.parametrize("bad", [dict(B=-1), dict(V=0), dict(V=(1 << 20) + 1), dict(B=1 << 30, V=1 << 20), dict(P=2), dict(P=5), dict(G=0, P=0), dict(G=-1), dict(logits_dtype=2),
                                  dict(draft_dtype=-1), dict(logits=None), dict(draft=None), dict(tokens=None), dict(u_accept=None),
                                  dict(u_draw=None), dict(accepted=None), dict(next=None)])
 def test_verify_refusals(bad):
     lib = _lib.load()
-    assert lib.dvq_prior_verify(ctypes.byref(_verify_args(**bad)), None) == -1 and lib.dvq_last_error()
-    assert lib.dvq_prior_verify(None, None) == -1
+    assert lib.dvq_prior_verify(ctypes.byref(_verify_args(**bad)), 16, 1 << 40, None) == -1 and lib.dvq_last_error()
+    assert lib.dvq_prior_verify(None, 16, 1 << 40, None) == -1
+
+
+def test_verify_refuses_a_workspace_too_small():
+    """Long rows whose codes lie apart, and few long rows, need one."""
+    lib = _lib.load()
+    for kw in (dict(V=5000, logits_v=9, draft_v=1), dict(V=5000, logits_v=1, draft_v=1)):
+        a = _verify_args(**kw)
+        need = lib.dvq_prior_verify_workspace_bytes(ctypes.byref(a))
+        assert need > 0
+        for ws, size in ((None, need), (16, need - 1), (24, need)):
+            assert lib.dvq_prior_verify(ctypes.byref(a), ws, size, None) == -1
+    assert lib.dvq_prior_verify_workspace_bytes(ctypes.byref(_verify_args(V=1000, logits_v=1, draft_v=1))) == 0
+    assert lib.dvq_prior_verify_workspace_bytes(ctypes.byref(_verify_args(V=5000, logits_v=1, draft_v=1, B=5000))) == 0
 
 
 def test_empty_calls_return_without_a_launch():
     lib = _lib.load()
     assert _quantize(lib, M=0) == 0 and _product(lib, M=0) == 0
-    assert lib.dvq_prior_verify(ctypes.byref(_verify_args(B=0)), None) == 0
+    assert lib.dvq_prior_verify(ctypes.byref(_verify_args(B=0)), None, 0, None) == 0
 
 
 def test_cpu_tensors_and_wrong_types_are_refused():
