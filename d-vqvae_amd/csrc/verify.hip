@@ -133,33 +133,33 @@ __device__ __forceinline__ Exp verify_table(double* lds) {
 // exp(x - ref) in 32 bits for the tests.
 __device__ __forceinline__ float verify_exp32(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504f); }
 
+// Eight codes side by side as they lie in memory (16-byte loads at any alignment).
+template <typename T> struct Raw;
+template <> struct Raw<float> {
+    f32x4 w[2];
+    __device__ __forceinline__ void load(const float* p) { __builtin_memcpy(&w[0], p, 16); __builtin_memcpy(&w[1], p + 4, 16); }
+    __device__ __forceinline__ float operator[](int j) const { return w[j >> 2][j & 3]; }
+};
+template <> struct Raw<unsigned short> {
+    u16x8 w;
+    __device__ __forceinline__ void load(const unsigned short* p) { __builtin_memcpy(&w, p, 16); }
+    __device__ __forceinline__ float operator[](int j) const { return bf16_bits_to_f32(w[j]); }
+};
+
 // This lane's eight codes of the tile that starts at code v0, `fill` behind the row's end.  Where target and draft both
-// have unit stride: codes v0 + 8 lane + j (16-byte loads at any alignment), otherwise v0 + 64 j + lane for both.
+// have unit stride: codes v0 + 8 lane + j, otherwise v0 + 64 j + lane for both.
 template <typename T>
 __device__ __forceinline__ void verify_tile(const T* row, int64_t sv, bool unit, int v0, int V, int lane, float fill, float (&x)[8]) {
-    if (unit) {
-        const int v = v0 + 8 * lane;
-        if (v + 8 <= V) {
-            if constexpr (sizeof(T) == 2) {
-                u16x8 w;
-                __builtin_memcpy(&w, row + v, 16);
+    if (unit && v0 + kTile <= V) {
+        Raw<T> r;
+        r.load(row + v0 + 8 * lane);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = bf16_bits_to_f32(w[j]);
-            } else {
-                f32x4 w[2];
-                __builtin_memcpy(&w[0], row + v, 16);
-                __builtin_memcpy(&w[1], row + v + 4, 16);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = w[j >> 2][j & 3];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = v + j < V ? verify_load(row + v + j) : fill;
-        }
+        for (int j = 0; j < 8; ++j) x[j] = r[j];
     } else {
+        const int first = unit ? v0 + 8 * lane : v0 + lane, step = unit ? 1 : 64;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int v = v0 + 64 * j + lane;
+            const int v = first + step * j;
             x[j] = v < V ? verify_load(row + v * sv) : fill;
         }
     }
@@ -200,18 +200,28 @@ __device__ __forceinline__ Sum sum_join(const Exp& ex, const Sum* parts) {      
 
 enum { VERIFY_KEEP = 0, VERIFY_REJECT = 1, VERIFY_BAD = 2, VERIFY_UNSURE = 3 };
 
-// The test of one drafted code; p, q: sums of the position's logits (q unused with PROBS).  `exact`: the sums were taken
-// in 64 bits.
-template <typename T, typename D, bool PROBS>
-__device__ __forceinline__ int verify_test(const Exp& ex, const VerifyArgs& a, int64_t b, int g, const Sum& p, const Sum& q, bool exact) {
-    if (!sum_ok(p) || (!PROBS && !sum_ok(q))) return VERIFY_BAD;
+// What the test of one drafted code reads beside the sums, fetched before them.
+struct Drafted { float t, d; double u; bool inside; };
+template <typename T, typename D>
+__device__ __forceinline__ Drafted verify_fetch(const VerifyArgs& a, int64_t b, int g) {
+    Drafted f = {0.f, 0.f, 0.0, false};
     const int64_t x = a.tokens[b * a.tb + g * a.tg];
-    if (x < 0 || x >= a.V) return VERIFY_REJECT;
-    const float t = verify_load(reinterpret_cast<const T*>(a.logits) + b * a.lb + g * a.lp + x * a.lv);
-    const float d = verify_load(reinterpret_cast<const D*>(a.draft) + b * a.db + g * a.dg + x * a.dv);
-    if (PROBS && !(d >= 0.f && d < __builtin_inff())) return VERIFY_BAD;
-    const double px = ex((double)t - (double)p.ref) / p.s;
-    const double lhs = a.u[b * a.ub + g * a.ug] * (PROBS ? (double)d : ex((double)d - (double)q.ref) / q.s);
+    f.u = a.u[b * a.ub + g * a.ug];
+    f.inside = x >= 0 && x < a.V;
+    if (f.inside) {
+        f.t = verify_load(reinterpret_cast<const T*>(a.logits) + b * a.lb + g * a.lp + x * a.lv);
+        f.d = verify_load(reinterpret_cast<const D*>(a.draft) + b * a.db + g * a.dg + x * a.dv);
+    }
+    return f;
+}
+// p, q: sums of the position's logits (q unused with PROBS).  `exact`: the sums were taken in 64 bits.
+template <bool PROBS>
+__device__ __forceinline__ int verify_test(const Exp& ex, const Drafted& f, const Sum& p, const Sum& q, bool exact) {
+    if (!sum_ok(p) || (!PROBS && !sum_ok(q))) return VERIFY_BAD;
+    if (!f.inside) return VERIFY_REJECT;
+    if (PROBS && !(f.d >= 0.f && f.d < __builtin_inff())) return VERIFY_BAD;
+    const double px = ex((double)f.t - (double)p.ref) / p.s;
+    const double lhs = f.u * (PROBS ? (double)f.d : ex((double)f.d - (double)q.ref) / q.s);
     if (!exact && px > 0.0 && lhs > 0.0 && !(fabs(lhs - px) > kVerifyMargin * px)) return VERIFY_UNSURE;
     return lhs < px ? VERIFY_KEEP : VERIFY_REJECT;
 }
@@ -376,8 +386,13 @@ __device__ __noinline__ double verify_row_sum64(Exp ex, const T* row, int64_t sv
 // ------------------------------------------------------------------------------------------------ rows of up to 1024 codes
 // One workgroup per row, one wave per position: `blockDim / 64` positions at a time until the first that stops the row.
 // Its wave holds the position's logits in registers and draws from them.
-template <int TILES, typename T, typename D, bool PROBS>
+//
+// STAGED: the prior's forward hands its logits over as [B, V, cells], all positions of a code side by side.  Read position
+// by position, every position fetches every cache line of the row again (from L2: 4096 grids of 9 x 512 took 38 us, bound
+// by that); the row's block is copied into LDS once instead.
+template <int TILES, bool STAGED, typename T, typename D, bool PROBS>
 __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
+    extern __shared__ __align__(16) char block[];
     __shared__ int state[16];
     __shared__ double lds[kTile + kTile / 8], table[16];
     const Exp ex = verify_table(table);
@@ -386,16 +401,36 @@ __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
     const int V = a.V;
     const int n = verify_length(a, b);
     const float none = -__builtin_inff();
+    T* const staged = reinterpret_cast<T*>(block);
+    if (STAGED) {
+        const T* from = reinterpret_cast<const T*>(a.logits) + b * a.lb;
+        constexpr int N = 16 / sizeof(T);
+        const int total = V * a.P;
+        int i = threadIdx.x * N;
+#pragma unroll 4
+        for (; i + N <= total; i += blockDim.x * N) {
+            u32x4 v;
+            __builtin_memcpy(&v, from + i, 16);
+            *reinterpret_cast<u32x4*>(staged + i) = v;
+        }
+        for (; i < total; ++i) staged[i] = from[i];              // (at most one thread has a rest)
+        __syncthreads();
+    }
     for (int base = 0;; base += waves) {
         const int g = base + wave;                               // n: the position behind all drafts
         float t[TILES][8], q[TILES][8];
+        Drafted f;
+        if (g < n) f = verify_fetch<T, D>(a, b, g);
         const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)g * a.lp;
         const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
         Sum p = {none, 0.0}, s = {none, 0.0};
         int st = g == n ? VERIFY_REJECT : VERIFY_KEEP;           // (behind n: not looked at)
         if (g <= n && g < a.P) {
 #pragma unroll
-            for (int i = 0; i < TILES; ++i) verify_tile(lr, a.lv, a.unit, i * kTile, V, lane, none, t[i]);
+            for (int i = 0; i < TILES; ++i) {
+                if (STAGED) verify_tile(staged + g, a.P, false, i * kTile, V, lane, none, t[i]);
+                else verify_tile(lr, a.lv, a.unit, i * kTile, V, lane, none, t[i]);
+            }
             if (!PROBS && g < n)
 #pragma unroll
                 for (int i = 0; i < TILES; ++i) verify_tile(dr, a.dv, a.unit, i * kTile, V, lane, none, q[i]);
@@ -408,7 +443,7 @@ __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
                     for (int i = 0; i < TILES; ++i) sum_add(ex, s, q[i]);
                     s = sum_wave(ex, s);
                 }
-                st = verify_test<T, D, PROBS>(ex, a, b, g, p, s, false);
+                st = verify_test<PROBS>(ex, f, p, s, false);
                 if (st == VERIFY_UNSURE) {
                     double e = 0.0;
 #pragma unroll
@@ -424,7 +459,7 @@ __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
                             for (int j = 0; j < 8; ++j) e += ex((double)q[i][j] - (double)s.ref);
                         s.s = wave_sum(e);
                     }
-                    st = verify_test<T, D, PROBS>(ex, a, b, g, p, s, true);
+                    st = verify_test<PROBS>(ex, f, p, s, true);
                 }
             } else if (!sum_ok(p)) st = VERIFY_BAD;
         }
@@ -551,28 +586,51 @@ __device__ __forceinline__ void verify_finish(const Exp& ex, const VerifyArgs& a
     if (lane == 0) args.next[b] = at;
 }
 
-template <int WAVES, typename T>
-__device__ __forceinline__ Sum verify_row_sum(const Exp& ex, const T* row, int V, Sum* parts) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    Sum a = {-__builtin_inff(), 0.0};
-#pragma unroll 2
-    for (int v0 = wave * kTile; v0 < V; v0 += WAVES * kTile) {
-        float x[8];
-        verify_tile(row, 1, true, v0, V, lane, -__builtin_inff(), x);
-        sum_add(ex, a, x);
+// This wave's share of the test sums of tiles first, first + step, .. < end of a row and of its draft's (with `both`), codes
+// side by side.  The loads of a batch of tiles of both rows go out before the first of them is used.
+template <typename T, typename D>
+__device__ __forceinline__ void verify_sums(const Exp& ex, const T* lr, const D* dr, bool both, int V, int first, int step, int end, int lane, Sum& p, Sum& q) {
+    constexpr int NB = sizeof(T) == 2 ? 4 : 2;
+    const float none = -__builtin_inff();
+    for (int i = first; i < end; i += NB * step) {
+        if (i + (NB - 1) * step < end && (i + (NB - 1) * step + 1) * kTile <= V) {
+            Raw<T> x[NB];
+            Raw<D> y[NB];
+#pragma unroll
+            for (int k = 0; k < NB; ++k) {
+                x[k].load(lr + (i + k * step) * kTile + 8 * lane);
+                if (both) y[k].load(dr + (i + k * step) * kTile + 8 * lane);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < NB; ++k) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = x[k][j];
+                sum_add(ex, p, v);
+                if (both) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = y[k][j];
+                    sum_add(ex, q, v);
+                }
+            }
+        } else {
+            for (int k = i; k < end && k < i + NB * step; k += step) {
+                float v[8], z[8];
+                verify_tile(lr, 1, true, k * kTile, V, lane, none, v);
+                if (both) verify_tile(dr, 1, true, k * kTile, V, lane, none, z);
+                sum_add(ex, p, v);
+                if (both) sum_add(ex, q, z);
+            }
+        }
     }
-    a = sum_wave(ex, a);
-    __syncthreads();
-    if (lane == 0) parts[wave] = a;
-    __syncthreads();
-    return sum_join<WAVES>(ex, parts);
 }
 
 // Codes side by side (a.unit).
 template <int WAVES, typename T, typename D, bool PROBS>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(4))) void verify_row_kernel(VerifyArgs a) {
     extern __shared__ double tile_a[];                           // per tile of the row: a, c, near
-    __shared__ Sum parts[2][WAVES];
+    __shared__ Sum parts[2][2][WAVES];
     __shared__ double parts64[2][WAVES], lds[kTile + kTile / 8], table[16];
     const Exp ex = verify_table(table);
     const int64_t b = blockIdx.x;
@@ -585,19 +643,28 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(4)))
     const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db;
     Sum p = {0.f, 1.0}, q = {0.f, 1.0};
     int g = 0, st = VERIFY_KEEP;
-    for (; g < a.P; ++g, lr += a.lp, dr += a.dg) {
-        if (g > n) break;
-        p = verify_row_sum<WAVES>(ex, lr, V, parts[0]);
+    for (; g < a.P && g <= n; ++g, lr += a.lp, dr += a.dg) {
+        const bool both = !PROBS && g < n;
+        Drafted f;
+        if (g < n) f = verify_fetch<T, D>(a, b, g);
+        p = q = Sum{-__builtin_inff(), 0.0};
+        verify_sums(ex, lr, dr, both, V, wave, WAVES, tiles, lane, p, q);
+        p = sum_wave(ex, p);
+        if (both) q = sum_wave(ex, q);
+        Sum (*at)[WAVES] = parts[g & 1];                         // (in turns: one barrier a position)
+        if (lane == 0) { at[0][wave] = p; at[1][wave] = q; }
+        __syncthreads();
+        p = sum_join<WAVES>(ex, at[0]);
+        if (both) q = sum_join<WAVES>(ex, at[1]);
         if (g == n) {                                            // every draft kept: one more code
             st = sum_ok(p) ? VERIFY_REJECT : VERIFY_BAD;
             break;
         }
-        if (!PROBS) q = verify_row_sum<WAVES>(ex, dr, V, parts[1]);
-        st = verify_test<T, D, PROBS>(ex, a, b, g, p, q, false); // (the same for every thread: one code's values)
+        st = verify_test<PROBS>(ex, f, p, q, false);             // (the same for every thread: one code's values)
         if (st == VERIFY_UNSURE) {
             p.s = verify_row_sum64(ex, lr, 1, true, V, (double)p.ref, parts64[0]);
             if (!PROBS) q.s = verify_row_sum64(ex, dr, 1, true, V, (double)q.ref, parts64[1]);
-            st = verify_test<T, D, PROBS>(ex, a, b, g, p, q, true);
+            st = verify_test<PROBS>(ex, f, p, q, true);
         }
         if (st != VERIFY_KEEP) break;
     }
@@ -675,15 +742,18 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_stats_kernel(VerifyAr
         const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
         const bool both = !PROBS && g < n;
         Sum p = {-__builtin_inff(), 0.0}, q = p;
-        for (int i = chunk * kChunk + wave; i < (chunk + 1) * kChunk && i * kTile < a.V; i += kSplitWaves) {
-            float x[8];
-            verify_tile(lr, a.lv, a.unit, i * kTile, a.V, lane, -__builtin_inff(), x);
-            sum_add(ex, p, x);
-            if (both) {
-                verify_tile(dr, a.dv, a.unit, i * kTile, a.V, lane, -__builtin_inff(), x);
-                sum_add(ex, q, x);
+        const int tiles = (a.V + kTile - 1) / kTile, last = (chunk + 1) * kChunk < tiles ? (chunk + 1) * kChunk : tiles;
+        if (a.unit) verify_sums(ex, lr, dr, both, a.V, chunk * kChunk + wave, kSplitWaves, last, lane, p, q);
+        else
+            for (int i = chunk * kChunk + wave; i < last; i += kSplitWaves) {
+                float x[8];
+                verify_tile(lr, a.lv, false, i * kTile, a.V, lane, -__builtin_inff(), x);
+                sum_add(ex, p, x);
+                if (both) {
+                    verify_tile(dr, a.dv, false, i * kTile, a.V, lane, -__builtin_inff(), x);
+                    sum_add(ex, q, x);
+                }
             }
-        }
         p = sum_wave(ex, p);
         if (both) q = sum_wave(ex, q);
         __syncthreads();
@@ -730,10 +800,12 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_pass_kernel(VerifyArg
         const int mine = base + wave;
         int s = mine == n ? (n < a.P ? VERIFY_REJECT : VERIFY_BAD) : VERIFY_KEEP;
         if (mine <= n && mine < a.P) {
+            Drafted f;
+            if (mine < n) f = verify_fetch<T, D>(a, b, mine);
             p = split_join(ex, row.p + mine * chunks, chunks, lane);
             if (mine < n) {
                 if (!PROBS) q = split_join(ex, row.q + mine * chunks, chunks, lane);
-                s = verify_test<T, D, PROBS>(ex, a, b, mine, p, q, false);
+                s = verify_test<PROBS>(ex, f, p, q, false);
             } else if (!sum_ok(p)) s = VERIFY_BAD;
         }
         __syncthreads();
@@ -750,7 +822,7 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_pass_kernel(VerifyArg
                 const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
                 p.s = verify_row_sum64(ex, lr, a.lv, a.unit, a.V, (double)p.ref, parts64);
                 if (!PROBS) q.s = verify_row_sum64(ex, dr, a.dv, a.unit, a.V, (double)q.ref, parts64);
-                st = verify_test<T, D, PROBS>(ex, a, b, g, p, q, true);
+                st = verify_test<PROBS>(ex, verify_fetch<T, D>(a, b, g), p, q, true);
             }
         }
     }
@@ -777,36 +849,63 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_pass_kernel(VerifyArg
 // One workgroup per row: the draw.
 template <typename T, typename D, bool PROBS>
 __global__ __launch_bounds__(kSplitWaves * 64) void verify_draw_kernel(VerifyArgs a, char* ws) {
-    __shared__ double lds[kTile + kTile / 8], table[16];
-    const Exp ex = verify_table(table);
+    extern __shared__ double tile_a[];                           // per tile of the row: a, c, near
+    __shared__ double parts64[2][kSplitWaves], lds[kTile + kTile / 8], table[16];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int64_t b = blockIdx.x;
     const SplitRow row = split_row(ws, a, b);
+    const int tiles = (a.V + kTile - 1) / kTile, n = verify_length(a, b);
     const Decision d = *row.d;
+    double* tile_c = tile_a + tiles;
+    unsigned char* tile_near = reinterpret_cast<unsigned char*>(tile_c + tiles);
+    double sp = 0.0, sq = 0.0;
+    if (d.st == VERIFY_REJECT)                                   // (the tiles of other rows were not written)
+        for (int i = threadIdx.x; i < tiles; i += kSplitWaves * 64) {
+            sp += row.sp[i];
+            sq += row.sq[i];
+            tile_a[i] = row.a[i];
+            tile_c[i] = row.c[i];
+            tile_near[i] = row.near[i];
+        }
+    const Exp ex = verify_table(table);
     if (d.st != VERIFY_REJECT) return;
-    const int tiles = (a.V + kTile - 1) / kTile;
-    const Weights w = {(double)d.p_ref, (double)d.q_ref, d.k, d.g < verify_length(a, b)};
+    sp = wave_sum(sp);
+    sq = wave_sum(sq);
+    if (lane == 0) { parts64[0][wave] = sp; parts64[1][wave] = sq; }
+    __syncthreads();
+    sp = sq = 0.0;
+#pragma unroll
+    for (int i = 0; i < kSplitWaves; ++i) { sp += parts64[0][i]; sq += parts64[1][i]; }
+    const Weights w = {(double)d.p_ref, (double)d.q_ref, d.k, d.g < n};
     const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)d.g * a.lp;
     const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)d.g * a.dg;
-    const double sp = verify_total(row.sp, tiles), sq = verify_total(row.sq, tiles);
-    verify_finish<T, D, PROBS>(ex, a, b, lr, dr, w, a.unit, sp, sq, row.a, row.c, row.near, tiles, lds);
+    verify_finish<T, D, PROBS>(ex, a, b, lr, dr, w, a.unit, sp, sq, tile_a, tile_c, tile_near, tiles, lds);
 }
 
 // Rows that the workgroup-per-row form takes; fewer, or codes that do not lie side by side, are cut among workgroups.
 constexpr int kRowsMin = 192;
+constexpr int kShortWaves = 16384;
 static bool verify_split(int64_t B, int V, bool unit) { return V > 2 * kTile && (!unit || B < kRowsMin); }
 
 template <typename T, typename D, bool PROBS>
 static int verify_launch(const VerifyArgs& a, char* ws, hipStream_t st) {
     const dim3 grid((unsigned)a.B);
     if (a.V <= 2 * kTile) {
-        // positions at a time: all at once for few rows, one after the other where the rows alone fill the card
-        int64_t waves = 8192 / a.B;
+        // positions at a time: all at once for few rows, few where the rows alone fill the card
+        int64_t waves = kShortWaves / a.B;
         if (waves > a.G + 1) waves = a.G + 1;
         if (waves > 16) waves = 16;
         if (waves < 1) waves = 1;
         const dim3 blk((unsigned)waves * 64);
-        if (a.V <= kTile) hipLaunchKernelGGL((verify_short_kernel<1, T, D, PROBS>), grid, blk, 0, st, a);
-        else hipLaunchKernelGGL((verify_short_kernel<2, T, D, PROBS>), grid, blk, 0, st, a);
+        const size_t block = (size_t)a.V * a.P * sizeof(T);
+        const bool staged = a.P > 1 && a.lp == 1 && a.lv == a.P && block <= 32768;
+        if (a.V <= kTile) {
+            if (staged) hipLaunchKernelGGL((verify_short_kernel<1, true, T, D, PROBS>), grid, blk, block, st, a);
+            else hipLaunchKernelGGL((verify_short_kernel<1, false, T, D, PROBS>), grid, blk, 0, st, a);
+        } else {
+            if (staged) hipLaunchKernelGGL((verify_short_kernel<2, true, T, D, PROBS>), grid, blk, block, st, a);
+            else hipLaunchKernelGGL((verify_short_kernel<2, false, T, D, PROBS>), grid, blk, 0, st, a);
+        }
         return check_launch("prior_verify");
     }
     const int tiles = (a.V + kTile - 1) / kTile;
@@ -815,12 +914,12 @@ static int verify_launch(const VerifyArgs& a, char* ws, hipStream_t st) {
         const dim3 blk(kSplitWaves * 64);
         hipLaunchKernelGGL((verify_stats_kernel<T, D, PROBS>), dim3((unsigned)(a.B * groups * chunks)), blk, 0, st, a, ws, chunks, groups);
         hipLaunchKernelGGL((verify_pass_kernel<T, D, PROBS>), dim3((unsigned)(a.B * per)), blk, 0, st, a, ws, chunks, per);
-        hipLaunchKernelGGL((verify_draw_kernel<T, D, PROBS>), grid, blk, 0, st, a, ws);
+        hipLaunchKernelGGL((verify_draw_kernel<T, D, PROBS>), grid, blk, (size_t)tiles * 17, st, a, ws);
         return check_launch("prior_verify");
     }
     const size_t lds = (size_t)tiles * 17;
-    if (a.B >= 768) hipLaunchKernelGGL((verify_row_kernel<8, T, D, PROBS>), grid, dim3(512), lds, st, a);
-    else hipLaunchKernelGGL((verify_row_kernel<16, T, D, PROBS>), grid, dim3(1024), lds, st, a);
+    if (a.B >= 768) hipLaunchKernelGGL((verify_row_kernel<4, T, D, PROBS>), grid, dim3(256), lds, st, a);
+    else hipLaunchKernelGGL((verify_row_kernel<8, T, D, PROBS>), grid, dim3(512), lds, st, a);
     return check_launch("prior_verify");
 }
 
