@@ -12,7 +12,7 @@
 //     sums taken again in 64 bits.
 //   Draw: one position per row, 64-bit exponentials, in one pass although the weights e_p - k e_q (k = S_p / S_q) need the
 //     pass's own sums: k is known to kVerifyMargin from the test, which settles the sign of all weights but those next to
-//     zero, and with the signs settled a tile's mass is sum e_p - k sum e_q over its positive codes.  Tiles that hold a code
+//     zero, and with the signs settled a tile's mass follows k through the sum of e_q over its positive codes.  Tiles that hold a code
 //     next to zero are done again once k is known.  A tile is 512 codes, one wave; the tiles' masses find the tile, a scan
 //     inside it the code.
 // Three forms: rows of up to 1024 codes stay in the registers of one wave per position; longer rows have a workgroup per
@@ -27,9 +27,9 @@ constexpr double kVerifyNoMass = 9.094947017729282e-13;   // 2^-40
 constexpr int kTile = 512;                                // codes of a tile: 8 per lane
 // Relative error of u q / p from sums taken in 32 bits.  A term exp2((x - ref) log2 e) carries |x - ref| 1.5 * 2^-23 from its
 // argument (difference, constant and product rounded) and 2^-23 from the exponential; eight of them are added in 32 bits
-// (7 * 2^-24), everything after that in 64.  ref lies at most kVerifySlack below the largest logit and the mean of
+// (3 * 2^-24), everything after that in 64.  ref lies at most kVerifySlack below the largest logit and the mean of
 // |x - ref| under the distribution is at most kVerifySlack + ln V <= 8 + 13.9, so a sum is off by less than
-// 22 * 1.5 * 2^-23 + 2^-23 + 7 * 2^-24 = 4.5e-6 relative, the quotient of two by less than 1e-5.  Four times that:
+// 22 * 1.5 * 2^-23 + 2^-23 + 3 * 2^-24 = 4.3e-6 relative, the quotient of two by less than 1e-5.  Four times that:
 constexpr double kVerifyMargin = 4e-5;
 constexpr float kVerifySlack = 8.f;
 
@@ -99,39 +99,40 @@ __device__ __forceinline__ float wave_max(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
-// exp(d), d <= 700 and not NaN, in 64 bits: d = k ln 2 / 16 + f with |f| <= ln 2 / 32, the Taylor polynomial of degree 6 (its
-// rest is below f^7 / 7! = 5e-16) times 2^(k / 16), the sixteenths from a table in LDS (16 entries of 8 bytes: every lane's
-// read is in a bank of its own or shared).  Adding 1.5 * 2^52 leaves k in the low bits.  Below -746 the result is 0.
-__device__ __constant__ const double kVerifySixteenths[16] = {
-    1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916,
-    1.189207115002721, 1.241857812073484, 1.2968395546510096, 1.3542555469368927,
-    1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543,
-    1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+// exp(d), d <= 700 and not NaN, in 64 bits: with y = 32 d / ln 2 and k the whole number next to it, 2^(k / 32) -- 32nds of an
+// octave from a table in LDS (32 entries of 8 bytes: a half wave's reads are in banks of their own or shared) -- times the
+// Taylor polynomial of exp((y - k) ln 2 / 32), whose rest after degree 5 is below (ln 2 / 64)^6 / 6! = 2.3e-15.  Adding
+// 1.5 * 2^52 leaves k in the low bits.  Below -746 the result is 0 (-inf among it).
+__device__ __constant__ const double kVerify32nds[32] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
 struct Exp {
     const double* tab;
     __device__ __forceinline__ double operator()(double d) const {
-        d = fmax(d, -746.0);
-        const double t = __builtin_fma(d, 23.083120654223414, 6755399441055744.0);
+        d = fmax(d, -750.0);
+        const double t = __builtin_fma(d, 46.16624130844683, 6755399441055744.0);       // 32 / ln 2
         const int k = (int)__builtin_bit_cast(long long, t);
-        const double f = __builtin_fma(t - 6755399441055744.0, -0.043321698784996584, d);
-        double s = __builtin_fma(f, 1.0 / 720.0, 1.0 / 120.0);
-        s = __builtin_fma(s, f, 1.0 / 24.0);
-        s = __builtin_fma(s, f, 1.0 / 6.0);
-        s = __builtin_fma(s, f, 0.5);
+        const double f = __builtin_fma(d, 46.16624130844683, 6755399441055744.0 - t);
+        double s = __builtin_fma(f, 3.973709984549416e-11, 9.172562701824643e-09);
+        s = __builtin_fma(s, f, 1.693850972437182e-06);
+        s = __builtin_fma(s, f, 0.0002345961982022468);
+        s = __builtin_fma(s, f, 0.02166084939249829);
         s = __builtin_fma(s, f, 1.0);
-        s = __builtin_fma(s, f, 1.0);
-        return __builtin_ldexp(s * tab[k & 15], k >> 4);
+        return __builtin_ldexp(s * tab[k & 31], k >> 5);
     }
 };
 // The table in LDS; every thread of the workgroup calls it once.
 __device__ __forceinline__ Exp verify_table(double* lds) {
-    if (threadIdx.x < 16) lds[threadIdx.x] = kVerifySixteenths[threadIdx.x];
+    if (threadIdx.x < 32) lds[threadIdx.x] = kVerify32nds[threadIdx.x];
     __syncthreads();
     return Exp{lds};
 }
-
-// exp(x - ref) in 32 bits for the tests.
-__device__ __forceinline__ float verify_exp32(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504f); }
 
 // Eight codes side by side as they lie in memory (16-byte loads at any alignment).
 template <typename T> struct Raw;
@@ -183,10 +184,10 @@ __device__ __forceinline__ void sum_add(const Exp& ex, Sum& a, const float (&x)[
         a.ref = m;
     }
     const float ref = a.ref > -__builtin_inff() ? a.ref : 0.f;       // (nothing but -inf and NaN so far)
-    float f = 0.f;
+    float e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f += verify_exp32(x[j] - ref);
-    a.s += (double)f;
+    for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f((x[j] - ref) * 1.44269504f);
+    a.s += (double)(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
 }
 __device__ __forceinline__ Sum sum_wave(const Exp& ex, const Sum& a) {
     const float top = wave_max(a.ref);
@@ -220,8 +221,9 @@ __device__ __forceinline__ int verify_test(const Exp& ex, const Drafted& f, cons
     if (!sum_ok(p) || (!PROBS && !sum_ok(q))) return VERIFY_BAD;
     if (!f.inside) return VERIFY_REJECT;
     if (PROBS && !(f.d >= 0.f && f.d < __builtin_inff())) return VERIFY_BAD;
-    const double px = ex((double)f.t - (double)p.ref) / p.s;
-    const double lhs = f.u * (PROBS ? (double)f.d : ex((double)f.d - (double)q.ref) / q.s);
+    // u q < p, both sides times the two sums
+    const double px = PROBS ? ex((double)f.t - (double)p.ref) : ex((double)f.t - (double)p.ref) * q.s;
+    const double lhs = f.u * (PROBS ? (double)f.d : ex((double)f.d - (double)q.ref)) * p.s;
     if (!exact && px > 0.0 && lhs > 0.0 && !(fabs(lhs - px) > kVerifyMargin * px)) return VERIFY_UNSURE;
     return lhs < px ? VERIFY_KEEP : VERIFY_REJECT;
 }
@@ -260,29 +262,40 @@ __device__ __forceinline__ double verify_sum8(const double (&w)[8]) {
     return ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
 }
 
-// What the one pass over a tile leaves (the same in every lane): sums over its codes and over its positive ones.
-struct Tile { double sp, sq, a, c; bool near; };
+// What the one pass leaves: this lane's sums of e_p and e_q, and of a tile (the same in every lane) the mass with the k that
+// is known so far, the sum of e_q over its positive codes (the mass falls by it times what k lacks), and whether it holds
+// a code whose sign that k does not settle.
+struct Tile { double mass, c; bool near; };
 
 // One wave.  w.k is within kVerifyMargin / 4 of the true one.
-template <typename T, typename D, bool PROBS>
-__device__ __forceinline__ Tile verify_pass(const Exp& ex, const VerifyArgs& a, const T* lr, const D* dr, const Weights& w, bool unit, int v0, int lane) {
-    double ep[8], eq[8], pa = 0.0, pc = 0.0;
-    verify_terms<T, D, PROBS>(ex, a, lr, dr, w, unit, v0, lane, ep, eq);
+template <bool PROBS, typename T, typename D>
+__device__ __forceinline__ Tile verify_pass(const Exp& ex, const Weights& w, const T& t, const D& q, double& sp, double& sq) {
+    double mass[2] = {0.0, 0.0}, c[2] = {0.0, 0.0}, p2[2] = {0.0, 0.0}, q2[2] = {0.0, 0.0};
     bool near = false;
-    if (w.residual) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const double kq = w.k * eq[j], d = ep[j] - kq;
+    for (int j = 0; j < 8; ++j) {
+        const double ep = ex((double)t[j] - w.p_ref);
+        p2[j & 1] += ep;
+        if (w.residual) {
+            const float v = q[j];
+            const double eq = !PROBS ? ex((double)v - w.q_ref) : (v >= 0.f && v < __builtin_inff()) ? (double)v : __builtin_nan("");
+            const double kq = w.k * eq, d = ep - kq;
+            q2[j & 1] += eq;
+            mass[j & 1] += fmax(d, 0.0);
+            c[j & 1] += d > 0.0 ? eq : 0.0;
             near |= fabs(d) < kVerifyMargin * kq;
-            if (d > 0.0) { pa += ep[j]; pc += eq[j]; }
         }
+        if (j & 1) __builtin_amdgcn_sched_barrier(0);            // (all eight at once do not fit the registers of four waves)
     }
-    Tile t;
-    t.sp = wave_sum(verify_sum8(ep));
-    t.sq = t.a = t.c = 0.0;
-    if (w.residual) { t.sq = wave_sum(verify_sum8(eq)); t.a = wave_sum(pa); t.c = wave_sum(pc); }
-    t.near = __any(near);
-    return t;
+    sp += p2[0] + p2[1];
+    sq += q2[0] + q2[1];
+    Tile r = {0.0, 0.0, false};
+    if (w.residual) {
+        r.mass = wave_sum(mass[0] + mass[1]);
+        r.c = wave_sum(c[0] + c[1]);
+        r.near = __any(near);
+    } else r.mass = wave_sum(p2[0] + p2[1]);
+    return r;
 }
 // Mass of a tile with the weights known exactly; one wave.
 template <typename T, typename D, bool PROBS>
@@ -392,14 +405,17 @@ __device__ __noinline__ double verify_row_sum64(Exp ex, const T* row, int64_t sv
 // by that); the row's block is copied into LDS once instead.
 template <int TILES, bool STAGED, typename T, typename D, bool PROBS>
 __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
-    extern __shared__ __align__(16) char block[];
+    extern __shared__ __align__(16) char block[];                // the staged block, later room for verify_locate
     __shared__ int state[16];
-    __shared__ double lds[kTile + kTile / 8], table[16];
-    const Exp ex = verify_table(table);
+    __shared__ double table[32];
+    double* const lds = reinterpret_cast<double*>(block);
     const int64_t b = blockIdx.x;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     const int V = a.V;
     const int n = verify_length(a, b);
+    const double at_draw = a.r[b * a.rb];
+    Drafted f;
+    if (wave < n) f = verify_fetch<T, D>(a, b, wave);
     const float none = -__builtin_inff();
     T* const staged = reinterpret_cast<T*>(block);
     if (STAGED) {
@@ -414,13 +430,13 @@ __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
             *reinterpret_cast<u32x4*>(staged + i) = v;
         }
         for (; i < total; ++i) staged[i] = from[i];              // (at most one thread has a rest)
-        __syncthreads();
     }
+    const Exp ex = verify_table(table);
     for (int base = 0;; base += waves) {
         const int g = base + wave;                               // n: the position behind all drafts
         float t[TILES][8], q[TILES][8];
-        Drafted f;
-        if (g < n) f = verify_fetch<T, D>(a, b, g);
+        Drafted ahead;
+        if (g + waves < n) ahead = verify_fetch<T, D>(a, b, g + waves);
         const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)g * a.lp;
         const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
         Sum p = {none, 0.0}, s = {none, 0.0};
@@ -470,6 +486,7 @@ __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
             __syncthreads();
             for (stop = 0; stop < waves && state[stop] == VERIFY_KEEP; ++stop) {}
         }
+        f = ahead;
         if (stop == waves) continue;                             // (position n always stops: the loop ends)
         if (wave != stop) return;
         if (lane == 0) a.accepted[b] = g;
@@ -522,7 +539,7 @@ __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
             if (lane == 0) a.next[b] = -1;
             return;
         }
-        const double thr = a.r[b * a.rb] * total;
+        const double thr = at_draw * total;
         int at = 0;
         if (TILES == 1) at = verify_locate(w[0], a.unit, 0, 0.0, thr, !(total > thr), lds);
         else {
@@ -536,17 +553,18 @@ __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
 }
 
 // --------------------------------------------------------------------------------- longer rows, one workgroup per row
-// The draw of a row whose tiles have been passed over: a[i], c[i] and near[i] of every tile in (LDS or other) memory, sp and sq
-// their sums.  Leaves a[i] = mass; every wave calls it.
+// The draw of a row whose tiles have been passed over: mass, c and near of every tile in LDS, sp and sq the sums of e_p and e_q.
+// Every wave calls it.
 template <typename T, typename D, bool PROBS>
 __device__ __forceinline__ void verify_finish(const Exp& ex, const VerifyArgs& args, int64_t b, const T* lr, const D* dr, Weights w, bool unit, double sp,
                                               double sq, double* a, const double* c, const unsigned char* near, int tiles, double* lds) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     double total = 0.0;
     if (w.residual) {
-        w.k = PROBS ? sp : sp / sq;
+        const double k = PROBS ? sp : sp / sq;
         for (int i = threadIdx.x; i < tiles; i += blockDim.x)
-            if (!near[i]) a[i] = __builtin_fma(-w.k, c[i], a[i]);
+            if (!near[i]) a[i] = __builtin_fma(w.k - k, c[i], a[i]);
+        w.k = k;
         int turn = 0;                                            // tiles to do again are dealt to the waves one by one
         for (int base = 0; base < tiles; base += 64)
             for (unsigned long long m = __ballot(base + lane < tiles && near[base + lane]); m; m &= m - 1) {
@@ -631,7 +649,7 @@ template <int WAVES, typename T, typename D, bool PROBS>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(4))) void verify_row_kernel(VerifyArgs a) {
     extern __shared__ double tile_a[];                           // per tile of the row: a, c, near
     __shared__ Sum parts[2][2][WAVES];
-    __shared__ double parts64[2][WAVES], lds[kTile + kTile / 8], table[16];
+    __shared__ double parts64[2][WAVES], lds[kTile + kTile / 8], table[32];
     const Exp ex = verify_table(table);
     const int64_t b = blockIdx.x;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -675,16 +693,22 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(4)))
     }
     const Weights w = {(double)p.ref, (double)q.ref, PROBS ? p.s : p.s / q.s, g < n};
     double sp = 0.0, sq = 0.0;
+    const float none = -__builtin_inff();
+    float t[8], d[8];
+    verify_tile(lr, 1, true, wave * kTile, V, lane, none, t);
+    if (w.residual) verify_tile(dr, 1, true, wave * kTile, V, lane, PROBS ? 0.f : none, d);
     for (int i = wave; i < tiles; i += WAVES) {
-        const Tile t = verify_pass<T, D, PROBS>(ex, a, lr, dr, w, true, i * kTile, lane);
-        sp += t.sp;
-        sq += t.sq;
-        if (lane == 0) {
-            tile_a[i] = w.residual ? t.a : t.sp;
-            tile_c[i] = t.c;
-            tile_near[i] = t.near;
-        }
+        float x[8], y[8];                                        // the next tile is on its way during the work on this one
+        verify_tile(lr, 1, true, (i + WAVES) * kTile, V, lane, none, x);
+        if (w.residual) verify_tile(dr, 1, true, (i + WAVES) * kTile, V, lane, PROBS ? 0.f : none, y);
+        __builtin_amdgcn_sched_barrier(0);
+        const Tile r = verify_pass<PROBS>(ex, w, t, d, sp, sq);
+        if (lane == 0) { tile_a[i] = r.mass; tile_c[i] = r.c; tile_near[i] = r.near; }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { t[j] = x[j]; d[j] = y[j]; }
     }
+    sp = wave_sum(sp);
+    sq = wave_sum(sq);
     __syncthreads();
     if (lane == 0) { parts64[0][wave] = sp; parts64[1][wave] = sq; }
     __syncthreads();
@@ -728,7 +752,7 @@ __device__ __forceinline__ SplitRow split_row(char* ws, const VerifyArgs& a, int
 template <typename T, typename D, bool PROBS>
 __global__ __launch_bounds__(kSplitWaves * 64) void verify_stats_kernel(VerifyArgs a, char* ws, int chunks, int groups) {
     __shared__ Sum parts[2][kSplitWaves];
-    __shared__ double table[16];
+    __shared__ double table[32];
     const Exp ex = verify_table(table);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int64_t id = blockIdx.x;
@@ -787,7 +811,7 @@ template <typename T, typename D, bool PROBS>
 __global__ __launch_bounds__(kSplitWaves * 64) void verify_pass_kernel(VerifyArgs a, char* ws, int chunks, int groups) {
     __shared__ Sum sums[2][kSplitWaves];
     __shared__ int state[kSplitWaves];
-    __shared__ double parts64[kSplitWaves], table[16];
+    __shared__ double parts64[kSplitWaves], table[32];
     const Exp ex = verify_table(table);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int64_t b = (int64_t)blockIdx.x / groups;
@@ -836,13 +860,19 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_pass_kernel(VerifyArg
     if (st != VERIFY_REJECT || i * kTile >= a.V) return;
     const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)g * a.lp;
     const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
-    const Tile t = verify_pass<T, D, PROBS>(ex, a, lr, dr, w, a.unit, i * kTile, lane);
+    float t[8], d[8];
+    verify_tile(lr, a.lv, a.unit, i * kTile, a.V, lane, -__builtin_inff(), t);
+    if (w.residual) verify_tile(dr, a.dv, a.unit, i * kTile, a.V, lane, PROBS ? 0.f : -__builtin_inff(), d);
+    double sp = 0.0, sq = 0.0;
+    const Tile r = verify_pass<PROBS>(ex, w, t, d, sp, sq);
+    sp = wave_sum(sp);
+    sq = wave_sum(sq);
     if (lane == 0) {
-        row.sp[i] = t.sp;
-        row.sq[i] = t.sq;
-        row.a[i] = w.residual ? t.a : t.sp;
-        row.c[i] = t.c;
-        row.near[i] = t.near;
+        row.sp[i] = sp;
+        row.sq[i] = sq;
+        row.a[i] = r.mass;
+        row.c[i] = r.c;
+        row.near[i] = r.near;
     }
 }
 
@@ -850,7 +880,7 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_pass_kernel(VerifyArg
 template <typename T, typename D, bool PROBS>
 __global__ __launch_bounds__(kSplitWaves * 64) void verify_draw_kernel(VerifyArgs a, char* ws) {
     extern __shared__ double tile_a[];                           // per tile of the row: a, c, near
-    __shared__ double parts64[2][kSplitWaves], lds[kTile + kTile / 8], table[16];
+    __shared__ double parts64[2][kSplitWaves], lds[kTile + kTile / 8], table[32];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int64_t b = blockIdx.x;
     const SplitRow row = split_row(ws, a, b);
@@ -897,14 +927,15 @@ static int verify_launch(const VerifyArgs& a, char* ws, hipStream_t st) {
         if (waves > 16) waves = 16;
         if (waves < 1) waves = 1;
         const dim3 blk((unsigned)waves * 64);
-        const size_t block = (size_t)a.V * a.P * sizeof(T);
+        const size_t block = (size_t)a.V * a.P * sizeof(T), room = (kTile + kTile / 8) * sizeof(double);
         const bool staged = a.P > 1 && a.lp == 1 && a.lv == a.P && block <= 32768;
+        const size_t lds = staged && block > room ? block : room;
         if (a.V <= kTile) {
-            if (staged) hipLaunchKernelGGL((verify_short_kernel<1, true, T, D, PROBS>), grid, blk, block, st, a);
-            else hipLaunchKernelGGL((verify_short_kernel<1, false, T, D, PROBS>), grid, blk, 0, st, a);
+            if (staged) hipLaunchKernelGGL((verify_short_kernel<1, true, T, D, PROBS>), grid, blk, lds, st, a);
+            else hipLaunchKernelGGL((verify_short_kernel<1, false, T, D, PROBS>), grid, blk, lds, st, a);
         } else {
-            if (staged) hipLaunchKernelGGL((verify_short_kernel<2, true, T, D, PROBS>), grid, blk, block, st, a);
-            else hipLaunchKernelGGL((verify_short_kernel<2, false, T, D, PROBS>), grid, blk, 0, st, a);
+            if (staged) hipLaunchKernelGGL((verify_short_kernel<2, true, T, D, PROBS>), grid, blk, lds, st, a);
+            else hipLaunchKernelGGL((verify_short_kernel<2, false, T, D, PROBS>), grid, blk, lds, st, a);
         }
         return check_launch("prior_verify");
     }
