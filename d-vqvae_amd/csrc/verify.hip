@@ -48,6 +48,9 @@ struct VerifyArgs {
 __device__ __forceinline__ float verify_load(const float* p) { return *p; }
 __device__ __forceinline__ float verify_load(const unsigned short* p) { return bf16_bits_to_f32(*p); }
 
+// The wave's number, known to be the same in every lane (addresses that follow from it are scalar).
+__device__ __forceinline__ int verify_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 // One step of a wave reduction: the value of the lane that the DPP control names, `none` where there is no such lane.
 template <int CTRL>
 __device__ __forceinline__ float verify_dpp(float v, float none) {
@@ -78,6 +81,15 @@ __device__ __forceinline__ double wave_scan(double v) {
     const double h = verify_dpp<0x143>(v);
     if (row & 2) v += h;
     return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v += verify_dpp<0x111>(v, 0.f);
+    v += verify_dpp<0x112>(v, 0.f);
+    v += verify_dpp<0x114>(v, 0.f);
+    v += verify_dpp<0x118>(v, 0.f);
+    v += verify_dpp<0x142>(v, 0.f);
+    v += verify_dpp<0x143>(v, 0.f);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 __device__ __forceinline__ double wave_sum(double v) {            // (only lane 63 has to be right: no row is spared)
     v += verify_dpp<0x111>(v);
@@ -147,15 +159,28 @@ template <> struct Raw<unsigned short> {
     __device__ __forceinline__ float operator[](int j) const { return bf16_bits_to_f32(w[j]); }
 };
 
-// This lane's eight codes of the tile that starts at code v0, `fill` behind the row's end.  Where target and draft both
-// have unit stride: codes v0 + 8 lane + j, otherwise v0 + 64 j + lane for both.
+// First code that verify_tile reads for the tile at v0: with unit stride the last tile of a row is read from 512 codes before
+// the row's end (whole 16-byte loads, no lane by itself), and those that belong to the tile in front of it are dropped.
+__device__ __forceinline__ int verify_base(bool unit, int v0, int V) { return unit && V >= kTile && v0 + kTile > V ? V - kTile : v0; }
+
+// This lane's eight codes of the tile at v0, `fill` for codes that are not in it or not in the row.  Where target and draft
+// both have unit stride: codes base + 8 lane + j, otherwise v0 + 64 j + lane for both.
 template <typename T>
 __device__ __forceinline__ void verify_tile(const T* row, int64_t sv, bool unit, int v0, int V, int lane, float fill, float (&x)[8]) {
-    if (unit && v0 + kTile <= V) {
+    if (unit && V >= kTile) {
+        const int base = verify_base(unit, v0, V), skip = v0 - base - 8 * lane;
         Raw<T> r;
-        r.load(row + v0 + 8 * lane);
+        r.load(row + base + 8 * lane);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = r[j];
+        if (base != v0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = j < skip ? fill : x[j];
+        }
+    } else if (v0 + kTile <= V) {
+        const T* at = row + (v0 + lane) * sv;
+#pragma unroll
+        for (int j = 0; j < 8; ++j, at += 64 * sv) x[j] = verify_load(at);
     } else {
         const int first = unit ? v0 + 8 * lane : v0 + lane, step = unit ? 1 : 64;
 #pragma unroll
@@ -197,6 +222,28 @@ template <int N>
 __device__ __forceinline__ Sum sum_join(const Exp& ex, const Sum* parts) {         // every wave for itself, all the same
     const int lane = threadIdx.x & 63;
     return sum_wave(ex, lane < N ? parts[lane] : Sum{-__builtin_inff(), 0.0});
+}
+
+// The test sum of a row that a wave holds: its largest logit is at hand, and the lanes' sums are added in 32 bits (ten
+// roundings; with |x - ref| <= ln 1024 in the mean still well inside kVerifyMargin).
+template <int TILES>
+__device__ __forceinline__ Sum sum_held(const float (&x)[TILES][8]) {
+    float m = x[0][0];
+#pragma unroll
+    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, x[i][j]);
+    m = wave_max(m);
+    float f = 0.f;
+    if (m > -__builtin_inff())
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+            float e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f((x[i][j] - m) * 1.44269504f);
+            f += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+        }
+    return Sum{m, (double)wave_sum(f)};
 }
 
 enum { VERIFY_KEEP = 0, VERIFY_REJECT = 1, VERIFY_BAD = 2, VERIFY_UNSURE = 3 };
@@ -310,7 +357,7 @@ __device__ __forceinline__ double verify_tile_mass(const Exp& ex, const VerifyAr
 // One wave: the first code of the tile at v0 whose cumulated weight (with `before` in front of it) exceeds thr, the last code
 // with weight if none does (the tile's own sum was taken in another order) or if `over`.  w: the weights as verify_tile
 // lays them out; lds: 576 doubles.
-__device__ __forceinline__ int verify_locate(const double (&w)[8], bool unit, int v0, double before, double thr, bool over, double* lds) {
+__device__ __forceinline__ int verify_locate(const double (&w)[8], bool unit, int v0, int V, double before, double thr, bool over, double* lds) {
     const int lane = threadIdx.x & 63;
     double c[8];
 #pragma unroll
@@ -340,7 +387,7 @@ __device__ __forceinline__ int verify_locate(const double (&w)[8], bool unit, in
             if (!found && c[j] > 0.0 && cum > thr) { found = true; at = j; }
         }
     }
-    return v0 + 8 * l + __builtin_amdgcn_readlane(at, l);
+    return verify_base(unit, v0, V) + 8 * l + __builtin_amdgcn_readlane(at, l);
 }
 
 // The tile that holds the draw, from the masses of all tiles (one wave): returns its number, `before` = mass in front of it;
@@ -376,7 +423,7 @@ __device__ __forceinline__ double verify_total(const double* v, int n) {
 // Sum of exp(x - ref) of a whole row in 64 bits by the whole workgroup, for the tests too near to tell.
 template <typename T>
 __device__ __noinline__ double verify_row_sum64(Exp ex, const T* row, int64_t sv, bool unit, int V, double ref, double* parts) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    const int wave = verify_wave(), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     double s = 0.0;
     for (int v0 = wave * kTile; v0 < V; v0 += waves * kTile) {
         float x[8];
@@ -404,13 +451,13 @@ __device__ __noinline__ double verify_row_sum64(Exp ex, const T* row, int64_t sv
 // by position, every position fetches every cache line of the row again (from L2: 4096 grids of 9 x 512 took 38 us, bound
 // by that); the row's block is copied into LDS once instead.
 template <int TILES, bool STAGED, typename T, typename D, bool PROBS>
-__global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
+__global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(TILES == 1 && PROBS ? 8 : 4))) void verify_short_kernel(VerifyArgs a) {
     extern __shared__ __align__(16) char block[];                // the staged block, later room for verify_locate
     __shared__ int state[16];
     __shared__ double table[32];
     double* const lds = reinterpret_cast<double*>(block);
     const int64_t b = blockIdx.x;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    const int wave = verify_wave(), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     const int V = a.V;
     const int n = verify_length(a, b);
     const double at_draw = a.r[b * a.rb];
@@ -444,21 +491,15 @@ __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
         if (g <= n && g < a.P) {
 #pragma unroll
             for (int i = 0; i < TILES; ++i) {
-                if (STAGED) verify_tile(staged + g, a.P, false, i * kTile, V, lane, none, t[i]);
+                if (STAGED) verify_tile(staged + g, (int64_t)a.P, false, i * kTile, V, lane, none, t[i]);
                 else verify_tile(lr, a.lv, a.unit, i * kTile, V, lane, none, t[i]);
             }
             if (!PROBS && g < n)
 #pragma unroll
                 for (int i = 0; i < TILES; ++i) verify_tile(dr, a.dv, a.unit, i * kTile, V, lane, none, q[i]);
-#pragma unroll
-            for (int i = 0; i < TILES; ++i) sum_add(ex, p, t[i]);
-            p = sum_wave(ex, p);
+            p = sum_held(t);
             if (g < n) {
-                if (!PROBS) {
-#pragma unroll
-                    for (int i = 0; i < TILES; ++i) sum_add(ex, s, q[i]);
-                    s = sum_wave(ex, s);
-                }
+                if (!PROBS) s = sum_held(q);
                 st = verify_test<PROBS>(ex, f, p, s, false);
                 if (st == VERIFY_UNSURE) {
                     double e = 0.0;
@@ -541,11 +582,11 @@ __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
         }
         const double thr = at_draw * total;
         int at = 0;
-        if (TILES == 1) at = verify_locate(w[0], a.unit, 0, 0.0, thr, !(total > thr), lds);
+        if (TILES == 1) at = verify_locate(w[0], a.unit, 0, V, 0.0, thr, !(total > thr), lds);
         else {
             const bool second = mass[0] > thr ? false : (mass[TILES - 1] > 0.0 || !(mass[0] > 0.0));
-            at = second ? verify_locate(w[TILES - 1], a.unit, kTile, mass[0], thr, !(total > thr), lds)
-                        : verify_locate(w[0], a.unit, 0, 0.0, thr, !(mass[0] > thr), lds);
+            at = second ? verify_locate(w[TILES - 1], a.unit, kTile, V, mass[0], thr, !(total > thr), lds)
+                        : verify_locate(w[0], a.unit, 0, V, 0.0, thr, !(mass[0] > thr), lds);
         }
         if (lane == 0) a.next[b] = at;
         return;
@@ -558,7 +599,7 @@ __global__ __launch_bounds__(1024) void verify_short_kernel(VerifyArgs a) {
 template <typename T, typename D, bool PROBS>
 __device__ __forceinline__ void verify_finish(const Exp& ex, const VerifyArgs& args, int64_t b, const T* lr, const D* dr, Weights w, bool unit, double sp,
                                               double sq, double* a, const double* c, const unsigned char* near, int tiles, double* lds) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    const int wave = verify_wave(), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     double total = 0.0;
     if (w.residual) {
         const double k = PROBS ? sp : sp / sq;
@@ -600,47 +641,55 @@ __device__ __forceinline__ void verify_finish(const Exp& ex, const VerifyArgs& a
     verify_terms<T, D, PROBS>(ex, args, lr, dr, w, unit, i * kTile, lane, ep, eq);
 #pragma unroll
     for (int j = 0; j < 8; ++j) ep[j] = verify_weight(w, ep[j], eq[j]);
-    const int at = verify_locate(ep, unit, i * kTile, before, thr, over, lds);
+    const int at = verify_locate(ep, unit, i * kTile, args.V, before, thr, over, lds);
     if (lane == 0) args.next[b] = at;
 }
 
 // This wave's share of the test sums of tiles first, first + step, .. < end of a row and of its draft's (with `both`), codes
-// side by side.  The loads of a batch of tiles of both rows go out before the first of them is used.
+// side by side.  The loads of a batch of tiles of both rows go out before the batch in front of it is worked on.
 template <typename T, typename D>
 __device__ __forceinline__ void verify_sums(const Exp& ex, const T* lr, const D* dr, bool both, int V, int first, int step, int end, int lane, Sum& p, Sum& q) {
-    constexpr int NB = sizeof(T) == 2 ? 4 : 2;
+    constexpr int NB = 2;
     const float none = -__builtin_inff();
-    for (int i = first; i < end; i += NB * step) {
-        if (i + (NB - 1) * step < end && (i + (NB - 1) * step + 1) * kTile <= V) {
-            Raw<T> x[NB];
-            Raw<D> y[NB];
+    const int full = V / kTile < end ? V / kTile : end;         // tiles before `full` hold 512 codes
+    const auto whole = [&](int i) { return i + (NB - 1) * step < full; };
+    const auto batch = [&](int i, Raw<T> (&x)[NB], Raw<D> (&y)[NB]) {
 #pragma unroll
-            for (int k = 0; k < NB; ++k) {
-                x[k].load(lr + (i + k * step) * kTile + 8 * lane);
-                if (both) y[k].load(dr + (i + k * step) * kTile + 8 * lane);
-            }
-            __builtin_amdgcn_sched_barrier(0);
+        for (int k = 0; k < NB; ++k) {
+            x[k].load(lr + (i + k * step) * kTile + 8 * lane);
+            if (both) y[k].load(dr + (i + k * step) * kTile + 8 * lane);
+        }
+    };
+    int i = first;
+    Raw<T> x[NB];
+    Raw<D> y[NB];
+    if (whole(i)) batch(i, x, y);
+    for (; whole(i); i += NB * step) {
+        Raw<T> nx[NB];
+        Raw<D> ny[NB];
+        if (whole(i + NB * step)) batch(i + NB * step, nx, ny);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int k = 0; k < NB; ++k) {
-                float v[8];
+        for (int k = 0; k < NB; ++k) {
+            float v[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = x[k][j];
-                sum_add(ex, p, v);
-                if (both) {
+            for (int j = 0; j < 8; ++j) v[j] = x[k][j];
+            sum_add(ex, p, v);
+            if (both) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = y[k][j];
-                    sum_add(ex, q, v);
-                }
-            }
-        } else {
-            for (int k = i; k < end && k < i + NB * step; k += step) {
-                float v[8], z[8];
-                verify_tile(lr, 1, true, k * kTile, V, lane, none, v);
-                if (both) verify_tile(dr, 1, true, k * kTile, V, lane, none, z);
-                sum_add(ex, p, v);
-                if (both) sum_add(ex, q, z);
+                for (int j = 0; j < 8; ++j) v[j] = y[k][j];
+                sum_add(ex, q, v);
             }
         }
+#pragma unroll
+        for (int k = 0; k < NB; ++k) { x[k] = nx[k]; y[k] = ny[k]; }
+    }
+    for (; i < end; i += step) {
+        float v[8], z[8];
+        verify_tile(lr, 1, true, i * kTile, V, lane, none, v);
+        if (both) verify_tile(dr, 1, true, i * kTile, V, lane, none, z);
+        sum_add(ex, p, v);
+        if (both) sum_add(ex, q, z);
     }
 }
 
@@ -652,7 +701,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(4)))
     __shared__ double parts64[2][WAVES], lds[kTile + kTile / 8], table[32];
     const Exp ex = verify_table(table);
     const int64_t b = blockIdx.x;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = verify_wave(), lane = threadIdx.x & 63;
     const int V = a.V, tiles = (V + kTile - 1) / kTile;
     double* tile_c = tile_a + tiles;
     unsigned char* tile_near = reinterpret_cast<unsigned char*>(tile_c + tiles);
@@ -754,7 +803,7 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_stats_kernel(VerifyAr
     __shared__ Sum parts[2][kSplitWaves];
     __shared__ double table[32];
     const Exp ex = verify_table(table);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = verify_wave(), lane = threadIdx.x & 63;
     const int64_t id = blockIdx.x;
     const int chunk = (int)(id % chunks), group = (int)(id / chunks % groups);
     const int64_t b = id / chunks / groups;
@@ -813,7 +862,7 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_pass_kernel(VerifyArg
     __shared__ int state[kSplitWaves];
     __shared__ double parts64[kSplitWaves], table[32];
     const Exp ex = verify_table(table);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = verify_wave(), lane = threadIdx.x & 63;
     const int64_t b = (int64_t)blockIdx.x / groups;
     const int first = (int)((int64_t)blockIdx.x % groups);
     const int n = verify_length(a, b);
@@ -881,7 +930,7 @@ template <typename T, typename D, bool PROBS>
 __global__ __launch_bounds__(kSplitWaves * 64) void verify_draw_kernel(VerifyArgs a, char* ws) {
     extern __shared__ double tile_a[];                           // per tile of the row: a, c, near
     __shared__ double parts64[2][kSplitWaves], lds[kTile + kTile / 8], table[32];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = verify_wave(), lane = threadIdx.x & 63;
     const int64_t b = blockIdx.x;
     const SplitRow row = split_row(ws, a, b);
     const int tiles = (a.V + kTile - 1) / kTile, n = verify_length(a, b);
