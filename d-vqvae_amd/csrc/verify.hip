@@ -27,9 +27,11 @@ constexpr double kVerifyNoMass = 9.094947017729282e-13;   // 2^-40
 constexpr int kTile = 512;                                // codes of a tile: 8 per lane
 // Relative error of u q / p from sums taken in 32 bits.  A term exp2((x - ref) log2 e) carries |x - ref| 1.5 * 2^-23 from its
 // argument (difference, constant and product rounded) and 2^-23 from the exponential; eight of them are added in 32 bits
-// (3 * 2^-24), everything after that in 64.  ref lies at most kVerifySlack below the largest logit and the mean of
-// |x - ref| under the distribution is at most kVerifySlack + ln V <= 8 + 13.9, so a sum is off by less than
-// 22 * 1.5 * 2^-23 + 2^-23 + 3 * 2^-24 = 4.3e-6 relative, the quotient of two by less than 1e-5.  Four times that:
+// (3 * 2^-24), the eights in 64.  ref lies at most kVerifySlack below the largest logit and the mean of |x - ref| under the
+// distribution is at most kVerifySlack + ln V <= 8 + 13.9, so a lane's sum is off by less than 22 * 1.5 * 2^-23 + 2^-23 + 3 *
+// 2^-24 = 4.3e-6 relative.  Joining lanes, waves and workgroups moves sums by the difference of two such reference points,
+// counted in the mean above, at 2^-23 + 7 * 2^-24 = 5.4e-7 each of three times.  A sum is off by less than 6e-6, the quotient
+// of two by less than 1.2e-5.  More than three times that:
 constexpr double kVerifyMargin = 4e-5;
 constexpr float kVerifySlack = 8.f;
 
@@ -193,35 +195,42 @@ __device__ __forceinline__ void verify_tile(const T* row, int64_t sv, bool unit,
 
 // Reference point and sum of exp(x - ref) of logits seen so far; no distribution: ref = -inf, or s not a number (a NaN or
 // +inf among the logits makes it one).
-struct Sum { float ref; double s; };
+struct Sum { float ref, at; double s; };                          // at: ref, or 0 where ref is -inf
 __device__ __forceinline__ bool sum_ok(const Sum& a) { return a.ref > -__builtin_inff() && a.ref < __builtin_inff() && a.s == a.s; }
 __device__ __forceinline__ double sum_moved(const Exp& ex, const Sum& a, float ref) {        // a.s for reference point ref >= a.ref
     return a.ref > -__builtin_inff() && a.ref < ref ? a.s * ex((double)a.ref - (double)ref) : a.s;
 }
 
-// The reference moves up only where the next eight exceed it by more than kVerifySlack, and then exactly.
-__device__ __forceinline__ void sum_add(const Exp& ex, Sum& a, const float (&x)[8]) {
+// The reference moves up only where the next eight codes of some lane exceed it by more than kVerifySlack: what that lane has
+// summed is then less than e^-8 of what it sums now, and 32 bits are enough to move it.
+__device__ __forceinline__ void sum_add(Sum& a, const float (&x)[8]) {
     float m = x[0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) m = fmaxf(m, x[j]);
-    if (m > a.ref + kVerifySlack) {
-        a.s = sum_moved(ex, a, m);
-        a.ref = m;
+    const bool up = m > a.ref + kVerifySlack;
+    if (__any(up)) {
+        if (up) {
+            a.s *= (double)__builtin_amdgcn_exp2f((a.ref - m) * 1.44269504f);
+            a.ref = m;
+        }
+        a.at = a.ref > -__builtin_inff() ? a.ref : 0.f;              // (nothing but -inf and NaN so far: any point will do)
     }
-    const float ref = a.ref > -__builtin_inff() ? a.ref : 0.f;       // (nothing but -inf and NaN so far)
     float e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f((x[j] - ref) * 1.44269504f);
+    for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f((x[j] - a.at) * 1.44269504f);
     a.s += (double)(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
 }
-__device__ __forceinline__ Sum sum_wave(const Exp& ex, const Sum& a) {
-    const float top = wave_max(a.ref);
-    return Sum{top, wave_sum(sum_moved(ex, a, top))};
+// Sums of several lanes or parts as one, moved to the largest reference point and added in 32 bits; the same in every lane.
+__device__ __forceinline__ Sum sum_join(float ref, double s) {
+    const float top = wave_max(ref);
+    const float f = ref < top ? (float)s * __builtin_amdgcn_exp2f((ref - top) * 1.44269504f) : (float)s;
+    return Sum{top, top, (double)wave_sum(ref > -__builtin_inff() ? f : s == s ? 0.f : __builtin_nanf(""))};
 }
-template <int N>
-__device__ __forceinline__ Sum sum_join(const Exp& ex, const Sum* parts) {         // every wave for itself, all the same
+__device__ __forceinline__ Sum sum_wave(const Sum& a) { return sum_join(a.ref, a.s); }
+__device__ __forceinline__ Sum sum_parts(const Sum* parts, int n) {                // every wave for itself, all the same
     const int lane = threadIdx.x & 63;
-    return sum_wave(ex, lane < N ? parts[lane] : Sum{-__builtin_inff(), 0.0});
+    const Sum t = lane < n ? parts[lane] : Sum{-__builtin_inff(), 0.f, 0.0};
+    return sum_join(t.ref, t.s);
 }
 
 // The test sum of a row that a wave holds: its largest logit is at hand, and the lanes' sums are added in 32 bits (ten
@@ -243,28 +252,38 @@ __device__ __forceinline__ Sum sum_held(const float (&x)[TILES][8]) {
             for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f((x[i][j] - m) * 1.44269504f);
             f += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
         }
-    return Sum{m, (double)wave_sum(f)};
+    return Sum{m, m, (double)wave_sum(f)};
 }
 
 enum { VERIFY_KEEP = 0, VERIFY_REJECT = 1, VERIFY_BAD = 2, VERIFY_UNSURE = 3 };
 
-// What the test of one drafted code reads beside the sums, fetched before them.
-struct Drafted { float t, d; double u; bool inside; };
+// What the tests of a row's drafted codes read beside the sums: lane l holds that of position g0 + l, so that it is asked for
+// once, in front of everything else.  A code outside the table reads the table's end.
 template <typename T, typename D>
-__device__ __forceinline__ Drafted verify_fetch(const VerifyArgs& a, int64_t b, int g) {
-    Drafted f = {0.f, 0.f, 0.0, false};
-    const int64_t x = a.tokens[b * a.tb + g * a.tg];
-    f.u = a.u[b * a.ub + g * a.ug];
-    f.inside = x >= 0 && x < a.V;
-    if (f.inside) {
-        f.t = verify_load(reinterpret_cast<const T*>(a.logits) + b * a.lb + g * a.lp + x * a.lv);
-        f.d = verify_load(reinterpret_cast<const D*>(a.draft) + b * a.db + g * a.dg + x * a.dv);
+struct Drafted {
+    float t, d; double u; int inside;
+    __device__ __forceinline__ void fetch(const VerifyArgs& a, int64_t b, int g0, int n, int lane) {
+        if (g0 >= n) return;
+        const int g = g0 + lane < n ? g0 + lane : n - 1;
+        const int64_t x = a.tokens[b * a.tb + g * a.tg], at = x < 0 ? 0 : x < a.V ? x : a.V - 1;
+        inside = x == at;
+        u = a.u[b * a.ub + g * a.ug];
+        t = verify_load(reinterpret_cast<const T*>(a.logits) + b * a.lb + g * a.lp + at * a.lv);
+        d = verify_load(reinterpret_cast<const D*>(a.draft) + b * a.db + g * a.dg + at * a.dv);
     }
-    return f;
-}
+    __device__ __forceinline__ Drafted of(int l) const {             // lane l's, in every lane
+        Drafted f;
+        f.t = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, t), l));
+        f.d = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, d), l));
+        f.u = verify_lane(u, l);
+        f.inside = __builtin_amdgcn_readlane(inside, l);
+        return f;
+    }
+};
+
 // p, q: sums of the position's logits (q unused with PROBS).  `exact`: the sums were taken in 64 bits.
-template <bool PROBS>
-__device__ __forceinline__ int verify_test(const Exp& ex, const Drafted& f, const Sum& p, const Sum& q, bool exact) {
+template <bool PROBS, typename T, typename D>
+__device__ __forceinline__ int verify_test(const Exp& ex, const Drafted<T, D>& f, const Sum& p, const Sum& q, bool exact) {
     if (!sum_ok(p) || (!PROBS && !sum_ok(q))) return VERIFY_BAD;
     if (!f.inside) return VERIFY_REJECT;
     if (PROBS && !(f.d >= 0.f && f.d < __builtin_inff())) return VERIFY_BAD;
@@ -314,7 +333,7 @@ __device__ __forceinline__ double verify_sum8(const double (&w)[8]) {
 // a code whose sign that k does not settle.
 struct Tile { double mass, c; bool near; };
 
-// One wave.  w.k is within kVerifyMargin / 4 of the true one.
+// One wave.  w.k is within kVerifyMargin / 3 of the true one.
 template <bool PROBS, typename T, typename D>
 __device__ __forceinline__ Tile verify_pass(const Exp& ex, const Weights& w, const T& t, const D& q, double& sp, double& sq) {
     double mass[2] = {0.0, 0.0}, c[2] = {0.0, 0.0}, p2[2] = {0.0, 0.0}, q2[2] = {0.0, 0.0};
@@ -461,8 +480,8 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(TILES == 1
     const int V = a.V;
     const int n = verify_length(a, b);
     const double at_draw = a.r[b * a.rb];
-    Drafted f;
-    if (wave < n) f = verify_fetch<T, D>(a, b, wave);
+    Drafted<T, D> drafted;
+    drafted.fetch(a, b, 0, n, lane);
     const float none = -__builtin_inff();
     T* const staged = reinterpret_cast<T*>(block);
     if (STAGED) {
@@ -482,11 +501,10 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(TILES == 1
     for (int base = 0;; base += waves) {
         const int g = base + wave;                               // n: the position behind all drafts
         float t[TILES][8], q[TILES][8];
-        Drafted ahead;
-        if (g + waves < n) ahead = verify_fetch<T, D>(a, b, g + waves);
+        if (base / 64 != (base - waves) / 64 && base > 0) drafted.fetch(a, b, base / 64 * 64, n, lane);
         const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)g * a.lp;
         const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
-        Sum p = {none, 0.0}, s = {none, 0.0};
+        Sum p = {none, 0.f, 0.0}, s = {none, 0.f, 0.0};
         int st = g == n ? VERIFY_REJECT : VERIFY_KEEP;           // (behind n: not looked at)
         if (g <= n && g < a.P) {
 #pragma unroll
@@ -499,6 +517,7 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(TILES == 1
                 for (int i = 0; i < TILES; ++i) verify_tile(dr, a.dv, a.unit, i * kTile, V, lane, none, q[i]);
             p = sum_held(t);
             if (g < n) {
+                const Drafted<T, D> f = drafted.of(g & 63);
                 if (!PROBS) s = sum_held(q);
                 st = verify_test<PROBS>(ex, f, p, s, false);
                 if (st == VERIFY_UNSURE) {
@@ -527,7 +546,6 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(TILES == 1
             __syncthreads();
             for (stop = 0; stop < waves && state[stop] == VERIFY_KEEP; ++stop) {}
         }
-        f = ahead;
         if (stop == waves) continue;                             // (position n always stops: the loop ends)
         if (wave != stop) return;
         if (lane == 0) a.accepted[b] = g;
@@ -645,52 +663,82 @@ __device__ __forceinline__ void verify_finish(const Exp& ex, const VerifyArgs& a
     if (lane == 0) args.next[b] = at;
 }
 
-// This wave's share of the test sums of tiles first, first + step, .. < end of a row and of its draft's (with `both`), codes
-// side by side.  The loads of a batch of tiles of both rows go out before the batch in front of it is worked on.
-template <typename T, typename D>
-__device__ __forceinline__ void verify_sums(const Exp& ex, const T* lr, const D* dr, bool both, int V, int first, int step, int end, int lane, Sum& p, Sum& q) {
-    constexpr int NB = 2;
-    const float none = -__builtin_inff();
-    const int full = V / kTile < end ? V / kTile : end;         // tiles before `full` hold 512 codes
-    const auto whole = [&](int i) { return i + (NB - 1) * step < full; };
-    const auto batch = [&](int i, Raw<T> (&x)[NB], Raw<D> (&y)[NB]) {
+// Adds eight codes of a row to a lane's sum; those before `skip` are left out.
+template <typename T>
+__device__ __forceinline__ void sum_raw(Sum& a, const Raw<T>& x) {
+    float v[8];
 #pragma unroll
-        for (int k = 0; k < NB; ++k) {
-            x[k].load(lr + (i + k * step) * kTile + 8 * lane);
-            if (both) y[k].load(dr + (i + k * step) * kTile + 8 * lane);
-        }
-    };
-    int i = first;
-    Raw<T> x[NB];
-    Raw<D> y[NB];
-    if (whole(i)) batch(i, x, y);
-    for (; whole(i); i += NB * step) {
-        Raw<T> nx[NB];
-        Raw<D> ny[NB];
-        if (whole(i + NB * step)) batch(i + NB * step, nx, ny);
-        __builtin_amdgcn_sched_barrier(0);
+    for (int j = 0; j < 8; ++j) v[j] = x[j];
+    sum_add(a, v);
+}
+template <typename T>
+__device__ __forceinline__ void sum_raw(Sum& a, const Raw<T>& x, int skip) {
+    float v[8];
 #pragma unroll
-        for (int k = 0; k < NB; ++k) {
-            float v[8];
+    for (int j = 0; j < 8; ++j) v[j] = j < skip ? -__builtin_inff() : x[j];
+    sum_add(a, v);
+}
+
+// Tiles of a row and (Q) of its draft's on their way into registers, a ring of N: while one is worked on, the others are in
+// flight, and behind a position's last tiles the next position's first ones -- asked for before it is known whether the
+// row gets there, N tiles in vain once a row against a memory latency in every position.  No load is left out (one that
+// may be makes the compiler wait for all): where there is nothing to load it is a line that is at hand.
+template <typename T, typename D, bool Q>
+struct Ring {
+    static constexpr int N = sizeof(T) == 2 ? 4 : 2;
+    Raw<T> x[N], tx;                                             // tx, ty: the last 512 codes, for those behind the whole tiles
+    Raw<D> y[N], ty;
+};
+// A wave's tiles of whole rows: wave, wave + step, .. < full; t counts them.
+struct Share {
+    int wave, step, full, cnt, rounds;
+    __device__ __forceinline__ Share(int w, int s, int V, int n)
+        : wave(w), step(s), full(V / kTile), cnt((V / kTile - w + s - 1) / s), rounds(0) {
+        cnt = cnt > 0 ? cnt : 0;
+        rounds = cnt > n ? (cnt + n - 1) / n * n : n;
+    }
+    __device__ __forceinline__ int at(int t, int lane) const {
+        const int tile = wave + t * step;
+        return (tile < full ? tile : full - 1) * kTile + 8 * lane;
+    }
+};
+template <typename T, typename D, bool Q>
+__device__ __forceinline__ void verify_start(Ring<T, D, Q>& ring, const Share& w, const T* lr, const D* dr, bool both, int V, int lane) {
+    ring.tx.load(lr + V - kTile + 8 * lane);
+    if (Q) ring.ty.load(dr + (both ? V - kTile + 8 * lane : 8 * lane));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = x[k][j];
-            sum_add(ex, p, v);
-            if (both) {
+    for (int s = 0; s < Ring<T, D, Q>::N; ++s) {
+        ring.x[s].load(lr + w.at(s, lane));
+        if (Q) ring.y[s].load(dr + (both ? w.at(s, lane) : 8 * lane));
+    }
+}
+// This wave's share of the test sums of one position, whose first tiles the ring holds; nl, nd, nboth: the next position's.
+template <typename T, typename D, bool Q>
+__device__ __forceinline__ void verify_sums(Ring<T, D, Q>& ring, const Share& w, const T* lr, const D* dr, bool both, const T* nl, const D* nd, bool nboth,
+                                            int V, int lane, Sum& p, Sum& q) {
+    constexpr int N = Ring<T, D, Q>::N;
+    for (int i = 0; i < w.rounds; i += N) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = y[k][j];
-                sum_add(ex, q, v);
+        for (int s = 0; s < N; ++s) {
+            if (i + s < w.cnt) {
+                sum_raw(p, ring.x[s]);
+                if (Q && both) sum_raw(q, ring.y[s]);
             }
+            const int t = i + s + N;
+            const bool own = t < w.rounds;
+            const int at = w.at(own ? t : t - w.rounds, lane);
+            ring.x[s].load((own ? lr : nl) + at);
+            if (Q) ring.y[s].load((own ? dr : nd) + ((own ? both : nboth) ? at : 8 * lane));
+            __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int k = 0; k < NB; ++k) { x[k] = nx[k]; y[k] = ny[k]; }
     }
-    for (; i < end; i += step) {
-        float v[8], z[8];
-        verify_tile(lr, 1, true, i * kTile, V, lane, none, v);
-        if (both) verify_tile(dr, 1, true, i * kTile, V, lane, none, z);
-        sum_add(ex, p, v);
-        if (both) sum_add(ex, q, z);
+    if (w.full * kTile < V && w.full % w.step == w.wave) {
+        const int skip = w.full * kTile - (V - kTile) - 8 * lane;
+        sum_raw(p, ring.tx, skip);
+        if (Q && both) sum_raw(q, ring.ty, skip);
     }
+    ring.tx.load(nl + V - kTile + 8 * lane);
+    if (Q) ring.ty.load(nd + (nboth ? V - kTile + 8 * lane : 8 * lane));
 }
 
 // Codes side by side (a.unit).
@@ -708,25 +756,34 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(4)))
     const int n = verify_length(a, b);
     const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb;
     const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db;
-    Sum p = {0.f, 1.0}, q = {0.f, 1.0};
+    Sum p = {0.f, 0.f, 1.0}, q = {0.f, 0.f, 1.0};
     int g = 0, st = VERIFY_KEEP;
-    for (; g < a.P && g <= n; ++g, lr += a.lp, dr += a.dg) {
-        const bool both = !PROBS && g < n;
-        Drafted f;
-        if (g < n) f = verify_fetch<T, D>(a, b, g);
-        p = q = Sum{-__builtin_inff(), 0.0};
-        verify_sums(ex, lr, dr, both, V, wave, WAVES, tiles, lane, p, q);
-        p = sum_wave(ex, p);
-        if (both) q = sum_wave(ex, q);
+    Drafted<T, D> drafted;
+    drafted.fetch(a, b, 0, n, lane);
+    const Share share(wave, WAVES, V, Ring<T, D, !PROBS>::N);
+    Ring<T, D, !PROBS> ring;
+    if (a.G == 0) dr = reinterpret_cast<const D*>(lr);           // (read in vain, and 512 codes of either type fit a row)
+    verify_start(ring, share, lr, dr, n > 0, V, lane);
+    for (; g < a.P && g <= n; ++g) {
+        const bool both = !PROBS && g < n, more = g + 1 < a.P && g + 1 <= n, nboth = !PROBS && g + 1 < n;
+        const T* nl = more ? lr + a.lp : lr;
+        const D* nd = g + 1 < n ? dr + a.dg : dr;
+        if (g > 0 && g % 64 == 0) drafted.fetch(a, b, g, n, lane);
+        p = q = Sum{-__builtin_inff(), 0.f, 0.0};
+        verify_sums(ring, share, lr, dr, both, nl, nd, nboth, V, lane, p, q);
+        __builtin_amdgcn_sched_barrier(0);
+        p = sum_wave(p);
+        if (both) q = sum_wave(q);
         Sum (*at)[WAVES] = parts[g & 1];                         // (in turns: one barrier a position)
         if (lane == 0) { at[0][wave] = p; at[1][wave] = q; }
         __syncthreads();
-        p = sum_join<WAVES>(ex, at[0]);
-        if (both) q = sum_join<WAVES>(ex, at[1]);
+        p = sum_parts(at[0], WAVES);
+        if (both) q = sum_parts(at[1], WAVES);
         if (g == n) {                                            // every draft kept: one more code
             st = sum_ok(p) ? VERIFY_REJECT : VERIFY_BAD;
             break;
         }
+        const Drafted<T, D> f = drafted.of(g & 63);
         st = verify_test<PROBS>(ex, f, p, q, false);             // (the same for every thread: one code's values)
         if (st == VERIFY_UNSURE) {
             p.s = verify_row_sum64(ex, lr, 1, true, V, (double)p.ref, parts64[0]);
@@ -734,6 +791,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(4)))
             st = verify_test<PROBS>(ex, f, p, q, true);
         }
         if (st != VERIFY_KEEP) break;
+        lr = nl;
+        dr = nd;
     }
     if (threadIdx.x == 0) a.accepted[b] = g;
     if (st != VERIFY_REJECT) {
@@ -743,18 +802,34 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(4)))
     const Weights w = {(double)p.ref, (double)q.ref, PROBS ? p.s : p.s / q.s, g < n};
     double sp = 0.0, sq = 0.0;
     const float none = -__builtin_inff();
-    float t[8], d[8];
-    verify_tile(lr, 1, true, wave * kTile, V, lane, none, t);
-    if (w.residual) verify_tile(dr, 1, true, wave * kTile, V, lane, PROBS ? 0.f : none, d);
-    for (int i = wave; i < tiles; i += WAVES) {
-        float x[8], y[8];                                        // the next tile is on its way during the work on this one
-        verify_tile(lr, 1, true, (i + WAVES) * kTile, V, lane, none, x);
-        if (w.residual) verify_tile(dr, 1, true, (i + WAVES) * kTile, V, lane, PROBS ? 0.f : none, y);
-        __builtin_amdgcn_sched_barrier(0);
-        const Tile r = verify_pass<PROBS>(ex, w, t, d, sp, sq);
-        if (lane == 0) { tile_a[i] = r.mass; tile_c[i] = r.c; tile_near[i] = r.near; }
+    // two tiles in turns, as in verify_sums
+    Raw<T> t[2];
+    Raw<D> d[2];
+    const auto load = [&](int k, int i) {
+        i = i < tiles ? i : tiles - 1;
+        const int at = verify_base(true, i * kTile, V) + 8 * lane;
+        t[k].load(lr + at);
+        d[k].load(dr + (w.residual ? at : 8 * lane));
+    };
+    const auto pass = [&](int k, int i) {
+        const int skip = i * kTile - verify_base(true, i * kTile, V) - 8 * lane;
+        float x[8], y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { t[j] = x[j]; d[j] = y[j]; }
+        for (int j = 0; j < 8; ++j) {
+            x[j] = j < skip ? none : t[k][j];
+            y[j] = j < skip ? (PROBS ? 0.f : none) : d[k][j];
+        }
+        const Tile r = verify_pass<PROBS>(ex, w, x, y, sp, sq);
+        if (lane == 0) { tile_a[i] = r.mass; tile_c[i] = r.c; tile_near[i] = r.near; }
+    };
+    load(0, wave);
+    for (int i = wave; i < tiles; i += 2 * WAVES) {
+        load(1, i + WAVES);
+        __builtin_amdgcn_sched_barrier(0);
+        pass(0, i);
+        load(0, i + 2 * WAVES);
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + WAVES < tiles) pass(1, i + WAVES);
     }
     sp = wave_sum(sp);
     sq = wave_sum(sq);
@@ -814,27 +889,48 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_stats_kernel(VerifyAr
         const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)g * a.lp;
         const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
         const bool both = !PROBS && g < n;
-        Sum p = {-__builtin_inff(), 0.0}, q = p;
+        Sum p = {-__builtin_inff(), 0.f, 0.0}, q = p;
         const int tiles = (a.V + kTile - 1) / kTile, last = (chunk + 1) * kChunk < tiles ? (chunk + 1) * kChunk : tiles;
-        if (a.unit) verify_sums(ex, lr, dr, both, a.V, chunk * kChunk + wave, kSplitWaves, last, lane, p, q);
+        if (a.unit) {
+            constexpr int N = kChunk / kSplitWaves;              // this wave's tiles, all asked for at once
+            Raw<T> x[N];
+            Raw<D> y[N];
+            int at[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int i = chunk * kChunk + wave + k * kSplitWaves;
+                at[k] = verify_base(true, (i < tiles ? i : tiles - 1) * kTile, a.V) + 8 * lane;
+                x[k].load(lr + at[k]);
+            }
+            if (both)
+#pragma unroll
+                for (int k = 0; k < N; ++k) y[k].load(dr + at[k]);
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int i = chunk * kChunk + wave + k * kSplitWaves;
+                if (i >= last) continue;
+                sum_raw(p, x[k], i * kTile - at[k]);
+                if (both) sum_raw(q, y[k], i * kTile - at[k]);
+            }
+        }
         else
             for (int i = chunk * kChunk + wave; i < last; i += kSplitWaves) {
                 float x[8];
                 verify_tile(lr, a.lv, false, i * kTile, a.V, lane, -__builtin_inff(), x);
-                sum_add(ex, p, x);
+                sum_add(p, x);
                 if (both) {
                     verify_tile(dr, a.dv, false, i * kTile, a.V, lane, -__builtin_inff(), x);
-                    sum_add(ex, q, x);
+                    sum_add(q, x);
                 }
             }
-        p = sum_wave(ex, p);
-        if (both) q = sum_wave(ex, q);
+        p = sum_wave(p);
+        if (both) q = sum_wave(q);
         __syncthreads();
         if (lane == 0) { parts[0][wave] = p; parts[1][wave] = q; }
         __syncthreads();
         if (wave == 0) {
-            p = sum_join<kSplitWaves>(ex, parts[0]);
-            q = sum_join<kSplitWaves>(ex, parts[1]);
+            p = sum_parts(parts[0], kSplitWaves);
+            q = sum_parts(parts[1], kSplitWaves);
             if (lane == 0) {
                 row.p[g * chunks + chunk] = p;
                 if (both) row.q[g * chunks + chunk] = q;
@@ -844,14 +940,14 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_stats_kernel(VerifyAr
 }
 
 __device__ __forceinline__ Sum split_join(const Exp& ex, const Sum* parts, int chunks, int lane) {       // one wave
-    Sum a = {-__builtin_inff(), 0.0};
+    Sum a = {-__builtin_inff(), 0.f, 0.0};
     for (int i = lane; i < chunks; i += 64) {
         const Sum t = parts[i];
         const float top = fmaxf(a.ref, t.ref);
         a.s = sum_moved(ex, a, top) + sum_moved(ex, t, top);
         a.ref = top;
     }
-    return sum_wave(ex, a);
+    return sum_wave(a);
 }
 
 // One tile per wave of the position that stops the row.  Every workgroup finds that position for itself from the chunks' sums,
@@ -867,18 +963,19 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_pass_kernel(VerifyArg
     const int first = (int)((int64_t)blockIdx.x % groups);
     const int n = verify_length(a, b);
     const SplitRow row = split_row(ws, a, b);
-    Sum p = {0.f, 1.0}, q = {0.f, 1.0};
+    Sum p = {0.f, 0.f, 1.0}, q = {0.f, 0.f, 1.0};
     int st = VERIFY_KEEP, g = 0;
+    Drafted<T, D> drafted;
+    drafted.fetch(a, b, 0, n, lane);
     for (int base = 0; st == VERIFY_KEEP; base += kSplitWaves) {
         const int mine = base + wave;
         int s = mine == n ? (n < a.P ? VERIFY_REJECT : VERIFY_BAD) : VERIFY_KEEP;
         if (mine <= n && mine < a.P) {
-            Drafted f;
-            if (mine < n) f = verify_fetch<T, D>(a, b, mine);
+            if (base / 64 != (base - kSplitWaves) / 64 && base > 0) drafted.fetch(a, b, base / 64 * 64, n, lane);
             p = split_join(ex, row.p + mine * chunks, chunks, lane);
             if (mine < n) {
                 if (!PROBS) q = split_join(ex, row.q + mine * chunks, chunks, lane);
-                s = verify_test<PROBS>(ex, f, p, q, false);
+                s = verify_test<PROBS>(ex, drafted.of(mine & 63), p, q, false);
             } else if (!sum_ok(p)) s = VERIFY_BAD;
         }
         __syncthreads();
@@ -895,7 +992,7 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_pass_kernel(VerifyArg
                 const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
                 p.s = verify_row_sum64(ex, lr, a.lv, a.unit, a.V, (double)p.ref, parts64);
                 if (!PROBS) q.s = verify_row_sum64(ex, dr, a.dv, a.unit, a.V, (double)q.ref, parts64);
-                st = verify_test<PROBS>(ex, verify_fetch<T, D>(a, b, g), p, q, true);
+                st = verify_test<PROBS>(ex, drafted.of(g & 63), p, q, true);
             }
         }
     }
