@@ -31,14 +31,14 @@ struct Int8Batch {
     void* y[kInt8MaxBatch];
 };
 
-// Code of x in a row whose factor is inv = 127 / a in 64 bits: the nearest whole number to the EXACT quotient 127 x / a,
-// ties to even.  x * inv is off by at most 2^-46 (|quotient| <= 127).  A quotient that is not a half differs from every
-// half by at least 2^-34 (x and a have 24-bit significands, and near a half at most 8 binary places lie between them),
-// so rounding to multiples of 2^-40 first (adding and taking away 1.5 * 2^12 does that) makes a true tie exact and
-// moves nothing else across one.
-__device__ __forceinline__ int int8_code(float x, double inv) {
-    const double t = ((double)x * inv + 6144.0) - 6144.0;
-    return (int)rint(t);
+// Code of x in a row whose factor is inv = 127 / a in 64 bits, in the low 8 bits: the nearest whole number to the EXACT quotient
+// 127 x / a, ties to even.  The first sum rounds x * inv to a multiple of 2^-40 (6144 = 1.5 * 2^12): the product is off by
+// 2^-46 at most, and a quotient that is not a half differs from every half by at least 2^-34 (x and a have 24-bit
+// significands, and near a half at most 8 binary places lie between them), so a true tie becomes exact and nothing else
+// moves across one.  The second rounds to the whole number and leaves it in the low bits.
+__device__ __forceinline__ unsigned int8_code(float x, double inv) {
+    const double t = __builtin_fma((double)x, inv, 6144.0) + (6755399441055744.0 - 6144.0);
+    return (unsigned)__builtin_bit_cast(unsigned long long, t);
 }
 
 // 16 bytes of a row from byte k on, zeros behind the row's end; any alignment, never reads outside the row.
@@ -103,11 +103,11 @@ __device__ __forceinline__ double int8_inv(unsigned top, float& scale) {
     return finite && top > 0 ? 127.0 / amax : 0.0;
 }
 __device__ __forceinline__ unsigned int8_codes4(f32x4 v, double inv) {
-    if (!(inv > 0.0)) return 0;
-    unsigned c = 0;
+    unsigned c[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c |= (unsigned)(int8_code(v[j], inv) & 0xFF) << (8 * j);
-    return c;
+    for (int j = 0; j < 4; ++j) c[j] = int8_code(v[j], inv);
+    const unsigned lo = __builtin_amdgcn_perm(c[1], c[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000C0Cu);
+    return inv > 0.0 ? lo | hi : 0u;
 }
 
 // One wave per row; rows of up to kInt8Held features are read once and stay in registers between the maximum and the codes.
@@ -173,56 +173,76 @@ __device__ __forceinline__ float int8_scale(int acc, float s, float t, float b, 
 __device__ __forceinline__ void int8_store(float* y, float v) { *y = v; }
 __device__ __forceinline__ void int8_store(unsigned short* y, float v) { *y = f32_to_bf16_bits(v); }
 
-// Few rows: a workgroup takes 16 output channels of up to 16 rows over the whole of k, split among its eight waves, and
-// adds the waves' sums in LDS.  Every weight byte is read once, straight into the operand registers of the 16x16x64
-// instruction, and is requested before the rows are quantised -- by every workgroup for itself into LDS (16-byte pieces
-// of row r at piece ^ (r & 7), so that the eight rows of a read phase lie in different banks): the whole layer is one
-// launch.  K <= kInt8Held.
-template <typename T, typename Y>
+// 16 elements of a row from element k on (k % 16 == 0), zeros behind the row's end.
+template <typename T>
+__device__ __forceinline__ void int8_load16(const T* x, int k, int K, bool wide, f32x4 (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = int8_load4(x, k + 4 * j, K, wide);
+}
+
+// Few rows: a workgroup takes 16 output channels of up to 16 rows over the whole of k, cut among its eight waves, and adds
+// the waves' sums in LDS; the rows are quantised by every workgroup for itself, so that the layer is one launch.  A wave
+// reads weights and activations of its own share of k straight in the operand layout of the 16x16x64 instruction (lane l: 16
+// consecutive k of row l % 16) and quantises in registers; all that the waves exchange before the products is the rows'
+// maxima.  STEPS: blocks of 64 k per wave; K <= 512 STEPS.
+template <int STEPS, typename T, typename Y>
 __global__ __launch_bounds__(512) void int8_rows16_kernel(Int8Batch p, int64_t ldx, int64_t ldw, int M, int K, int N, int relu, int64_t ldy) {
-    extern __shared__ __align__(16) int8_t smem[];
+    __shared__ unsigned tops[8][16];
     __shared__ float sc[16];
+    __shared__ __align__(16) int red[8 * 256];
     const int bz = blockIdx.y, n0 = (int)blockIdx.x * 16;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int Kp = (K + 127) / 128 * 128, steps = Kp / 64;
-    const int wr = n0 + (lane & 15) < N ? n0 + (lane & 15) : N - 1;
+    const int r = lane & 15, kl = 64 * wave + 16 * (lane >> 4);
+    const int wr = n0 + r < N ? n0 + r : N - 1;
     const int8_t* w = p.W[bz] + (int64_t)wr * ldw;
-    i32x4 wf[kInt8Held / 512];
+    const T* x = reinterpret_cast<const T*>(p.x[bz]) + (int64_t)(r < M ? r : M - 1) * ldx;
+    const bool wide = (reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T))) == 0;
+    i32x4 wf[STEPS];
+    f32x4 v[STEPS][4];
+    unsigned a = 0;
+    if (K % 16 == 0 && __all(wide)) {
+        // whole pieces: a lane behind the row's end reads its last piece, and its weights are zeros
 #pragma unroll
-    for (int i = 0; i < kInt8Held / 512; ++i)
-        if (wave + 8 * i < steps) wf[i] = int8_chunk(w, 64 * (wave + 8 * i) + 16 * (lane >> 4), K);
-    for (int r = wave; r < M; r += 8) {
-        const T* x = reinterpret_cast<const T*>(p.x[bz]) + r * ldx;
-        const bool wide = (reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T))) == 0;
-        f32x4 v[kInt8Held / 256];
-        unsigned a = 0;
+        for (int i = 0; i < STEPS; ++i) {
+            const int k = kl + 512 * i, at = k < K ? k : K - 16;
+            __builtin_memcpy(&wf[i], w + at, 16);
+            int8_load16(x, at, K, true, v[i]);
+        }
 #pragma unroll
-        for (int i = 0; i < kInt8Held / 256; ++i)
-            if (i * 256 < K) v[i] = int8_load4(x, i * 256 + lane * 4, K, wide);
+        for (int i = 0; i < STEPS; ++i) {
+            if (kl + 512 * i >= K) wf[i] = i32x4{0, 0, 0, 0};
+        }
+    } else {
 #pragma unroll
-        for (int i = 0; i < kInt8Held / 256; ++i)
-            if (i * 256 < K) a = int8_top(a, v[i]);
-        float s;
-        const double inv = int8_inv(wave_top(a), s);
-        if (lane == 0) sc[r] = s;
-#pragma unroll
-        for (int i = 0; i < kInt8Held / 256; ++i) {
-            const int k = i * 256 + lane * 4;
-            if (i * 256 < K && k < Kp) *reinterpret_cast<unsigned*>(smem + r * Kp + (((k >> 4) ^ (r & 7)) << 4) + (k & 15)) = int8_codes4(v[i], inv);
+        for (int i = 0; i < STEPS; ++i) {
+            wf[i] = int8_chunk(w, kl + 512 * i, K);
+            int8_load16(x, kl + 512 * i, K, wide, v[i]);
         }
     }
-    __syncthreads();
-    i32x4 acc = {0, 0, 0, 0};
-    const int r = lane & 15;                    // (rows beyond M hold whatever was there: they reach outputs beyond M only)
 #pragma unroll
-    for (int i = 0; i < kInt8Held / 512; ++i)
-        if (wave + 8 * i < steps) {
-            const int piece = 4 * (wave + 8 * i) + (lane >> 4);
-            const i32x4 xf = *reinterpret_cast<const i32x4*>(smem + r * Kp + ((piece ^ (r & 7)) << 4));
-            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[i], xf, acc, 0, 0, 0);
-        }
+    for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a = int8_top(a, v[i][j]);
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1) {
+        const unsigned other = __shfl_xor(a, o, 64);
+        a = other > a ? other : a;
+    }
+    if (lane < 16) tops[wave][lane] = a;
     __syncthreads();
-    int* red = reinterpret_cast<int*>(smem);
+#pragma unroll
+    for (int g = 0; g < 8; ++g) a = tops[g][r] > a ? tops[g][r] : a;
+    float s;
+    const double inv = int8_inv(a, s);
+    if (tid < 16) sc[tid] = s;
+    i32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+        i32x4 xf;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xf[j] = (int)int8_codes4(v[i][j], inv);
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[i], xf, acc, 0, 0, 0);
+    }
     *reinterpret_cast<i32x4*>(red + wave * 256 + lane * 4) = acc;
     __syncthreads();
     if (tid >= 256) return;
@@ -233,6 +253,14 @@ __global__ __launch_bounds__(512) void int8_rows16_kernel(Int8Batch p, int64_t l
     for (int g = 0; g < 8; ++g) sum += red[g * 256 + (m + 16 * (n >> 2)) * 4 + (n & 3)];
     int8_store(reinterpret_cast<Y*>(p.y[bz]) + m * ldy + n0 + n,
                int8_scale(sum, sc[m], p.ws[bz][n0 + n], p.b[bz] ? p.b[bz][n0 + n] : 0.f, relu));
+}
+template <typename T, typename Y>
+static int int8_rows16(const Int8Batch& p, int n_batch, int64_t ldx, int64_t ldw, int M, int K, int N, int relu, int64_t ldy, hipStream_t st) {
+    const dim3 grid((unsigned)((N + 15) / 16), (unsigned)n_batch), blk(512);
+    if (K <= 1024) hipLaunchKernelGGL((int8_rows16_kernel<2, T, Y>), grid, blk, 0, st, p, ldx, ldw, M, K, N, relu, ldy);
+    else if (K <= 2560) hipLaunchKernelGGL((int8_rows16_kernel<5, T, Y>), grid, blk, 0, st, p, ldx, ldw, M, K, N, relu, ldy);
+    else hipLaunchKernelGGL((int8_rows16_kernel<8, T, Y>), grid, blk, 0, st, p, ldx, ldw, M, K, N, relu, ldy);
+    return check_launch("linear_int8");
 }
 
 // Rows quantised before, few tiles: 16 channels x 16 RM rows per workgroup over the whole of k, split among eight waves; both
@@ -435,7 +463,7 @@ extern "C" int dvq_int8_quantize_rows(const void* x, int dtype, int64_t ldx, int
     return check_launch("int8_quantize_rows");
 }
 
-extern "C" int dvq_linear_int8(int n_batch, const void* const* x, int x_dtype, const float* const* xs, int64_t ldx, const void* const* W,
+extern "C" int dvq_linear_int8_batched(int n_batch, const void* const* x, int x_dtype, const float* const* xs, int64_t ldx, const void* const* W,
                                const float* const* ws, int64_t ldw, const float* const* b, int M, int K, int N, int relu,
                                void* const* y, int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
     if (n_batch < 1 || n_batch > kInt8MaxBatch) return fail(DVQ_EINVAL, "linear_int8: 1..%d products per launch", kInt8MaxBatch);
@@ -459,17 +487,12 @@ extern "C" int dvq_linear_int8(int n_batch, const void* const* x, int x_dtype, c
     hipStream_t st = as_stream(stream);
     const bool f32 = y_dtype == DVQ_F32;
     if (!codes && int8_one_launch(M, K)) {
-        const int Kp = (K + 127) / 128 * 128;
-        const size_t lds = (size_t)16 * Kp > 8192 ? (size_t)16 * Kp : 8192;      // <= 64 KiB
-        const dim3 grid((unsigned)((N + 15) / 16), (unsigned)n_batch), blk(512);
-        if (x_dtype == DVQ_F32) {
-            if (f32) hipLaunchKernelGGL((int8_rows16_kernel<float, float>), grid, blk, lds, st, p, ldx, ldw, M, K, N, relu, ldy);
-            else hipLaunchKernelGGL((int8_rows16_kernel<float, unsigned short>), grid, blk, lds, st, p, ldx, ldw, M, K, N, relu, ldy);
-        } else {
-            if (f32) hipLaunchKernelGGL((int8_rows16_kernel<unsigned short, float>), grid, blk, lds, st, p, ldx, ldw, M, K, N, relu, ldy);
-            else hipLaunchKernelGGL((int8_rows16_kernel<unsigned short, unsigned short>), grid, blk, lds, st, p, ldx, ldw, M, K, N, relu, ldy);
-        }
-        return check_launch("linear_int8");
+        typedef unsigned short u16;
+        if (x_dtype == DVQ_F32)
+            return f32 ? int8_rows16<float, float>(p, n_batch, ldx, ldw, M, K, N, relu, ldy, st)
+                       : int8_rows16<float, u16>(p, n_batch, ldx, ldw, M, K, N, relu, ldy, st);
+        return f32 ? int8_rows16<u16, float>(p, n_batch, ldx, ldw, M, K, N, relu, ldy, st)
+                   : int8_rows16<u16, u16>(p, n_batch, ldx, ldw, M, K, N, relu, ldy, st);
     }
     // What the tiles cannot read in place -- features to quantise, rows that do not start at multiples of 16 bytes -- is
     // laid out in the workspace by one launch.
@@ -506,4 +529,9 @@ extern "C" int dvq_linear_int8(int n_batch, const void* const* x, int x_dtype, c
     }
     return f32 ? int8_product<float>(p, n_batch, ldx, ldw, M, Kt, N, relu, ldy, tiles, st)
                : int8_product<unsigned short>(p, n_batch, ldx, ldw, M, Kt, N, relu, ldy, tiles, st);
+}
+
+extern "C" int dvq_linear_int8(const void* x, int x_dtype, const float* xs, int64_t ldx, const void* W, const float* ws, int64_t ldw, const float* b,
+                               int M, int K, int N, int relu, void* y, int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
+    return dvq_linear_int8_batched(1, &x, x_dtype, &xs, ldx, &W, &ws, ldw, &b, M, K, N, relu, &y, y_dtype, ldy, workspace, workspace_bytes, stream);
 }

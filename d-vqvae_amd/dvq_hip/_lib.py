@@ -95,11 +95,14 @@ SIGNATURES = {
     "dvq_linear_bf16": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p]),
     "dvq_int8_quantize_rows": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p]),
     "dvq_linear_int8_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
-    "dvq_linear_int8": (c_int, [c_int, POINTER(c_void_p), c_int, POINTER(c_void_p), c_int64, POINTER(c_void_p), POINTER(c_void_p), c_int64,
-                                POINTER(c_void_p), c_int, c_int, c_int, c_int, POINTER(c_void_p), c_int, c_int64, c_void_p, c_size_t,
-                                c_void_p]),
-    "dvq_prior_verify_workspace_bytes": (c_size_t, [POINTER(DvqPriorVerify)]),
-    "dvq_prior_verify": (c_int, [POINTER(DvqPriorVerify), c_void_p, c_size_t, c_void_p]),
+    "dvq_linear_int8": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int,
+                                c_void_p, c_int, c_int64, c_void_p, c_size_t, c_void_p]),
+    "dvq_linear_int8_batched": (c_int, [c_int, POINTER(c_void_p), c_int, POINTER(c_void_p), c_int64, POINTER(c_void_p), POINTER(c_void_p),
+                                        c_int64, POINTER(c_void_p), c_int, c_int, c_int, c_int, POINTER(c_void_p), c_int, c_int64,
+                                        c_void_p, c_size_t, c_void_p]),
+    # (the DvqPriorVerify structure, or its bytes)
+    "dvq_prior_verify_workspace_bytes": (c_size_t, [c_void_p]),
+    "dvq_prior_verify": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "dvq_prior_packed_bytes": (c_size_t, [c_int, c_int, c_int]),
     "dvq_prior_pack_weight": (c_int, [c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_void_p]),
     "dvq_prior_embed": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),

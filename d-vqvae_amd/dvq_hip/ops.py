@@ -7,6 +7,7 @@ to live on a HIP device and raises otherwise -- there is no CPU path.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -333,34 +334,42 @@ def linear_batched(xs, Ws, bs, relu: bool = False, add_identity3: bool = False, 
 INT8_MAX_K = (1 << 17) - 1       # longest sum of products of 8-bit codes that 32 bits hold exactly
 
 
+# The current stream's handle, without the Stream object around it where torch offers that (1.5 us less per call).
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _launch(fn, name: str, dev: torch.device, *args) -> None:
     """Call a C entry with `dev` current and torch's stream of that device as the last argument."""
-    st = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        rc = fn(*args, st)
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, _current_stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, st)
-    _lib.check(rc, name)
+            rc = fn(*args, _current_stream(dev.index))
+    if rc != 0:
+        _lib.check(rc, name)
 
 
-def _rows(t: torch.Tensor, what: str, dtypes, dev=None):
-    """Row stride of a 2-D HIP tensor with unit inner stride."""
-    if t.dim() != 2 or t.dtype not in dtypes:
-        raise RuntimeError(f"{what} must be a 2-D tensor of {' or '.join(str(d) for d in dtypes)}, got {tuple(t.shape)} {t.dtype}")
+_INT8, _FLOATS = (torch.int8,), (torch.float32, torch.bfloat16)
+_CODES = {torch.float32: DVQ_F32, torch.bfloat16: DVQ_BF16, torch.int8: DVQ_I8}
+
+
+def _rows(t: torch.Tensor, dtypes, dev, what: str, name: str) -> int:
+    """Row stride of a 2-D HIP tensor with unit inner stride, on `dev` unless that is None."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or t.dtype not in dtypes:
+        raise RuntimeError(f"{what}: {name} must be a 2-D tensor of {' or '.join(str(d) for d in dtypes)}, got {tuple(shape)} {t.dtype}")
     if not t.is_cuda:
         raise RuntimeError("dvq_hip kernels need tensors on a HIP device (got a CPU tensor); there is no CPU fallback")
     if dev is not None and t.device != dev:
-        raise RuntimeError(f"{what} is on {t.device}, the other operands on {dev}")
-    n, w = t.shape
-    if w > 1 and t.stride(1) != 1:
-        raise RuntimeError(f"{what} must have unit inner stride")
-    return t.stride(0) if n > 1 else max(w, 1)
+        raise RuntimeError(f"{what}: {name} is on {t.device}, the other operands on {dev}")
+    if shape[1] > 1 and stride[1] != 1:
+        raise RuntimeError(f"{what}: {name} must have unit inner stride")
+    return stride[0] if shape[0] > 1 else max(shape[1], 1)
 
 
-def _vector(t: torch.Tensor, what: str, n: int, dev) -> None:
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != dev:
-        raise RuntimeError(f"{what} must be a contiguous float32 [{n}] on {dev}")
+def _vector(t: torch.Tensor, n: int, dev, what: str, name: str) -> None:
+    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous() or t.device != dev:
+        raise RuntimeError(f"{what}: {name} must be a contiguous float32 [{n}] on {dev}")
 
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -369,7 +378,7 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     zeros has codes and scale 0; a row with an infinity or a NaN has codes 0 and scale NaN.  Rows of activations (a scale
     per token) and of weights [N,K] (a scale per output channel) are quantised alike.  The rows of the codes start at
     multiples of 64 bytes, where linear_int8 reads them in place."""
-    ldx = _rows(x, "quantize_rows: x", (torch.float32, torch.bfloat16))
+    ldx = _rows(x, _FLOATS, None, "quantize_rows", "x")
     M, K = x.shape
     if not 1 <= K <= INT8_MAX_K:
         raise RuntimeError(f"quantize_rows: 1..{INT8_MAX_K} features per row, got {K}")
@@ -389,68 +398,97 @@ def linear_int8(x, W: torch.Tensor, w_scale: torch.Tensor, b: Optional[torch.Ten
     scale float32 [M]) quantised before.  The sums are exact in 32-bit integers; scaling and bias are rounded once to the
     output's type, float32 or bfloat16.  `out` [M,N] may be a column slice of a wider row-major buffer (not of x's).
     Inference only: no gradient flows through the codes."""
-    if out is not None:
-        out_dtype = out.dtype
-    return _linear_int8([x], [W], [w_scale], [b], relu, out, out_dtype, "linear_int8")[0]
+    what = "linear_int8"
+    sx = None
+    if isinstance(x, (tuple, list)):
+        x, sx = x
+    ldx = _rows(x, _FLOATS if sx is None else _INT8, None, what, "x")
+    M, K = x.shape
+    dev = x.device
+    ldw, N = _int8_layer(W, w_scale, b, K, dev, what)
+    if sx is not None:
+        _vector(sx, M, dev, what, "the scale of x")
+    if out is None:
+        out = _int8_out(M, N, out_dtype, dev, what)
+        ldy = N
+    else:
+        ldy = _rows(out, _FLOATS, dev, what, "out")
+        if out.shape != (M, N) or ldy < N:
+            raise RuntimeError(f"{what}: out must be [{M},{N}] with rows that do not overlap")
+        if out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr() and M > 0:
+            raise RuntimeError(f"{what}: out must not lie in the memory of x")
+    if M == 0 or N == 0:
+        return out
+    lib = _lib.load()
+    ws, nbytes = _int8_workspace(lib, 1, M, K, N, sx is not None, dev)
+    _launch(lib.dvq_linear_int8, "dvq_linear_int8", dev, x.data_ptr(), _CODES[x.dtype], None if sx is None else sx.data_ptr(), ldx,
+            W.data_ptr(), w_scale.data_ptr(), ldw, None if b is None else b.data_ptr(), M, K, N, int(relu), out.data_ptr(),
+            _CODES[out.dtype], ldy, None if ws is None else ws.data_ptr(), nbytes)
+    return out
 
 
 def linear_int8_batched(xs, Ws, w_scales, bs, relu: bool = False, out_dtype: torch.dtype = torch.float32) -> list:
     """Several linear_int8() calls of one shape -- own x, W, w_scale and b each -- in one launch (up to 8)."""
-    n = len(xs)
+    n, what = len(xs), "linear_int8_batched"
     if not 1 <= n <= 8 or len(Ws) != n or len(w_scales) != n or len(bs) != n:
-        raise RuntimeError("linear_int8_batched: 1..8 products, one x, W, w_scale and b (or None) each")
-    return _linear_int8(list(xs), Ws, w_scales, bs, relu, None, out_dtype, "linear_int8_batched")
-
-
-def _linear_int8(xs, Ws, w_scales, bs, relu, out, out_dtype, what):
+        raise RuntimeError(f"{what}: 1..8 products, one x, W, w_scale and b (or None) each")
     pairs = isinstance(xs[0], (tuple, list))
     if any(isinstance(x, (tuple, list)) != pairs for x in xs):
         raise RuntimeError(f"{what}: either all x are quantised already or none")
-    if out_dtype not in (torch.float32, torch.bfloat16):
-        raise RuntimeError(f"{what}: output of float32 or bfloat16, not {out_dtype}")
-    feats, scales = [x[0] for x in xs] if pairs else xs, [x[1] for x in xs] if pairs else [None] * len(xs)
+    feats = [x[0] for x in xs] if pairs else xs
     first = feats[0]
-    ldx = _rows(first, f"{what}: x", (torch.int8,) if pairs else (torch.float32, torch.bfloat16))
+    ldx = _rows(first, _INT8 if pairs else _FLOATS, None, what, "x")
     M, K = first.shape
     dev = first.device
-    if not 1 <= K <= INT8_MAX_K:
-        raise RuntimeError(f"{what}: 1..{INT8_MAX_K} features per row, got {K}")
-    ldw = _rows(Ws[0], f"{what}: W", (torch.int8,), dev)
-    N = Ws[0].shape[0]
-    for x, sx, W, sw, b in zip(feats, scales, Ws, w_scales, bs):
-        if x is not first and (_rows(x, f"{what}: x", (first.dtype,), dev) != ldx or x.shape != first.shape):
-            raise RuntimeError(f"{what}: all x must have one shape, type and row stride")
-        if sx is not None:
-            _vector(sx, f"{what}: the scale of x", M, dev)
-        if _rows(W, f"{what}: W", (torch.int8,), dev) != ldw or W.shape != (N, K):
-            raise RuntimeError(f"{what}: W must be int8 [{N},{K}] (all of one row stride), got {tuple(W.shape)}")
-        _vector(sw, f"{what}: w_scale", N, dev)
-        if b is not None:
-            _vector(b, f"{what}: b", N, dev)
-    if out is not None:
-        ldy = _rows(out, f"{what}: out", (torch.float32, torch.bfloat16), dev)
-        if out.shape != (M, N) or ldy < N:
-            raise RuntimeError(f"{what}: out must be [{M},{N}] with rows that do not overlap")
-        if out.untyped_storage().data_ptr() == first.untyped_storage().data_ptr() and M > 0:
-            raise RuntimeError(f"{what}: out must not lie in the memory of x")
-        outs = [out]
-    else:
-        ldy = N
-        outs = [torch.empty(M, N, dtype=out_dtype, device=dev) for _ in xs]
+    ldw, N = _int8_layer(Ws[0], w_scales[0], None, K, dev, what)
+    kind = lambda t: (t.shape, t.dtype, t.stride(), t.device)
+    x0, w0, v0 = kind(first), kind(Ws[0]), kind(w_scales[0])         # the others are like the first
+    if any(kind(x) != x0 for x in feats) or any(kind(W) != w0 for W in Ws):
+        raise RuntimeError(f"{what}: all x, and all W, must have one shape, type and row stride, on {dev}")
+    if any(kind(s) != v0 for s in w_scales) or any(b is not None and kind(b) != v0 for b in bs):
+        raise RuntimeError(f"{what}: every w_scale and b must be a contiguous float32 [{N}] on {dev}")
+    if pairs:
+        for _, s in xs:
+            _vector(s, M, dev, what, "the scale of x")
+    # (n outputs cut from one buffer)
+    y = _int8_out(n * M, N, out_dtype, dev, what)
+    outs = list(y.view(n, M, N).unbind(0)) if M > 0 else [y] * n
     if M == 0 or N == 0:
         return outs
-    n = len(xs)
     arr = ctypes.c_void_p * n
     lib = _lib.load()
-    ws, nbytes = None, 0
-    if pairs or M > 16 or K > 4096:          # (few rows of floats: one launch without a workspace)
-        nbytes = lib.dvq_linear_int8_workspace_bytes(n, M, K, N)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _launch(lib.dvq_linear_int8, "dvq_linear_int8", dev, n, arr(*[x.data_ptr() for x in feats]), DVQ_I8 if pairs else _dtype_code(first),
-            arr(*[s.data_ptr() for s in scales]) if pairs else None, ldx, arr(*[W.data_ptr() for W in Ws]),
+    ws, nbytes = _int8_workspace(lib, n, M, K, N, pairs, dev)
+    step, base = M * N * y.element_size(), y.data_ptr()
+    _launch(lib.dvq_linear_int8_batched, "dvq_linear_int8_batched", dev, n, arr(*[x.data_ptr() for x in feats]), _CODES[first.dtype],
+            arr(*[s.data_ptr() for _, s in xs]) if pairs else None, ldx, arr(*[W.data_ptr() for W in Ws]),
             arr(*[s.data_ptr() for s in w_scales]), ldw, arr(*[None if b is None else b.data_ptr() for b in bs]), M, K, N, int(relu),
-            arr(*[o.data_ptr() for o in outs]), _dtype_code(outs[0]), ldy, _p(ws), nbytes)
+            arr(*[base + i * step for i in range(n)]), _CODES[y.dtype], N, None if ws is None else ws.data_ptr(), nbytes)
     return outs
+
+
+def _int8_layer(W, w_scale, b, K, dev, what):
+    """(row stride, output channels) of a layer's codes."""
+    ldw = _rows(W, _INT8, dev, what, "W")
+    N = W.shape[0]
+    if W.shape[1] != K or not 1 <= K <= INT8_MAX_K:
+        raise RuntimeError(f"{what}: x has {K} features, W {W.shape[1]} (1..{INT8_MAX_K})")
+    _vector(w_scale, N, dev, what, "w_scale")
+    if b is not None:
+        _vector(b, N, dev, what, "b")
+    return ldw, N
+
+
+def _int8_out(M, N, dtype, dev, what):
+    if dtype not in _FLOATS:
+        raise RuntimeError(f"{what}: output of float32 or bfloat16, not {dtype}")
+    return torch.empty((M, N), dtype=dtype, device=dev)
+
+
+def _int8_workspace(lib, n, M, K, N, pairs, dev):
+    if M <= 16 and K <= 4096 and not pairs:              # few rows of floats: one launch that needs none
+        return None, 0
+    nbytes = lib.dvq_linear_int8_workspace_bytes(n, M, K, N)
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev), nbytes
 
 
 # ------------------------------------------------------------------- call-site glue
@@ -682,36 +720,42 @@ def prior_verify(logits: torch.Tensor, draft: torch.Tensor, tokens: torch.Tensor
     if drawn from the prior one by one; the results are those of 64-bit arithmetic.  A code outside [0,V) is rejected,
     lengths are clamped to [0,G]; a distribution that is needed and has no mass (all -inf, or a NaN, +inf or negative
     probability in it) makes next -1."""
-    for t, what, dim, dtypes in ((logits, "logits", 3, (torch.float32, torch.bfloat16)), (draft, "draft", 3, (torch.float32, torch.bfloat16)),
-                                 (tokens, "tokens", 2, (torch.int64,)), (u_accept, "u_accept", 2, (torch.float64,)),
-                                 (u_draw, "u_draw", 1, (torch.float64,))) + (() if lengths is None else ((lengths, "lengths", 1, (torch.int64,)),)):
-        if t.dim() != dim or t.dtype not in dtypes:
-            raise RuntimeError(f"prior_verify: {what} must be {dim}-D of {' or '.join(str(d) for d in dtypes)}, got {tuple(t.shape)} {t.dtype}")
-        if not t.is_cuda:
-            raise RuntimeError("dvq_hip kernels need tensors on a HIP device (got a CPU tensor); there is no CPU fallback")
-        if t.device != logits.device:
-            raise RuntimeError(f"prior_verify: {what} is on {t.device}, logits on {logits.device}")
-    B, P, V = logits.shape
-    G = draft.shape[1]
-    if draft.shape != (B, G, V) or tokens.shape != (B, G) or u_accept.shape != (B, G) or u_draw.shape != (B,) or (
-            lengths is not None and lengths.shape != (B,)):
-        raise RuntimeError(f"prior_verify: logits [B,P,V] = {tuple(logits.shape)} with draft [B,G,V], tokens and u_accept [B,G], u_draw and "
-                           f"lengths [B]; got {tuple(draft.shape)}, {tuple(tokens.shape)}, {tuple(u_accept.shape)}, {tuple(u_draw.shape)}")
-    if P not in (G, G + 1) or P < 1 or V < 1:
+    shape, dev = logits.shape, logits.device
+    ok = (len(shape) == 3 and draft.dim() == 3 and logits.dtype in _FLOATS and draft.dtype in _FLOATS and tokens.dtype == torch.int64
+          and u_accept.dtype == torch.float64 and u_draw.dtype == torch.float64 and (lengths is None or lengths.dtype == torch.int64))
+    if ok:
+        B, P, V = shape
+        G = draft.shape[1]
+        ok = (draft.shape == (B, G, V) and tokens.shape == (B, G) and u_accept.shape == (B, G) and u_draw.shape == (B,)
+              and (lengths is None or lengths.shape == (B,)))
+    if not ok:
+        raise RuntimeError("prior_verify: logits [B,P,V] and draft [B,G,V] of float32 or bfloat16, tokens int64 [B,G], u_accept float64 [B,G], "
+                           "u_draw float64 [B], lengths int64 [B] or None expected; got " + ", ".join(
+                               "None" if t is None else f"{t.dtype} {tuple(t.shape)}" for t in (logits, draft, tokens, u_accept, u_draw, lengths)))
+    if not logits.is_cuda:
+        raise RuntimeError("dvq_hip kernels need tensors on a HIP device (got a CPU tensor); there is no CPU fallback")
+    if draft.device != dev or tokens.device != dev or u_accept.device != dev or u_draw.device != dev or (
+            lengths is not None and lengths.device != dev):
+        raise RuntimeError(f"prior_verify: all tensors must be on {dev}, where the logits are")
+    if (P != G and P != G + 1) or P < 1 or V < 1:
         raise RuntimeError(f"prior_verify: {P} positions of logits for {G} drafted codes (as many, or one more) of {V}")
-    out = torch.empty(2, B, dtype=torch.int64, device=logits.device)
-    accepted, nxt = out[0], out[1]
+    accepted, nxt = torch.empty((2, B), dtype=torch.int64, device=dev).unbind(0)
     if B == 0:
         return accepted, nxt
-    a = DvqPriorVerify(logits.data_ptr(), *logits.stride(), draft.data_ptr(), *draft.stride(), tokens.data_ptr(), *tokens.stride(),
-                       u_accept.data_ptr(), *u_accept.stride(), u_draw.data_ptr(), u_draw.stride(0),
-                       None if lengths is None else lengths.data_ptr(), 0 if lengths is None else lengths.stride(0),
-                       accepted.data_ptr(), nxt.data_ptr(), B, G, P, V, _dtype_code(logits), _dtype_code(draft), int(draft_probs))
-    lib, ref = _lib.load(), ctypes.byref(a)
-    nbytes = lib.dvq_prior_verify_workspace_bytes(ref)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
-    _launch(lib.dvq_prior_verify, "dvq_prior_verify", logits.device, ref, _p(ws), nbytes)
+    a = _VERIFY_ARGS.pack(logits.data_ptr(), *logits.stride(), draft.data_ptr(), *draft.stride(), tokens.data_ptr(), *tokens.stride(),
+                          u_accept.data_ptr(), *u_accept.stride(), u_draw.data_ptr(), u_draw.stride(0),
+                          0 if lengths is None else lengths.data_ptr(), 0 if lengths is None else lengths.stride(0),
+                          accepted.data_ptr(), nxt.data_ptr(), B, G, P, V, _CODES[logits.dtype], _CODES[draft.dtype], int(draft_probs))
+    lib = _lib.load()
+    nbytes = lib.dvq_prior_verify_workspace_bytes(a) if V > 1024 else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _launch(lib.dvq_prior_verify, "dvq_prior_verify", dev, a, None if ws is None else ws.data_ptr(), nbytes)
     return accepted, nxt
+
+
+# DvqPriorVerify as bytes (packing is a tenth of the cost of filling the ctypes structure)
+_VERIFY_ARGS = struct.Struct("@P3qP3qP2qP2qPqPqPPq6i")
+assert _VERIFY_ARGS.size == ctypes.sizeof(DvqPriorVerify)
 
 
 def prior_uniforms(first_id: int, n: int, n_cells: int, seed: int, device) -> torch.Tensor:

@@ -373,14 +373,19 @@ int dvq_prior_uniforms(int64_t first_id, int64_t n, int n_cells, uint64_t seed, 
  *   bits and rounded once to `y_dtype`.  x: [M,K] of x_dtype DVQ_F32 or DVQ_BF16 (c, s: as above, made in the call; xs is
  *   ignored) or DVQ_I8 (c = x, s = xs); row strides in elements, any alignment of the element.  W: int8 [N,K], b nullable.
  *   K < 2^17.  act: relu keeps a NaN.  y must not overlap x.
- *   x, xs, W, ws, b, y: host arrays of n_batch (1..8) device pointers, products of ONE shape in the same launches.
- *   workspace: dvq_linear_int8_workspace_bytes() bytes, 16-byte aligned; not touched (may be NULL) for M <= 16 rows of floats
+ * dvq_linear_int8_batched: products of ONE shape in the same launches; x, xs, W, ws, b, y: host arrays of n_batch (1..8) device
+ *   pointers.
+ *   workspace: dvq_linear_int8_workspace_bytes() bytes (n_batch = 1 for a single product), 16-byte aligned; not touched (may be NULL) for M <= 16 rows of floats
  *   with K <= 4096, and for DVQ_I8 with rows of x and W at multiples of 16 bytes and K % 16 == 0. */
 int dvq_int8_quantize_rows(const void* x, int dtype, int64_t ldx, int M, int K, void* codes, int64_t ldc, float* scale, void* stream);
 size_t dvq_linear_int8_workspace_bytes(int n_batch, int M, int K, int N);
-int dvq_linear_int8(int n_batch, const void* const* x, int x_dtype, const float* const* xs, int64_t ldx, const void* const* W,
-                    const float* const* ws, int64_t ldw, const float* const* b, int M, int K, int N, int relu,
-                    void* const* y, int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
+int dvq_linear_int8(const void* x, int x_dtype, const float* xs, int64_t ldx, const void* W, const float* ws, int64_t ldw,
+                    const float* b, int M, int K, int N, int relu, void* y, int y_dtype, int64_t ldy, void* workspace,
+                    size_t workspace_bytes, void* stream);
+int dvq_linear_int8_batched(int n_batch, const void* const* x, int x_dtype, const float* const* xs, int64_t ldx,
+                            const void* const* W, const float* const* ws, int64_t ldw, const float* const* b, int M, int K,
+                            int N, int relu, void* const* y, int y_dtype, int64_t ldy, void* workspace,
+                            size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------- verification of drafted codes
  * What a drafting model proposed for the prior (models.py:161-198): row b brings n = lengths[b] (NULL: G) codes

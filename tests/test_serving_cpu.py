@@ -60,7 +60,7 @@ def _quantize(lib, M=4, K=16, ldc=16, dtype=0, ldx=16, ptr=16, codes=16):
 
 def _product(lib, n=1, M=4, K=16, N=4, ldx=16, ldw=16, ldy=4, x_dtype=0, y_dtype=0, ptr=16, xs=True, ws=16, nbytes=1 << 40):
     arr = (VP * 8)(*[ptr] * 8)
-    return lib.dvq_linear_int8(n, arr, x_dtype, arr if xs else None, ldx, arr, arr, ldw, None, M, K, N, 0, arr, y_dtype, ldy, ws, nbytes, None)
+    return lib.dvq_linear_int8_batched(n, arr, x_dtype, arr if xs else None, ldx, arr, arr, ldw, None, M, K, N, 0, arr, y_dtype, ldy, ws, nbytes, None)
 
 
 @pytest.mark.parametrize("bad", [dict(K=0), dict(K=1 << 17, ldc=1 << 17), dict(ldc=24), dict(K=17), dict(M=-1), dict(dtype=2), dict(ptr=None),
@@ -77,6 +77,15 @@ def test_quantize_refusals(bad):
 def test_product_refusals(bad):
     lib = _lib.load()
     assert _product(lib, **bad) == -1 and lib.dvq_last_error()
+
+
+def test_single_product_refusals():
+    lib = _lib.load()
+    call = lambda x=16, W=16, y=16, x_dtype=0, xs=16, N=4, ws=16, M=4: lib.dvq_linear_int8(x, x_dtype, xs, 16, W, 16, 16, None, M, 16, N, 0, y, 0, 4,
+                                                                                        ws, 1 << 40, None)
+    assert call(M=0) == 0
+    for bad in (dict(x=None), dict(W=None), dict(y=None), dict(x_dtype=2, xs=None), dict(N=0), dict(M=20, ws=None)):
+        assert call(**bad) == -1 and lib.dvq_last_error()
 
 
 def test_workspace_of_the_product():
