@@ -5,6 +5,7 @@ distribution (`dvq_hip.ops.prior_verify`).
 `run` computes them in elementary torch operations, or through the framework's entry points where `own` is true; `exact`
 says in 64 bits what the outputs are.
 """
+import importlib
 import math
 import os
 import sys
@@ -18,11 +19,11 @@ TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16}
 
 
 def _ops():
-    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "d-vqvae_amd")
-    if root not in sys.path:
-        sys.path.insert(0, root)
-    from dvq_hip import ops
-    return ops
+    """The framework's entry points, imported once as a user's program does."""
+    if "dvq_hip.ops" not in sys.modules:
+        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "d-vqvae_amd"))
+        importlib.import_module("dvq_hip.ops")
+    return sys.modules["dvq_hip.ops"]
 
 
 def listed():
