@@ -13,8 +13,10 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kInt8MaxBatch = 8;
-// Fewer 64 x 64 tiles than this leave CUs without work: the kernel that splits k runs instead.
-constexpr int kInt8SplitBelow = 128;
+// Up to so many 64 x 64 tiles the kernel that splits k runs: its workgroups (four to a tile) then fit the CUs in one round.
+// Tiles against split, int8 operands in place: 64 tiles (128 x 2048 x 2048) 9.1 / 8.4 us, 32 (100 x 1000 x 512) 6.0 / 4.9;
+// 80 tiles (128 x 2560 x 1024) 6.8 / 8.7, 96 (200 x 1536 x 4096) 13.8 / 21.5.
+constexpr int kInt8SplitTo = 64;
 struct Int8Prepare {
     const void* x[kInt8MaxBatch];
     const int8_t* W[kInt8MaxBatch];
@@ -166,12 +168,19 @@ __global__ __launch_bounds__(64) void int8_prepare_kernel(Int8Prepare p, int64_t
 
 // Scaled in 64 bits, rounded once: no intermediate leaves the range of 32 bits where the result does not (s is up to 2^121,
 // the sum up to 2^31), at four 64-bit instructions per output.
-__device__ __forceinline__ float int8_scale(int acc, float s, float t, float b, int relu) {
-    const float v = (float)__builtin_fma((double)acc, (double)s * (double)t, (double)b);
+__device__ __forceinline__ float int8_scale(int acc, double s, double t, double b, int relu) {
+    const float v = (float)__builtin_fma((double)acc, s * t, b);
     return relu && v < 0.f ? 0.f : v;
 }
 __device__ __forceinline__ void int8_store(float* y, float v) { *y = v; }
 __device__ __forceinline__ void int8_store(unsigned short* y, float v) { *y = f32_to_bf16_bits(v); }
+__device__ __forceinline__ void int8_store4(float* y, const float (&v)[4]) { *reinterpret_cast<f32x4*>(y) = f32x4{v[0], v[1], v[2], v[3]}; }
+__device__ __forceinline__ void int8_store4(unsigned short* y, const float (&v)[4]) {
+    uint2 o;
+    o.x = f32_to_bf16_bits(v[0]) | (unsigned)f32_to_bf16_bits(v[1]) << 16;
+    o.y = f32_to_bf16_bits(v[2]) | (unsigned)f32_to_bf16_bits(v[3]) << 16;
+    *reinterpret_cast<uint2*>(y) = o;
+}
 
 // 16 elements of a row from element k on (k % 16 == 0), zeros behind the row's end.
 template <typename T>
@@ -306,52 +315,73 @@ __device__ __forceinline__ void int8_glds16(const void* gsrc_lane, void* lds_wav
                                      (__attribute__((address_space(3))) void*)lds_wave_base, 16, 0, 0);
 }
 
+// Waits until at most VM vector memory operations are under way and every LDS read has arrived.  (The builtin: the compiler
+// counts on from it, where it takes inline assembly for nothing and waits for everything again.)
+template <int VM>
+__device__ __forceinline__ void int8_wait() {
+    static_assert(VM >= 0 && VM < 64, "six bits");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((VM & 15) | ((VM >> 4) << 14) | (7 << 4));
+    asm volatile("" ::: "memory");
+}
+
 __device__ __attribute__((aligned(16))) const int int8_zeros[4] = {0, 0, 0, 0};
 
-// Tiles of BM x BN outputs, WVM x WVN waves, k in stages of 128 bytes through two LDS buffers: the copies of a stage go
-// straight from memory into LDS while the products of the one before run, one barrier a stage.  Rows of both operands
-// start at multiples of 16 bytes and K is a multiple of 16 (zeros behind the features).  A row's 128 bytes of a stage
-// lie in LDS with 16-byte piece c at place c ^ (row & 7): copies stay linear in LDS (each lane picks its source), and the
-// eight rows of a fragment's read phase lie in different banks.
-template <int BM, int BN, int WVM, int WVN, typename Y>
+// Tiles of BM x BN outputs, WVM x WVN waves, k in stages of BK bytes through a ring of R buffers in LDS: the copies of R
+// stages go straight from memory into LDS while the products of the stage in front of them run, one barrier a stage.  Rows
+// of both operands start at multiples of 16 bytes and K is a multiple of 16 (zeros behind the features); stages behind K
+// are copied from a line of zeros, so that every stage is the same number of loads.
+// LDS serves 16 lanes of a 16-byte read at a time from 64 banks (256 bytes): with rows of 128 (64) bytes those are 16 rows, of
+// which every second (fourth) falls on the same banks.  16-byte piece c of a row lies at place c ^ (row / 2 % 8) (c ^ (row / 4
+// % 4)), which spreads them over all banks; the copies stay linear in LDS, each lane picks its source.
+template <int BM, int BN, int WVM, int WVN, int BK, int R, typename Y>
 __global__ __launch_bounds__(WVM * WVN * 64) void int8_tile_kernel(Int8Batch p, int64_t ldx, int64_t ldw, int M, int K, int N, int relu, int64_t ldy) {
     constexpr int WV = WVM * WVN, TM = BM / WVM / 32, TN = BN / WVN / 32;
-    constexpr int UA = BM / 8, UB = BN / 8, PER = (UA + UB) / WV;      // units of 8 rows x 128 bytes
-    constexpr int STAGE = (BM + BN) * 128;
-    static_assert(TM >= 1 && TN >= 1 && (UA + UB) % WV == 0, "tile");
+    constexpr int PR = BK / 16, RU = 64 / PR, LOG = BK == 128 ? 1 : 2;      // pieces of a row, rows of a 1-KiB unit
+    constexpr int UA = BM / RU, UB = BN / RU, PER = (UA + UB) / WV;
+    constexpr int STAGE = (BM + BN) * BK;
+    static_assert((BK == 64 || BK == 128) && TM >= 1 && TN >= 1 && UA % WV == 0 && UB % WV == 0, "tile");
     extern __shared__ __align__(16) int8_t smem[];
+    __shared__ __align__(16) double tb[2 * BN];              // scales and biases of the tile's channels
     const int bz = blockIdx.y;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int nx = (N + BN - 1) / BN, ny = (M + BM - 1) / BM;
     int tx, ty;
     xcd_tile((int)blockIdx.x, nx, ny, tx, ty);
     const int m0 = ty * BM, n0 = tx * BN;
+    for (int n = tid; n < BN; n += WV * 64) {
+        const int at = n0 + n < N ? n0 + n : N - 1;
+        tb[n] = p.ws[bz][at];
+        tb[BN + n] = p.b[bz] ? p.b[bz][at] : 0.;
+    }
 
     const int8_t* src[PER];
-    const int piece = (lane & 7) ^ (lane >> 3);
+    static_assert(WV * RU % (PR << LOG) == 0, "a wave's units are alike");
+    const int urow = lane / PR, piece = (lane % PR) ^ (((wave * RU + urow) >> LOG) & (PR - 1));
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int u = wave + WV * i;
-        const int row = (u < UA ? m0 + u * 8 : n0 + (u - UA) * 8) + (lane >> 3);
-        src[i] = u < UA ? reinterpret_cast<const int8_t*>(p.x[bz]) + (int64_t)(row < M ? row : M - 1) * ldx + piece * 16
-                        : p.W[bz] + (int64_t)(row < N ? row : N - 1) * ldw + piece * 16;
+        const int u = (i < UA / WV ? i : i - UA / WV) * WV + wave;
+        const int row = (i < UA / WV ? m0 : n0) + u * RU + urow;
+        src[i] = i < UA / WV ? reinterpret_cast<const int8_t*>(p.x[bz]) + (int64_t)(row < M ? row : M - 1) * ldx + piece * 16
+                             : p.W[bz] + (int64_t)(row < N ? row : N - 1) * ldw + piece * 16;
     }
-    auto issue = [&](int st) {
-        int8_t* dst = smem + (st & 1) * STAGE + wave * 1024;
-        const int k0 = st * 128;
-        if (k0 + 128 <= K) {
+    uintptr_t zeros = reinterpret_cast<uintptr_t>(int8_zeros);
+    asm("" : "+s"(zeros));                                   // (known to be another object it becomes a load of its own, with half of the lanes)
+    int put = 0, k_put = 0;
+    auto issue = [&]() {
+        int8_t* dst = smem + put * STAGE + wave * 1024;
+        const bool in = k_put + piece * 16 < K;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) int8_glds16(src[i] + k0, dst + i * WV * 1024);
-        } else {
-            const bool in = k0 + piece * 16 < K;
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                int8_glds16(in ? static_cast<const void*>(src[i] + k0) : static_cast<const void*>(int8_zeros), dst + i * WV * 1024);
+        for (int i = 0; i < PER; ++i) {
+            const uintptr_t at = in ? reinterpret_cast<uintptr_t>(src[i] + k_put) : zeros;
+            int8_glds16(reinterpret_cast<const void*>(at), dst + (i < UA / WV ? i : i - UA / WV) * WV * 1024 + (i < UA / WV ? 0 : BM * BK));
         }
+        put = put + 1 == R ? 0 : put + 1;
+        k_put += BK;
     };
 
     const int wm = (wave / WVN) * (BM / WVM), wn = (wave % WVN) * (BN / WVN);
-    const int r = lane & 31, h = lane >> 5;
+    const int r = lane & 31, h = lane >> 5, f = (r >> LOG) & (PR - 1);
     i32x16 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -359,49 +389,98 @@ __global__ __launch_bounds__(WVM * WVN * 64) void int8_tile_kernel(Int8Batch p, 
         for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-    const int stages = (K + 127) / 128;
-    issue(0);
+    // The fragments of a step of 32 k are read during the products of the step in front of it, also across stages: the wait
+    // for the next stage and its barrier lie in front of a stage's last products.  At that barrier everyone holds the last
+    // fragments of this stage in registers, so that its buffer can be filled again.
+    constexpr int KK = BK / 32;
+    static_assert(KK % 2 == 0, "two sets of fragments in turns");
+    i32x4 fa[2][TM], fb[2][TN];
+    int get = 0;
+    auto read = [&](int kk, int set) {
+        const int8_t* sa = smem + get * STAGE + (wm + r) * BK;
+        const int8_t* sb = smem + get * STAGE + BM * BK + (wn + r) * BK;
+        const int at = ((2 * kk + h) ^ f) << 4;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) fa[set][i] = *reinterpret_cast<const i32x4*>(sa + i * 32 * BK + at);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) fb[set][j] = *reinterpret_cast<const i32x4*>(sb + j * 32 * BK + at);
+    };
+    const int stages = (K + BK - 1) / BK;
+#pragma unroll
+    for (int i = 0; i < R; ++i) issue();
+    int8_wait<(R - 1) * PER>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(0, 0);
     for (int st = 0; st < stages; ++st) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // own copies of this stage have landed
-        __syncthreads();                                     // everyone's have, and everyone is done with the other buffer
-        if (st + 1 < stages) issue(st + 1);
-        const int8_t* sa = smem + (st & 1) * STAGE + (wm + r) * 128;
-        const int8_t* sb = smem + (st & 1) * STAGE + (BM + wn + r) * 128;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            const int at = ((2 * kk + h) ^ (r & 7)) << 4;
-            i32x4 fa[TM], fb[TN];
-#pragma unroll
-            for (int i = 0; i < TM; ++i) fa[i] = *reinterpret_cast<const i32x4*>(sa + i * 32 * 128 + at);
-#pragma unroll
-            for (int j = 0; j < TN; ++j) fb[j] = *reinterpret_cast<const i32x4*>(sb + j * 32 * 128 + at);
+        for (int kk = 0; kk < KK; ++kk) {
+            if (kk + 1 < KK) read(kk + 1, (kk + 1) & 1);
+            else {
+                // own copies of the next stage have landed (R - 2 younger stages are under way), own reads of this one are done
+                int8_wait<(R - 2) * PER>();
+                __builtin_amdgcn_s_barrier();                // so have everyone's
+                asm volatile("" ::: "memory");
+                get = get + 1 == R ? 0 : get + 1;
+                read(0, 0);
+                issue();
+            }
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fb[j], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[kk & 1][j], fa[kk & 1][i], acc[i][j], 0, 0, 0);
         }
     }
+    int8_wait<0>();                                          // (the copies behind the last stage)
+    __syncthreads();                                         // nobody reads the ring any more
+    // A lane holds 4 x 4 channels of one row: 32 rows at a time they go through LDS, so that the stores are whole lines of
+    // consecutive channels (stored as they lie, 64 bytes of two rows per instruction, the outputs cost 50 of 190 us at 8192 x
+    // 4096 x 4096 in 16 bits and 10 of 30 us at 4096 x 2560 x 1024).
+    constexpr int COLS = TN * 32, RS = COLS * (int)sizeof(Y) + 16, PV = 16 / (int)sizeof(Y), LPR = COLS / PV;
+    static_assert(WV * 32 * RS <= R * STAGE, "the outputs fit the ring");
+    int8_t* slab = smem + wave * 32 * RS;
     Y* y = reinterpret_cast<Y*>(p.y[bz]);
-    const float* xs = p.xs[bz];
+    const int nw = n0 + wn;
+    const bool vec = nw + COLS <= N && ((reinterpret_cast<uintptr_t>(y) | (uintptr_t)(ldy * (int64_t)sizeof(Y))) % 16) == 0;
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const int n = n0 + wn + 32 * j + r;
-        if (n >= N) continue;
-        const float t = p.ws[bz][n], bias = p.b[bz] ? p.b[bz][n] : 0.f;
+    for (int i = 0; i < TM; ++i) {
+        const int mw = m0 + wm + 32 * i, m = mw + r;
+        const double s = (double)p.xs[bz][m < M ? m : M - 1];
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int m = m0 + wm + 32 * i + (e & 3) + 8 * (e >> 2) + 4 * h;
-                if (m < M) int8_store(y + (int64_t)m * ldy + n, int8_scale(acc[i][j][e], xs[m], t, bias, relu));
+            for (int q = 0; q < 4; ++q) {
+                const int n = 32 * j + 8 * q + 4 * h;
+                const double* t = tb + wn + n;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = int8_scale(acc[i][j][4 * q + e], s, t[e], t[BN + e], relu);
+                int8_store4(reinterpret_cast<Y*>(slab + r * RS) + n, v);
             }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (vec) {
+#pragma unroll
+            for (int c = 0; c < 32 * LPR / 64; ++c) {
+                const int row = (c * 64 + lane) / LPR, col = (c * 64 + lane) % LPR * PV;
+                const u32x4 v = *reinterpret_cast<const u32x4*>(slab + row * RS + col * (int)sizeof(Y));
+                if (mw + row < M) *reinterpret_cast<u32x4*>(y + (int64_t)(mw + row) * ldy + nw + col) = v;
+            }
+        } else {
+            for (int c = lane; c < 32 * COLS; c += 64) {
+                const int row = c / COLS, col = c % COLS;
+                if (mw + row < M && nw + col < N) y[(int64_t)(mw + row) * ldy + nw + col] = *(reinterpret_cast<const Y*>(slab + row * RS) + col);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
-template <int BM, int BN, int WVM, int WVN, typename Y>
+template <int BM, int BN, int WVM, int WVN, int BK, int R, typename Y>
 static int int8_tiles(const Int8Batch& p, int n_batch, int64_t ldx, int64_t ldw, int M, int K, int N, int relu, int64_t ldy, hipStream_t st) {
-    auto kern = int8_tile_kernel<BM, BN, WVM, WVN, Y>;
-    const size_t lds = 2 * (BM + BN) * 128;
+    auto kern = int8_tile_kernel<BM, BN, WVM, WVN, BK, R, Y>;
+    const size_t lds = (size_t)R * (BM + BN) * BK;
     if (int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), lds, "linear_int8")) return rc;
     const int64_t tiles = (int64_t)((M + BM - 1) / BM) * ((N + BN - 1) / BN);
     if (tiles > 0x7FFFFFFF) return fail(DVQ_EINVAL, "linear_int8: M x N too large");
@@ -415,7 +494,7 @@ static inline int64_t tile_count(int M, int N, int b, int n_batch) { return (int
 template <typename Y>
 static int int8_product(const Int8Batch& p, int n_batch, int64_t ldx, int64_t ldw, int M, int K, int N, int relu, int64_t ldy, bool aligned,
                         hipStream_t st) {
-    if (!aligned || tile_count(M, N, 64, n_batch) < kInt8SplitBelow) {
+    if (!aligned || tile_count(M, N, 64, n_batch) <= kInt8SplitTo) {
         const dim3 blk(512);
         const unsigned gx = (unsigned)((N + 15) / 16);
         if (M <= 16) hipLaunchKernelGGL((int8_split_kernel<1, Y>), dim3(gx, 1, n_batch), blk, 0, st, p, ldx, ldw, M, K, N, relu, ldy);
@@ -423,9 +502,13 @@ static int int8_product(const Int8Batch& p, int n_batch, int64_t ldx, int64_t ld
         else hipLaunchKernelGGL((int8_split_kernel<4, Y>), dim3(gx, (M + 63) / 64, n_batch), blk, 0, st, p, ldx, ldw, M, K, N, relu, ldy);
         return check_launch("linear_int8");
     }
-    if (tile_count(M, N, 256, n_batch) >= 224) return int8_tiles<256, 256, 2, 4, Y>(p, n_batch, ldx, ldw, M, K, N, relu, ldy, st);
-    if (tile_count(M, N, 128, n_batch) >= 192) return int8_tiles<128, 128, 2, 2, Y>(p, n_batch, ldx, ldw, M, K, N, relu, ldy, st);
-    return int8_tiles<64, 64, 2, 2, Y>(p, n_batch, ldx, ldw, M, K, N, relu, ldy, st);
+    // A larger tile reads its operands less often, a smaller one leaves fewer CUs idle.  Tiles of 256 / 128 / 64, us: 4096 x
+    // 2560 x 1024 (160 / 640 / 2560 tiles) 25 / 31 / 38, 2048 x 4096 x 4096 (128 / 512 / 2048) 58 / 60 / 85, 2048 x 2560 x 1024
+    // (80 / 320 / 1280) 24 / 20 / 20, 1024 x 2560 x 1024 (40 / 160 / 640) 23 / 12 / 14, 1024 x 2048 x 2048 (32 / 128 / 512) 31 /
+    // 15 / 13: the smallest as long as its tiles fit the chip in one round, two to a CU.
+    if (tile_count(M, N, 256, n_batch) >= 128) return int8_tiles<256, 256, 2, 4, 64, 4, Y>(p, n_batch, ldx, ldw, M, K, N, relu, ldy, st);
+    if (tile_count(M, N, 64, n_batch) > 512) return int8_tiles<128, 128, 2, 4, 128, 4, Y>(p, n_batch, ldx, ldw, M, K, N, relu, ldy, st);
+    return int8_tiles<64, 64, 2, 2, 128, 4, Y>(p, n_batch, ldx, ldw, M, K, N, relu, ldy, st);
 }
 
 static bool aligned16(const void* const* ptrs, int n, int64_t ld) {
@@ -496,7 +579,7 @@ extern "C" int dvq_linear_int8_batched(int n_batch, const void* const* x, int x_
     }
     // What the tiles cannot read in place -- features to quantise, rows that do not start at multiples of 16 bytes -- is
     // laid out in the workspace by one launch.
-    const bool tiles = tile_count(M, N, 64, n_batch) >= kInt8SplitBelow;
+    const bool tiles = tile_count(M, N, 64, n_batch) > kInt8SplitTo;
     const bool wide = K % 16 == 0;
     const bool copy_w = tiles && !(wide && aligned16(W, n_batch, ldw));
     const bool copy_x = !codes || (tiles && !(wide && aligned16(x, n_batch, ldx)));

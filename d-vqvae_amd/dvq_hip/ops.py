@@ -441,12 +441,14 @@ def linear_int8_batched(xs, Ws, w_scales, bs, relu: bool = False, out_dtype: tor
     M, K = first.shape
     dev = first.device
     ldw, N = _int8_layer(Ws[0], w_scales[0], None, K, dev, what)
-    kind = lambda t: (t.shape, t.dtype, t.stride(), t.device)
-    x0, w0, v0 = kind(first), kind(Ws[0]), kind(w_scales[0])         # the others are like the first
-    if any(kind(x) != x0 for x in feats) or any(kind(W) != w0 for W in Ws):
-        raise RuntimeError(f"{what}: all x, and all W, must have one shape, type and row stride, on {dev}")
-    if any(kind(s) != v0 for s in w_scales) or any(b is not None and kind(b) != v0 for b in bs):
-        raise RuntimeError(f"{what}: every w_scale and b must be a contiguous float32 [{N}] on {dev}")
+    # the others are like the first
+    for group, t0, message in ((feats, first, "all x must have one shape, type and row stride"), (Ws, Ws[0], "all W must have one shape and row stride"),
+                               (w_scales, w_scales[0], f"every w_scale must be a contiguous float32 [{N}]"),
+                               ([b for b in bs if b is not None], w_scales[0], f"every b must be a contiguous float32 [{N}]")):
+        shape, dtype, stride = t0.shape, t0.dtype, t0.stride()
+        for t in group:
+            if t.dtype != dtype or t.shape != shape or t.stride() != stride or t.device != dev:
+                raise RuntimeError(f"{what}: {message}, on {dev}")
     if pairs:
         for _, s in xs:
             _vector(s, M, dev, what, "the scale of x")
