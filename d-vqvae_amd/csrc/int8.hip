@@ -47,7 +47,14 @@ __device__ __forceinline__ unsigned int8_code(float x, double inv) {
 __device__ __forceinline__ i32x4 int8_chunk(const int8_t* row, int k, int K) {
     i32x4 v = {0, 0, 0, 0};
     if (k + 16 <= K) __builtin_memcpy(&v, row + k, 16);
-    else {
+    else if (K >= 16) {                                      // the row's last 16 bytes, moved down
+        unsigned __int128 u = 0;
+        if (k < K) {
+            __builtin_memcpy(&u, row + K - 16, 16);
+            u >>= 8 * (16 - (K - k));
+        }
+        __builtin_memcpy(&v, &u, 16);
+    } else {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
             if (k + j < K) v[j >> 2] |= (int)(unsigned char)row[k + j] << (8 * (j & 3));
