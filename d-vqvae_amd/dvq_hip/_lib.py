@@ -97,9 +97,9 @@ SIGNATURES = {
     "dvq_linear_int8_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "dvq_linear_int8": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int,
                                 c_void_p, c_int, c_int64, c_void_p, c_size_t, c_void_p]),
-    "dvq_linear_int8_batched": (c_int, [c_int, POINTER(c_void_p), c_int, POINTER(c_void_p), c_int64, POINTER(c_void_p), POINTER(c_void_p),
-                                        c_int64, POINTER(c_void_p), c_int, c_int, c_int, c_int, POINTER(c_void_p), c_int, c_int64,
-                                        c_void_p, c_size_t, c_void_p]),
+    # (lists of addresses, by their own address)
+    "dvq_linear_int8_batched": (c_int, [c_int, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_int,
+                                        c_int, c_void_p, c_int, c_int64, c_void_p, c_size_t, c_void_p]),
     # (the DvqPriorVerify structure, or its bytes)
     "dvq_prior_verify_workspace_bytes": (c_size_t, [c_void_p]),
     "dvq_prior_verify": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),

@@ -368,7 +368,7 @@ def _rows(t: torch.Tensor, dtypes, dev, what: str, name: str) -> int:
 
 
 def _vector(t: torch.Tensor, n: int, dev, what: str, name: str) -> None:
-    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous() or t.device != dev:
+    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous() or t.get_device() != dev.index:
         raise RuntimeError(f"{what}: {name} must be a contiguous float32 [{n}] on {dev}")
 
 
@@ -442,13 +442,17 @@ def linear_int8_batched(xs, Ws, w_scales, bs, relu: bool = False, out_dtype: tor
     dev = first.device
     ldw, N = _int8_layer(Ws[0], w_scales[0], None, K, dev, what)
     # the others are like the first
-    for group, t0, message in ((feats, first, "all x must have one shape, type and row stride"), (Ws, Ws[0], "all W must have one shape and row stride"),
-                               (w_scales, w_scales[0], f"every w_scale must be a contiguous float32 [{N}]"),
-                               ([b for b in bs if b is not None], w_scales[0], f"every b must be a contiguous float32 [{N}]")):
+    index = dev.index
+    for group, t0, ld, message in ((feats, first, ldx, "all x must have one shape, type and row stride"),
+                                   (Ws, Ws[0], ldw, "all W must have one shape and row stride")):
         shape, dtype, stride = t0.shape, t0.dtype, t0.stride()
         for t in group:
-            if t.dtype != dtype or t.shape != shape or t.stride() != stride or t.device != dev:
+            if t.dtype != dtype or t.shape != shape or t.get_device() != index or (t.stride() != stride and _rows(t, (dtype,), dev, what, "x or W") != ld):
                 raise RuntimeError(f"{what}: {message}, on {dev}")
+    for name, group in (("every w_scale", w_scales), ("every b", bs)):
+        for t in group:
+            if t is not None or group is w_scales:
+                _vector(t, N, dev, what, name)
     if pairs:
         for _, s in xs:
             _vector(s, M, dev, what, "the scale of x")
@@ -457,14 +461,17 @@ def linear_int8_batched(xs, Ws, w_scales, bs, relu: bool = False, out_dtype: tor
     outs = list(y.view(n, M, N).unbind(0)) if M > 0 else [y] * n
     if M == 0 or N == 0:
         return outs
-    arr = ctypes.c_void_p * n
     lib = _lib.load()
     ws, nbytes = _int8_workspace(lib, n, M, K, N, pairs, dev)
     step, base = M * N * y.element_size(), y.data_ptr()
-    _launch(lib.dvq_linear_int8_batched, "dvq_linear_int8_batched", dev, n, arr(*[x.data_ptr() for x in feats]), _CODES[first.dtype],
-            arr(*[s.data_ptr() for _, s in xs]) if pairs else None, ldx, arr(*[W.data_ptr() for W in Ws]),
-            arr(*[s.data_ptr() for s in w_scales]), ldw, arr(*[None if b is None else b.data_ptr() for b in bs]), M, K, N, int(relu),
-            arr(*[base + i * step for i in range(n)]), _CODES[y.dtype], N, None if ws is None else ws.data_ptr(), nbytes)
+    # the six lists of n addresses behind one another
+    lists = (ctypes.c_void_p * (6 * n))(*[x.data_ptr() for x in feats], *[W.data_ptr() for W in Ws], *[s.data_ptr() for s in w_scales],
+                                        *[None if b is None else b.data_ptr() for b in bs], *range(base, base + n * step, step),
+                                        *([s.data_ptr() for _, s in xs] if pairs else [None] * n))
+    at = ctypes.addressof(lists)
+    _launch(lib.dvq_linear_int8_batched, "dvq_linear_int8_batched", dev, n, at, _CODES[first.dtype], at + 40 * n if pairs else None, ldx,
+            at + 8 * n, at + 16 * n, ldw, at + 24 * n, M, K, N, int(relu), at + 32 * n, _CODES[y.dtype], N,
+            None if ws is None else ws.data_ptr(), nbytes)
     return outs
 
 
