@@ -36,6 +36,9 @@ __device__ __forceinline__ bool xcd_tile(int lin, int nx, int ny, int& tx, int& 
 void set_error(const char* fmt, ...);
 int fail(int code, const char* fmt, ...);
 
+// One dimension of a launch holds fewer than 2^32 threads.
+inline bool launch_fits(int64_t blocks, int threads) { return blocks <= 0x7FFFFFFF && blocks * threads <= 0xFFFFFFFFll; }
+
 // Checks the launch that was just enqueued.
 int check_launch(const char* what);
 

@@ -490,18 +490,18 @@ static int int8_tiles(const Int8Batch& p, int n_batch, int64_t ldx, int64_t ldw,
     const size_t lds = (size_t)R * (BM + BN) * BK;
     if (int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), lds, "linear_int8")) return rc;
     const int64_t tiles = (int64_t)((M + BM - 1) / BM) * ((N + BN - 1) / BN);
-    if (tiles > 0x7FFFFFFF) return fail(DVQ_EINVAL, "linear_int8: M x N too large");
+    if (!launch_fits(tiles, WVM * WVN * 64)) return fail(DVQ_EINVAL, "linear_int8: M x N too large");
     hipLaunchKernelGGL(kern, dim3((unsigned)tiles, (unsigned)n_batch), dim3(WVM * WVN * 64), lds, st, p, ldx, ldw, M, K, N, relu, ldy);
     return check_launch("linear_int8");
 }
 
 static inline int64_t tile_count(int M, int N, int b, int n_batch) { return (int64_t)((M + b - 1) / b) * ((N + b - 1) / b) * n_batch; }
 
-// The product of rows that are codes already (p.x); `aligned`: rows of both operands at multiples of 16 bytes, K % 16 == 0.
+// The product of rows that are codes already (p.x).  `tiles`: rows of both operands start at multiples of 16 bytes, K % 16 == 0.
 template <typename Y>
-static int int8_product(const Int8Batch& p, int n_batch, int64_t ldx, int64_t ldw, int M, int K, int N, int relu, int64_t ldy, bool aligned,
+static int int8_product(const Int8Batch& p, int n_batch, int64_t ldx, int64_t ldw, int M, int K, int N, int relu, int64_t ldy, bool tiles,
                         hipStream_t st) {
-    if (!aligned || tile_count(M, N, 64, n_batch) <= kInt8SplitTo) {
+    if (!tiles) {
         const dim3 blk(512);
         const unsigned gx = (unsigned)((N + 15) / 16);
         if (M <= 16) hipLaunchKernelGGL((int8_split_kernel<1, Y>), dim3(gx, 1, n_batch), blk, 0, st, p, ldx, ldw, M, K, N, relu, ldy);
@@ -544,6 +544,7 @@ extern "C" int dvq_int8_quantize_rows(const void* x, int dtype, int64_t ldx, int
     if (dtype != DVQ_F32 && dtype != DVQ_BF16) return fail(DVQ_EINVAL, "int8_quantize_rows: dtype must be DVQ_F32 or DVQ_BF16");
     if (M < 0 || K < 1 || K >= (1 << 17) || ldx < 0 || ldc < K || (ldc % 16) != 0 || ldc > (1 << 30))
         return fail(DVQ_EINVAL, "int8_quantize_rows: M >= 0, 1 <= K < 2^17, ldc >= K a multiple of 16 (got M = %d, K = %d, ldc = %lld)", M, K, (long long)ldc);
+    if (!launch_fits(M, 64)) return fail(DVQ_EINVAL, "int8_quantize_rows: M must stay below 2^26");
     if (M == 0) return DVQ_OK;
     if (!x || !codes || !scale || reinterpret_cast<uintptr_t>(codes) % 16) return fail(DVQ_EINVAL, "int8_quantize_rows: null or unaligned pointer");
     Int8Prepare p = {};
@@ -561,7 +562,7 @@ extern "C" int dvq_linear_int8_batched(int n_batch, const void* const* x, int x_
     if (y_dtype != DVQ_F32 && y_dtype != DVQ_BF16) return fail(DVQ_EINVAL, "linear_int8: y_dtype must be DVQ_F32 or DVQ_BF16");
     if (M < 0 || N < 1 || K < 1 || K >= (1 << 17)) return fail(DVQ_EINVAL, "linear_int8: M >= 0, N >= 1, 1 <= K < 2^17 (got M = %d, N = %d, K = %d)", M, N, K);
     if (ldx < 0 || ldw < 0 || ldy < N) return fail(DVQ_EINVAL, "linear_int8: bad row stride");
-    if (M > 0x7FFFFFFF - N) return fail(DVQ_EINVAL, "linear_int8: M + N must stay below 2^31");
+    if (M > (1 << 30) || N > (1 << 30)) return fail(DVQ_EINVAL, "linear_int8: M and N up to 2^30");
     if (M == 0) return DVQ_OK;
     const bool codes = x_dtype == DVQ_I8;
     if (!x || !W || !ws || !y || (codes && !xs)) return fail(DVQ_EINVAL, "linear_int8: null pointer");
@@ -577,6 +578,7 @@ extern "C" int dvq_linear_int8_batched(int n_batch, const void* const* x, int x_
     hipStream_t st = as_stream(stream);
     const bool f32 = y_dtype == DVQ_F32;
     if (!codes && int8_one_launch(M, K)) {
+        if (!launch_fits((N + 15) / 16, 512)) return fail(DVQ_EINVAL, "linear_int8: N too large");
         typedef unsigned short u16;
         if (x_dtype == DVQ_F32)
             return f32 ? int8_rows16<float, float>(p, n_batch, ldx, ldw, M, K, N, relu, ldy, st)
@@ -608,6 +610,7 @@ extern "C" int dvq_linear_int8_batched(int n_batch, const void* const* x, int x_
             if (copy_w) p.W[i] = q.w_codes[i];
         }
         const int rows = copy_x ? M : 0;
+        if (!launch_fits((int64_t)rows + (copy_w ? N : 0), 64)) return fail(DVQ_EINVAL, "linear_int8: too many rows to quantise or lay out (2^26)");
         const dim3 grid((unsigned)(rows + (copy_w ? N : 0)), (unsigned)n_batch);
         if (x_dtype == DVQ_F32) hipLaunchKernelGGL(int8_prepare_kernel<float>, grid, dim3(64), 0, st, q, ldx, ldw, rows, K, ldc);
         else if (x_dtype == DVQ_BF16) hipLaunchKernelGGL(int8_prepare_kernel<unsigned short>, grid, dim3(64), 0, st, q, ldx, ldw, rows, K, ldc);

@@ -287,9 +287,9 @@ __device__ __forceinline__ int verify_test(const Exp& ex, const Drafted<T, D>& f
     if (!sum_ok(p) || (!PROBS && !sum_ok(q))) return VERIFY_BAD;
     if (!f.inside) return VERIFY_REJECT;
     if (PROBS && !(f.d >= 0.f && f.d < __builtin_inff())) return VERIFY_BAD;
-    // u q < p, both sides times the two sums
+    // u q < p, both sides times the two sums; u last, so that equal distributions keep every u below 1
     const double px = PROBS ? ex((double)f.t - (double)p.ref) : ex((double)f.t - (double)p.ref) * q.s;
-    const double lhs = f.u * (PROBS ? (double)f.d : ex((double)f.d - (double)q.ref)) * p.s;
+    const double lhs = f.u * ((PROBS ? (double)f.d : ex((double)f.d - (double)q.ref)) * p.s);
     if (!exact && px > 0.0 && lhs > 0.0 && !(fabs(lhs - px) > kVerifyMargin * px)) return VERIFY_UNSURE;
     return lhs < px ? VERIFY_KEEP : VERIFY_REJECT;
 }
@@ -498,10 +498,14 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(TILES == 1
         for (; i < total; ++i) staged[i] = from[i];              // (at most one thread has a rest)
     }
     const Exp ex = verify_table(table);
+    int held = 0;                                                // first of the 64 drafted codes at hand
     for (int base = 0;; base += waves) {
         const int g = base + wave;                               // n: the position behind all drafts
         float t[TILES][8], q[TILES][8];
-        if (base / 64 != (base - waves) / 64 && base > 0) drafted.fetch(a, b, base / 64 * 64, n, lane);
+        if (g - held >= 64) {
+            held = g / 64 * 64;
+            drafted.fetch(a, b, held, n, lane);
+        }
         const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)g * a.lp;
         const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
         Sum p = {none, 0.f, 0.0}, s = {none, 0.f, 0.0};
@@ -970,8 +974,9 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_pass_kernel(VerifyArg
     for (int base = 0; st == VERIFY_KEEP; base += kSplitWaves) {
         const int mine = base + wave;
         int s = mine == n ? (n < a.P ? VERIFY_REJECT : VERIFY_BAD) : VERIFY_KEEP;
+        // (every wave, also one whose own position is not there: all of them read position g's if its test is unsure)
+        if (base > 0 && base % 64 == 0) drafted.fetch(a, b, base, n, lane);
         if (mine <= n && mine < a.P) {
-            if (base / 64 != (base - kSplitWaves) / 64 && base > 0) drafted.fetch(a, b, base / 64 * 64, n, lane);
             p = split_join(ex, row.p + mine * chunks, chunks, lane);
             if (mine < n) {
                 if (!PROBS) q = split_join(ex, row.q + mine * chunks, chunks, lane);
@@ -1120,9 +1125,11 @@ extern "C" int dvq_prior_verify(const DvqPriorVerify* v, void* workspace, size_t
     if (v->B == 0) return DVQ_OK;
     if (!v->logits || !v->u_draw || !v->accepted || !v->next || (v->G > 0 && (!v->draft || !v->tokens || !v->u_accept)))
         return fail(DVQ_EINVAL, "prior_verify: null pointer");
-    // (workgroups of the largest launch: one per row, position and chunk)
+    // (threads of the largest launch: a wave or more per row, four waves or more, or four per row, position and chunk)
+    const bool short_rows = v->V <= 2 * kTile, split = verify_split(v->B, v->V, v->logits_v == 1 && (v->draft_v == 1 || v->G == 0));
     const int64_t chunks = (v->V + kTile * kChunk - 1) / (kTile * kChunk), per = (v->V + kTile * kSplitWaves - 1) / (kTile * kSplitWaves);
-    if (v->B * (v->P * chunks > per ? v->P * chunks : per) > 0x7FFFFFFF) return fail(DVQ_EINVAL, "prior_verify: B x P x V too large");
+    const int64_t groups = !split ? 1 : v->P * chunks > per ? v->P * chunks : per;
+    if (!launch_fits(v->B * groups, short_rows ? 64 : kSplitWaves * 64)) return fail(DVQ_EINVAL, "prior_verify: B x P x V too large");
     const size_t need = dvq_prior_verify_workspace_bytes(v);
     if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
         return fail(DVQ_EINVAL, "prior_verify: needs a 16-byte aligned workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : 0);

@@ -296,3 +296,116 @@ def test_two_streams_at_once():
     for i in range(2):
         for a, n in got[i]:
             assert torch.equal(a, want[i][0]) and torch.equal(n, want[i][1])
+
+
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("B,G,P,V", [(1500, 70, 71, 20), (2, 130, 130, 40), (1, 70, 71, 600), (3, 65, 66, 520), (200, 66, 67, 1100), (800, 65, 65, 1030),
+                                     (2, 66, 67, 2000)])
+def test_more_drafted_codes_than_a_wave_has_lanes(B, G, P, V, probs):
+    """Drafts next to the target: rows of every length up to all G codes kept."""
+    c = make(B, G, P, V, probs=probs, sigma=0.01, seed=G + V)
+    a, _ = check(c, probs=probs)
+    assert (a > 64).any()
+    if not probs and B < 10:
+        c["draft"] = c["logits"][:, :G].clone()
+        a, _ = check(c)
+        assert (a == G).all()
+
+
+@pytest.mark.parametrize("G,P", [(65, 65), (65, 66), (66, 67), (68, 69)])
+@pytest.mark.parametrize("B,V", [(3, 40), (3, 1500), (200, 1500)])
+def test_a_border_behind_the_64th_code(B, V, G, P):
+    """The last drafted code's u a 1e-12th below and above p / q: an unsure test in the second set of drafted codes."""
+    c = make(B, G, P, V, seed=G + V)
+    c["draft"] = c["logits"][:, :G].clone()
+    c["draft"][:, G - 1] += torch.randn(B, V, generator=torch.Generator().manual_seed(V))
+    want = []
+    for b in range(B):
+        p, q = S.distribution(c["logits"][b, G - 1].numpy()), S.distribution(c["draft"][b, G - 1].numpy())
+        x = int(np.argmin(p / q))
+        c["tokens"][b, G - 1] = x
+        c["u_accept"][b, G - 1] = p[x] / q[x] * (1 - 1e-12 if b % 2 else 1 + 1e-12)
+        want.append(G if b % 2 else G - 1)
+    a, _ = check(c)
+    assert a.tolist() == want
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("B,G,P,V", [(192, 3, 3, 1025), (200, 3, 4, 1537), (768, 2, 3, 1025), (800, 3, 3, 2047), (200, 0, 1, 1300), (770, 0, 1, 1300),
+                                     (191, 3, 4, 1025), (193, 2, 3, 9000)])
+def test_a_workgroup_per_row(B, G, P, V, probs, dtype):
+    check(make(B, G, P, V, dtype, torch.float32 if probs else dtype, probs, sigma=0.3, seed=B), probs=probs)
+    check(make(B, G, P, V, dtype, torch.bfloat16, probs, sigma=0.3, seed=B, masked=0.4), lengths=torch.arange(B) % (G + 2), probs=probs)
+
+
+@pytest.mark.parametrize("B", [200, 800])
+def test_a_workgroup_per_row_with_odd_rows_of_its_own_types(B):
+    """Rows of odd lengths inside wider buffers (no row starts at a multiple of 16 bytes), target and draft of different types."""
+    def odd(k, v):
+        if k not in ("logits", "draft"):
+            return v
+        wide = torch.full((*v.shape[:-1], v.shape[-1] + 6), 9, dtype=v.dtype, device=DEV)
+        wide[..., 5:5 + v.shape[-1]] = v
+        return wide[..., 5:5 + v.shape[-1]]
+    for t, d in ((torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32)):
+        for probs in (False, True):
+            check(make(B, 3, 4, 1803, t, d, probs, sigma=0.3, seed=B), probs=probs, place=odd)
+
+
+@pytest.mark.parametrize("B", [200, 800])
+@pytest.mark.parametrize("sigma", [0.0, 1e-3, 3.0])
+@pytest.mark.parametrize("probs", [False, True])
+def test_a_workgroup_per_row_and_drafts_near_and_far(B, sigma, probs):
+    """Next to equal distributions leave residual weights next to zero in every tile, and next to no mass."""
+    c = make(B, 2, 3, 1600, probs=probs, sigma=sigma, seed=B)
+    check(c, probs=probs)
+    c["u_accept"][:, 1] = 1.0 - 2.0 ** -53                   # rejections even there
+    c["tokens"][::3] = 0
+    check(c, probs=probs)
+
+
+@pytest.mark.parametrize("B", [200, 800])
+@pytest.mark.parametrize("probs", [False, True])
+def test_a_workgroup_per_row_and_distributions_without_mass(B, probs):
+    c = make(B, 2, 3, 1100, probs=probs, sigma=0.1, seed=B)
+    for b in range(0, B, 2):
+        which = "logits" if b % 4 else "draft"
+        g, v = b // 4 % c[which].shape[1], (-INF, float("nan"), INF)[b // 2 % 3]
+        if v == -INF and not (probs and which == "draft"):
+            c[which][b, g] = v
+        else:
+            c[which][b, g, (b * 37) % 1100] = v
+    check(c, probs=probs)
+
+
+@pytest.mark.parametrize("B", [200, 800])
+def test_a_workgroup_per_row_next_to_the_borders(B):
+    """Acceptance and draws a 1e-12th and a 1e-11th next to a border."""
+    V = 1700
+    c = make(B, 1, 2, V, seed=V + B)
+    want = []
+    for b in range(B):
+        p, q = S.distribution(c["logits"][b, 0].numpy()), S.distribution(c["draft"][b, 0].numpy())
+        x = int(np.argmin(p / q))
+        c["tokens"][b, 0] = x
+        c["u_accept"][b, 0] = p[x] / q[x] * (1 - 1e-12 if b % 2 else 1 + 1e-12)
+        cdf = np.cumsum(S.distribution(c["logits"][b, 1].numpy()))
+        k = (b * 31) % (V - 1)
+        while min(cdf[k] - (cdf[k - 1] if k else 0.0), cdf[k + 1] - cdf[k]) < 1e-9:
+            k = (k + 1) % (V - 1)
+        c["u_draw"][b] = cdf[k] + (1e-11 if b % 4 == 3 else -1e-11)
+        want.append((b % 2, k + 1 if b % 4 == 3 else k))
+    a, n = check(c)
+    assert a.tolist() == [w[0] for w in want]
+    assert all(n[b] == w[1] for b, w in enumerate(want) if w[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,P", [(1, 2), (2, 3), (63, 5), (511, 3), (513, 9), (900, 9), (1000, 9), (1024, 16), (77, 16)])
+def test_logits_with_all_positions_of_a_code_side_by_side(V, P, dtype):
+    """The prior's layout in short rows: copied whole up to 32 KiB, read in place above."""
+    place = lambda k, v: v.transpose(1, 2).contiguous().transpose(1, 2) if k == "logits" else v
+    for B in (1, 40, 5000 if V * P < 400 else 60):
+        check(make(B, P - 1, P, V, dtype, sigma=0.3, seed=V), place=place)
+        check(make(B, P, P, V, dtype, probs=True, sigma=0.3, seed=V), probs=True, place=place)

@@ -152,3 +152,13 @@ def test_head_dtype_is_set_on_the_heads_alone():
     assert m.obj_encoder_type.compute_dtype == torch.float32 and m.GatedPixelCNN.compute_dtype == torch.float32
     with pytest.raises(ValueError):
         set_head_dtype(m, torch.float16)
+
+
+def test_sizes_that_no_launch_holds_are_refused():
+    lib = _lib.load()
+    assert _quantize(lib, M=1 << 26) == -1 and b"2^26" in lib.dvq_last_error()
+    for bad in (dict(M=1 << 26, N=1 << 10, ldy=1 << 10), dict(M=(1 << 30) + 1), dict(N=(1 << 30) + 1, ldy=1 << 31), dict(N=1 << 28, ldy=1 << 28),
+                dict(M=100, N=1 << 26, ldy=1 << 26, ldw=17)):
+        assert _product(lib, **bad) == -1 and lib.dvq_last_error()
+    for bad in (dict(B=1 << 26, V=8), dict(B=1 << 24, V=5000, logits_v=1, draft_v=1), dict(B=1 << 20, V=1 << 20, logits_v=9, draft_v=9)):
+        assert lib.dvq_prior_verify(ctypes.byref(_verify_args(**bad)), 16, 1 << 60, None) == -1 and b"too large" in lib.dvq_last_error()
