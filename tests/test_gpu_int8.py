@@ -257,3 +257,67 @@ def test_two_streams_at_once():
                 got[i].append(ops.linear_int8(xs[i], W, t, b))
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
+
+
+# ------------------------------------------------------------------- every tile
+# 64 x 64, 128 x 128 and 256 x 256 tiles: tails in rows and channels, k of one stage and less, of an odd number of stages, of
+# no whole pieces
+TILES = [(700, 64, 650), (450, 1037, 640), (1500, 200, 1400), (1411, 528, 1345), (2048, 16, 1536), (4000, 130, 2100), (8193, 64, 1000), (4099, 304, 2049),
+         (2048, 1040, 4096)]
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,K,N", TILES)
+def test_product_of_many_rows_equals_whole_number_arithmetic(M, K, N, out_dtype):
+    x = rows(M, K, torch.float32, M + K + N)
+    W, t, b = layer(N, K, N)
+    codes, scale = S.int8_codes(x)
+    relu = N % 2 == 0
+    y = ops.linear_int8(x.to(DEV), W.to(DEV), t.to(DEV), b.to(DEV), relu=relu, out_dtype=out_dtype)
+    check_output(y, codes, scale, W, t, b, relu)
+    # a row is the same bits alone, among few and among all
+    for n in (1, 16, 40, 300):
+        assert torch.equal(y[:n], ops.linear_int8(x[:n].to(DEV), W.to(DEV), t.to(DEV), b.to(DEV), relu=relu, out_dtype=out_dtype))
+    # columns of a wider buffer, at offsets that 16-byte stores reach and at others; what lies beside them stays
+    for left, right in ((8, 8), (3, 4)):
+        out = torch.full((M + 2, left + N + right), 5.0, dtype=out_dtype, device=DEV)
+        ops.linear_int8(x.to(DEV), W.to(DEV), t.to(DEV), b.to(DEV), relu=relu, out=out[1:-1, left:left + N])
+        assert torch.equal(out[1:-1, left:left + N], y)
+        assert (out[0] == 5).all() and (out[-1] == 5).all() and (out[:, :left] == 5).all() and (out[:, left + N:] == 5).all()
+
+
+@pytest.mark.parametrize("M,K,N", [(700, 80, 650), (1500, 200, 1400), (2100, 48, 1100)])
+def test_batches_of_many_rows_equal_one_at_a_time(M, K, N):
+    xs = [rows(M, K, torch.bfloat16, i).to(DEV) for i in range(8)]
+    layers = [layer(N, K, i) for i in range(8)]
+    Ws, ts = [l[0].to(DEV) for l in layers], [l[1].to(DEV) for l in layers]
+    bs = [l[2].to(DEV) if i % 3 else None for i, l in enumerate(layers)]
+    for y, x, W, t, b in zip(ops.linear_int8_batched(xs, Ws, ts, bs, relu=True), xs, Ws, ts, bs):
+        assert torch.equal(y, ops.linear_int8(x, W, t, b, relu=True))
+
+
+def test_rows_and_channels_of_no_finite_scale_in_every_tile():
+    for M, K, N in ((450, 96, 640), (1500, 96, 1400), (2048, 96, 4096)):
+        x = rows(M, K, torch.float32, M)
+        x[5, 3], x[M - 1, K - 1], x[M // 2] = float("nan"), float("inf"), 0.0
+        W, t, b = layer(N, K, N)
+        t[7], t[N - 1], b[9] = float("nan"), float("inf"), -float("inf")
+        codes, scale = S.int8_codes(x)
+        check_output(ops.linear_int8(x.to(DEV), W.to(DEV), t.to(DEV), b.to(DEV)), codes, scale, W, t, b, False)
+
+
+def test_single_rows_and_features_of_any_stride_together():
+    """One row's stride and one feature's are nobody's business."""
+    W, t, b = layer(40, 70, 2)
+    args = [W.to(DEV)] * 3, [t.to(DEV)] * 3, [b.to(DEV)] * 3
+    wide = torch.randn(9, 200, generator=torch.Generator().manual_seed(3)).to(DEV)
+    xs = [wide[1:2, :70], wide[3:4, 80:150].contiguous(), wide[::4][1:2, 10:80]]
+    for y, x in zip(ops.linear_int8_batched(xs, *args), xs):
+        assert torch.equal(y, ops.linear_int8(x, W.to(DEV), t.to(DEV), b.to(DEV)))
+    with pytest.raises(RuntimeError):
+        ops.linear_int8_batched([wide[:2, :70], wide[:2, 70:140].contiguous(), wide[:2, :70]], *args)
+    one = layer(40, 1, 4)
+    cols = [wide[:, 3:4], wide[:, 5:6].contiguous().t().contiguous().t(), wide[:, 9:10]]
+    layers = [one[0].to(DEV)] * 2, [one[1].to(DEV)] * 2, [one[2].to(DEV)] * 2
+    for y, x in zip(ops.linear_int8_batched([cols[0], cols[2]], *layers), (cols[0], cols[2])):
+        assert torch.equal(y, ops.linear_int8(x.contiguous(), one[0].to(DEV), one[1].to(DEV), one[2].to(DEV)))
