@@ -41,12 +41,21 @@ class _Int8Copy:
 
 
 def _int8_weight(layer):
-    """8-bit codes and per-channel scales of an nn.Linear's weight, kept on the layer and refreshed when the weight changes."""
+    """8-bit codes and per-channel scales of an nn.Linear's weight, kept on the layer and refreshed when the weight changes --
+    in place, where recorded graphs read them.  While a graph is recorded nothing is kept: the graph quantises for itself."""
     W = layer.weight.detach()
     key = (W.data_ptr(), W._version, dvq_hip.weights_epoch())
     kept = layer.__dict__.setdefault("_dvq_int8", _Int8Copy())
     if kept.key != key:
-        kept.codes, kept.scale = ops.quantize_rows(W.float())
+        codes, scale = ops.quantize_rows(W.float())
+        if torch.cuda.is_current_stream_capturing():
+            return codes, scale
+        if kept.key is not None and kept.codes.shape == codes.shape and kept.codes.device == codes.device:
+            kept.codes.copy_(codes)
+            kept.scale.copy_(scale)
+        else:
+            kept.codes, kept.scale = codes, scale
+        torch.cuda.current_stream(W.device).synchronize()        # other streams read them from now on
         kept.key = key
     return kept.codes, kept.scale
 

@@ -173,7 +173,7 @@ class GatedPixelCNN(dvq_hip.DropsPackedCopies, nn.Module):
         """Verify drafted grids x (int64 [B,H,W], raster order) against this prior: one forward with x as the history, then
         ops.prior_verify.  draft [B, H*W, input_dim]: the logits (draft_probs: probabilities, as generate(return_probs=True)
         of a drafting prior returns them) the codes were drawn from; u_accept float64 [B, H*W], u_draw float64 [B];
-        lengths int64 [B]: only the first so many cells of a grid are drafts.  Returns (accepted [B], next [B]): the first
+        lengths int64 [B]: only the first so many cells of a grid are drafts (the rest may hold anything).  Returns (accepted [B], next [B]): the first
         accepted cells of a grid and the code after them, where there is a cell for it (-1 where not), are distributed as
         generate()'s."""
         if x.dim() != 3:
@@ -184,7 +184,8 @@ class GatedPixelCNN(dvq_hip.DropsPackedCopies, nn.Module):
             return empty, empty.clone()
         if draft.dim() != 3 or draft.shape[:2] != (B, H * W):
             raise RuntimeError(f"GatedPixelCNN.verify: draft must be [{B},{H * W},codes], got {tuple(draft.shape)}")
-        cells = self.forward(x, label).flatten(2).transpose(1, 2)             # [B, H*W, codes], a view
+        # (cells behind a grid's drafts may hold anything, and a code outside the table is rejected: neither is looked up)
+        cells = self.forward(x.clamp(0, self.embedding.num_embeddings - 1), label).flatten(2).transpose(1, 2)     # [B, H*W, codes], a view
         return ops.prior_verify(cells, draft, x.reshape(B, H * W), u_accept, u_draw, lengths, draft_probs)
 
     # ------------------------------------------------------------------ sampling

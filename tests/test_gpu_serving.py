@@ -159,3 +159,58 @@ def test_8_bit_drafting_head_and_verification_together():
     ra, rn = S.verify(cells, d, x, ua, ud)
     assert np.array_equal(acc.cpu().numpy(), ra) and np.array_equal(nxt.cpu().numpy(), rn)
     assert 0 < acc.sum() < 9 * B
+
+
+def test_cells_behind_the_drafts_and_codes_outside_the_table():
+    """What lies behind a grid's drafts is not looked up; a drafted code outside the table is rejected, cells behind it are not
+    reached.  Every position's history is unchanged by either."""
+    B = 40
+    target = prior(4)
+    V = target.embedding.num_embeddings
+    g = torch.Generator().manual_seed(8)
+    label = torch.randint(0, 16, (B,), generator=g).to(DEV)
+    x = torch.randint(0, V, (B, 9), generator=g).to(DEV)
+    with torch.no_grad():
+        q = target(x.view(B, 3, 3), label).flatten(2).transpose(1, 2).contiguous()
+    u = lambda *s: torch.rand(*s, generator=g, dtype=torch.float64).to(DEV)
+    ua, ud, lengths = u(B, 9), u(B), torch.arange(B, device=DEV) % 10
+    acc, nxt = target.verify(x.view(B, 3, 3), label, q, ua, ud, lengths=lengths)
+    assert torch.equal(acc, lengths)                                  # drafted by the prior itself
+    behind = torch.arange(9, device=DEV)[None, :] >= lengths[:, None]
+    for fill in (-1, V, 1 << 40, -(1 << 62)):
+        y = torch.where(behind, fill, x)
+        a, n = target.verify(y.view(B, 3, 3), label, q, ua, ud, lengths=lengths)
+        assert torch.equal(a, acc) and torch.equal(n, nxt)
+        a, n = target.verify(y.view(B, 3, 3), label, q, ua, ud)       # now they are drafts
+        assert torch.equal(a, lengths) and (n[lengths < 9] >= 0).all() and (n[lengths == 9] == -1).all()
+
+
+def test_8_bit_heads_in_recorded_graphs():
+    """The first call recorded (the copy of the weights is not kept then), eager calls before its replay, a graph over a kept copy
+    that a changed weight refreshes in place, and a graph and eager calls in turns."""
+    e = set_head_dtype(head(Encoder, [64, 32], 16, 9), torch.int8)
+    x = torch.randn(40, 64, generator=torch.Generator().manual_seed(1)).to(DEV)
+    spare = set_head_dtype(head(Encoder, [64, 32], 16, 9), torch.int8)
+    want = spare(x)
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            spare(x)                                                  # (the kernels are loaded)
+        torch.cuda.current_stream().wait_stream(side)
+        with torch.cuda.graph(first):
+            a = e(x)
+        assert torch.equal(e(x), want)
+        with torch.cuda.graph(second):
+            b = e(x)
+        for scale in (1.0, 2.0, 0.5):
+            e.linear_means.weight.mul_(scale)
+            spare.linear_means.weight.mul_(scale)
+            want = spare(x)
+            first.replay()                                            # quantises for itself
+            assert torch.equal(a, want)
+            assert torch.equal(e(x), want)
+            second.replay()                                           # reads the copy that the call above refreshed
+            assert torch.equal(b, want)
+            torch.cuda.synchronize()
