@@ -258,13 +258,14 @@ __device__ __forceinline__ Sum sum_held(const float (&x)[TILES][8]) {
 enum { VERIFY_KEEP = 0, VERIFY_REJECT = 1, VERIFY_BAD = 2, VERIFY_UNSURE = 3 };
 
 // What the tests of a row's drafted codes read beside the sums: lane l holds that of position g0 + l, so that it is asked for
-// once, in front of everything else.  A code outside the table reads the table's end.
+// once, in front of everything else (the row's length among it: positions behind it are read in vain).  A code outside the
+// table reads the table's end.
 template <typename T, typename D>
 struct Drafted {
     float t, d; double u; int inside;
-    __device__ __forceinline__ void fetch(const VerifyArgs& a, int64_t b, int g0, int n, int lane) {
-        if (g0 >= n) return;
-        const int g = g0 + lane < n ? g0 + lane : n - 1;
+    __device__ __forceinline__ void fetch(const VerifyArgs& a, int64_t b, int g0, int lane) {
+        if (g0 >= a.G) return;
+        const int g = g0 + lane < a.G ? g0 + lane : a.G - 1;
         const int64_t x = a.tokens[b * a.tb + g * a.tg], at = x < 0 ? 0 : x < a.V ? x : a.V - 1;
         inside = x == at;
         u = a.u[b * a.ub + g * a.ug];
@@ -481,7 +482,7 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(TILES == 1
     const int n = verify_length(a, b);
     const double at_draw = a.r[b * a.rb];
     Drafted<T, D> drafted;
-    drafted.fetch(a, b, 0, n, lane);
+    drafted.fetch(a, b, 0, lane);
     const float none = -__builtin_inff();
     T* const staged = reinterpret_cast<T*>(block);
     if (STAGED) {
@@ -504,7 +505,7 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(TILES == 1
         float t[TILES][8], q[TILES][8];
         if (g - held >= 64) {
             held = g / 64 * 64;
-            drafted.fetch(a, b, held, n, lane);
+            drafted.fetch(a, b, held, lane);
         }
         const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)g * a.lp;
         const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
@@ -619,7 +620,7 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(TILES == 1
 // The draw of a row whose tiles have been passed over: mass, c and near of every tile in LDS, sp and sq the sums of e_p and e_q.
 // Every wave calls it.
 template <typename T, typename D, bool PROBS>
-__device__ __forceinline__ void verify_finish(const Exp& ex, const VerifyArgs& args, int64_t b, const T* lr, const D* dr, Weights w, bool unit, double sp,
+__device__ __forceinline__ void verify_finish(const Exp& ex, const VerifyArgs& args, int64_t b, double at_draw, const T* lr, const D* dr, Weights w, bool unit, double sp,
                                               double sq, double* a, const double* c, const unsigned char* near, int tiles, double* lds) {
     const int wave = verify_wave(), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     double total = 0.0;
@@ -656,7 +657,7 @@ __device__ __forceinline__ void verify_finish(const Exp& ex, const VerifyArgs& a
         if (lane == 0) args.next[b] = -1;
         return;
     }
-    const double thr = args.r[b * args.rb] * total;
+    const double thr = at_draw * total;
     double before, ep[8], eq[8];
     bool over;
     const int i = verify_pick(a, tiles, thr, before, over);
@@ -757,13 +758,14 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(4)))
     const int V = a.V, tiles = (V + kTile - 1) / kTile;
     double* tile_c = tile_a + tiles;
     unsigned char* tile_near = reinterpret_cast<unsigned char*>(tile_c + tiles);
-    const int n = verify_length(a, b);
     const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb;
     const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db;
     Sum p = {0.f, 0.f, 1.0}, q = {0.f, 0.f, 1.0};
     int g = 0, st = VERIFY_KEEP;
+    const int n = verify_length(a, b);
+    const double at_draw = a.r[b * a.rb];
     Drafted<T, D> drafted;
-    drafted.fetch(a, b, 0, n, lane);
+    drafted.fetch(a, b, 0, lane);
     const Share share(wave, WAVES, V, Ring<T, D, !PROBS>::N);
     Ring<T, D, !PROBS> ring;
     if (a.G == 0) dr = reinterpret_cast<const D*>(lr);           // (read in vain, and 512 codes of either type fit a row)
@@ -772,7 +774,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(4)))
         const bool both = !PROBS && g < n, more = g + 1 < a.P && g + 1 <= n, nboth = !PROBS && g + 1 < n;
         const T* nl = more ? lr + a.lp : lr;
         const D* nd = g + 1 < n ? dr + a.dg : dr;
-        if (g > 0 && g % 64 == 0) drafted.fetch(a, b, g, n, lane);
+        if (g > 0 && g % 64 == 0) drafted.fetch(a, b, g, lane);
         p = q = Sum{-__builtin_inff(), 0.f, 0.0};
         verify_sums(ring, share, lr, dr, both, nl, nd, nboth, V, lane, p, q);
         __builtin_amdgcn_sched_barrier(0);
@@ -843,7 +845,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(4)))
     sp = sq = 0.0;
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) { sp += parts64[0][i]; sq += parts64[1][i]; }
-    verify_finish<T, D, PROBS>(ex, a, b, lr, dr, w, true, sp, sq, tile_a, tile_c, tile_near, tiles, lds);
+    verify_finish<T, D, PROBS>(ex, a, b, at_draw, lr, dr, w, true, sp, sq, tile_a, tile_c, tile_near, tiles, lds);
 }
 
 // ------------------------------------------------------------- long rows cut among workgroups: three launches
@@ -880,8 +882,6 @@ __device__ __forceinline__ SplitRow split_row(char* ws, const VerifyArgs& a, int
 template <typename T, typename D, bool PROBS>
 __global__ __launch_bounds__(kSplitWaves * 64) void verify_stats_kernel(VerifyArgs a, char* ws, int chunks, int groups) {
     __shared__ Sum parts[2][kSplitWaves];
-    __shared__ double table[32];
-    const Exp ex = verify_table(table);
     const int wave = verify_wave(), lane = threadIdx.x & 63;
     const int64_t id = blockIdx.x;
     const int chunk = (int)(id % chunks), group = (int)(id / chunks % groups);
@@ -943,9 +943,10 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_stats_kernel(VerifyAr
     }
 }
 
-__device__ __forceinline__ Sum split_join(const Exp& ex, const Sum* parts, int chunks, int lane) {       // one wave
-    Sum a = {-__builtin_inff(), 0.f, 0.0};
-    for (int i = lane; i < chunks; i += 64) {
+// The chunks' sums as one (one wave); `a`: this lane's first part.
+__device__ __forceinline__ Sum split_join(const Exp& ex, Sum a, const Sum* parts, int chunks, int lane) {
+    if (lane >= chunks) a = Sum{-__builtin_inff(), 0.f, 0.0};
+    for (int i = lane + 64; i < chunks; i += 64) {
         const Sum t = parts[i];
         const float top = fmaxf(a.ref, t.ref);
         a.s = sum_moved(ex, a, top) + sum_moved(ex, t, top);
@@ -969,17 +970,25 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_pass_kernel(VerifyArg
     const SplitRow row = split_row(ws, a, b);
     Sum p = {0.f, 0.f, 1.0}, q = {0.f, 0.f, 1.0};
     int st = VERIFY_KEEP, g = 0;
+    Sum pp, qq;                                            // this lane's part of the wave's position
+    const auto ask = [&](int mine) {                             // (a position that is not there: the last one)
+        const int at = lane < chunks ? lane : chunks - 1;
+        pp = row.p[(mine < a.P ? mine : a.P - 1) * chunks + at];
+        if (!PROBS && a.G > 0) qq = row.q[(mine < a.G ? mine : a.G - 1) * chunks + at];
+    };
+    ask(wave);
     Drafted<T, D> drafted;
-    drafted.fetch(a, b, 0, n, lane);
+    drafted.fetch(a, b, 0, lane);
     for (int base = 0; st == VERIFY_KEEP; base += kSplitWaves) {
+        if (base > 0) ask(base + wave);
         const int mine = base + wave;
         int s = mine == n ? (n < a.P ? VERIFY_REJECT : VERIFY_BAD) : VERIFY_KEEP;
         // (every wave, also one whose own position is not there: all of them read position g's if its test is unsure)
-        if (base > 0 && base % 64 == 0) drafted.fetch(a, b, base, n, lane);
+        if (base > 0 && base % 64 == 0) drafted.fetch(a, b, base, lane);
         if (mine <= n && mine < a.P) {
-            p = split_join(ex, row.p + mine * chunks, chunks, lane);
+            p = split_join(ex, pp, row.p + mine * chunks, chunks, lane);
             if (mine < n) {
-                if (!PROBS) q = split_join(ex, row.q + mine * chunks, chunks, lane);
+                if (!PROBS) q = split_join(ex, qq, row.q + mine * chunks, chunks, lane);
                 s = verify_test<PROBS>(ex, drafted.of(mine & 63), p, q, false);
             } else if (!sum_ok(p)) s = VERIFY_BAD;
         }
@@ -1037,17 +1046,17 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_draw_kernel(VerifyArg
     const SplitRow row = split_row(ws, a, b);
     const int tiles = (a.V + kTile - 1) / kTile, n = verify_length(a, b);
     const Decision d = *row.d;
+    const double at_draw = a.r[b * a.rb];
     double* tile_c = tile_a + tiles;
     unsigned char* tile_near = reinterpret_cast<unsigned char*>(tile_c + tiles);
     double sp = 0.0, sq = 0.0;
-    if (d.st == VERIFY_REJECT)                                   // (the tiles of other rows were not written)
-        for (int i = threadIdx.x; i < tiles; i += kSplitWaves * 64) {
-            sp += row.sp[i];
-            sq += row.sq[i];
-            tile_a[i] = row.a[i];
-            tile_c[i] = row.c[i];
-            tile_near[i] = row.near[i];
-        }
+    for (int i = threadIdx.x; i < tiles; i += kSplitWaves * 64) {      // (not written where the row draws nothing, and not used there)
+        sp += row.sp[i];
+        sq += row.sq[i];
+        tile_a[i] = row.a[i];
+        tile_c[i] = row.c[i];
+        tile_near[i] = row.near[i];
+    }
     const Exp ex = verify_table(table);
     if (d.st != VERIFY_REJECT) return;
     sp = wave_sum(sp);
@@ -1060,7 +1069,7 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_draw_kernel(VerifyArg
     const Weights w = {(double)d.p_ref, (double)d.q_ref, d.k, d.g < n};
     const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)d.g * a.lp;
     const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)d.g * a.dg;
-    verify_finish<T, D, PROBS>(ex, a, b, lr, dr, w, a.unit, sp, sq, tile_a, tile_c, tile_near, tiles, lds);
+    verify_finish<T, D, PROBS>(ex, a, b, at_draw, lr, dr, w, a.unit, sp, sq, tile_a, tile_c, tile_near, tiles, lds);
 }
 
 // Rows that the workgroup-per-row form takes; fewer, or codes that do not lie side by side, are cut among workgroups.
