@@ -449,10 +449,10 @@ def linear_int8_batched(xs, Ws, w_scales, bs, relu: bool = False, out_dtype: tor
         for t in group:
             if t.dtype != dtype or t.shape != shape or t.get_device() != index or (t.stride() != stride and _rows(t, (dtype,), dev, what, "x or W") != ld):
                 raise RuntimeError(f"{what}: {message}, on {dev}")
-    for name, group in (("every w_scale", w_scales), ("every b", bs)):
-        for t in group:
-            if t is not None or group is w_scales:
-                _vector(t, N, dev, what, name)
+    shape, f32 = w_scales[0].shape, torch.float32
+    for t in (*w_scales, *[b for b in bs if b is not None]):
+        if t.dtype != f32 or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
+            raise RuntimeError(f"{what}: every w_scale and b must be a contiguous float32 [{N}] on {dev}")
     if pairs:
         for _, s in xs:
             _vector(s, M, dev, what, "the scale of x")
