@@ -442,7 +442,7 @@ __device__ __forceinline__ double verify_total(const double* v, int n) {
 
 // Sum of exp(x - ref) of a whole row in 64 bits by the whole workgroup, for the tests too near to tell.
 template <typename T>
-__device__ __noinline__ double verify_row_sum64(Exp ex, const T* row, int64_t sv, bool unit, int V, double ref, double* parts) {
+static __device__ __noinline__ double verify_row_sum64(Exp ex, const T* row, int64_t sv, bool unit, int V, double ref, double* parts) {
     const int wave = verify_wave(), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     double s = 0.0;
     for (int v0 = wave * kTile; v0 < V; v0 += waves * kTile) {
@@ -993,14 +993,18 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_pass_kernel(VerifyArg
             } else if (!sum_ok(p)) s = VERIFY_BAD;
         }
         __syncthreads();
-        if (lane == 0) { sums[0][wave] = p; sums[1][wave] = q; state[wave] = s; }
+        if (lane == 0) {
+            sums[0][wave] = p;
+            if (!PROBS) sums[1][wave] = q;
+            state[wave] = s;
+        }
         __syncthreads();
         for (int i = 0; i < kSplitWaves && st == VERIFY_KEEP; ++i) {     // (position n always stops: the loop ends)
             st = state[i];
             g = base + i;
             if (st == VERIFY_KEEP) continue;
             p = sums[0][i];
-            q = sums[1][i];
+            if (!PROBS) q = sums[1][i];
             if (st == VERIFY_UNSURE) {
                 const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)g * a.lp;
                 const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
