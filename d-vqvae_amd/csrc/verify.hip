@@ -463,6 +463,20 @@ static __device__ __noinline__ double verify_row_sum64(Exp ex, const T* row, int
     return all;
 }
 
+// Copies elements that lie side by side into LDS; the whole workgroup.
+template <typename T>
+__device__ __forceinline__ void verify_copy(const T* from, int total, T* to) {
+    constexpr int N = 16 / sizeof(T);
+    int i = threadIdx.x * N;
+#pragma unroll 4
+    for (; i + N <= total; i += blockDim.x * N) {
+        u32x4 v;
+        __builtin_memcpy(&v, from + i, 16);
+        *reinterpret_cast<u32x4*>(to + i) = v;
+    }
+    for (; i < total; ++i) to[i] = from[i];                      // (at most one thread has a rest)
+}
+
 // ------------------------------------------------------------------------------------------------ rows of up to 1024 codes
 // One workgroup per row, one wave per position: `blockDim / 64` positions at a time until the first that stops the row.
 // Its wave holds the position's logits in registers and draws from them.
@@ -487,16 +501,7 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(TILES == 1
     T* const staged = reinterpret_cast<T*>(block);
     if (STAGED) {
         const T* from = reinterpret_cast<const T*>(a.logits) + b * a.lb;
-        constexpr int N = 16 / sizeof(T);
-        const int total = V * a.P;
-        int i = threadIdx.x * N;
-#pragma unroll 4
-        for (; i + N <= total; i += blockDim.x * N) {
-            u32x4 v;
-            __builtin_memcpy(&v, from + i, 16);
-            *reinterpret_cast<u32x4*>(staged + i) = v;
-        }
-        for (; i < total; ++i) staged[i] = from[i];              // (at most one thread has a rest)
+        verify_copy(from, V * a.P, staged);
     }
     const Exp ex = verify_table(table);
     int held = 0;                                                // first of the 64 drafted codes at hand
@@ -858,13 +863,18 @@ struct SplitRow {
     Sum* p; Sum* q; Decision* d;
     double *sp, *sq, *a, *c; unsigned char* near;
 };
-__host__ __device__ inline int64_t split_bytes(int P, int G, int V) {
-    const int64_t tiles = (V + kTile - 1) / kTile, chunks = (tiles + kChunk - 1) / kChunk;
+// Test sums of a position: one per chunk, one per tile where codes do not lie side by side.
+__host__ __device__ inline int64_t split_parts(int V, bool unit) {
+    const int64_t tiles = (V + kTile - 1) / kTile;
+    return unit ? (tiles + kChunk - 1) / kChunk : tiles;
+}
+__host__ __device__ inline int64_t split_bytes(int P, int G, int V, bool unit) {
+    const int64_t tiles = (V + kTile - 1) / kTile, chunks = split_parts(V, unit);
     return (P + G) * chunks * (int64_t)sizeof(Sum) + (int64_t)sizeof(Decision) + 4 * tiles * 8 + (tiles + 15) / 16 * 16 + 8;
 }
 __device__ __forceinline__ SplitRow split_row(char* ws, const VerifyArgs& a, int64_t b) {
-    const int64_t tiles = (a.V + kTile - 1) / kTile, chunks = (tiles + kChunk - 1) / kChunk;
-    char* at = ws + b * ((split_bytes(a.P, a.G, a.V) + 15) / 16 * 16);
+    const int64_t tiles = (a.V + kTile - 1) / kTile, chunks = split_parts(a.V, a.unit);
+    char* at = ws + b * ((split_bytes(a.P, a.G, a.V, a.unit) + 15) / 16 * 16);
     SplitRow r;
     r.p = reinterpret_cast<Sum*>(at);
     r.q = r.p + a.P * chunks;
@@ -877,68 +887,92 @@ __device__ __forceinline__ SplitRow split_row(char* ws, const VerifyArgs& a, int
     return r;
 }
 
-// Test sums of one chunk: of one position, or, where codes lie apart and a chunk's positions share cache lines, of all of
-// them one after the other.  All positions are summed: which ones the row needs is not known yet.
+// Test sums of one chunk of one position.  All positions are summed: which ones the row needs is not known yet.
 template <typename T, typename D, bool PROBS>
-__global__ __launch_bounds__(kSplitWaves * 64) void verify_stats_kernel(VerifyArgs a, char* ws, int chunks, int groups) {
+__global__ __launch_bounds__(kSplitWaves * 64) void verify_stats_kernel(VerifyArgs a, char* ws, int chunks) {
     __shared__ Sum parts[2][kSplitWaves];
     const int wave = verify_wave(), lane = threadIdx.x & 63;
     const int64_t id = blockIdx.x;
-    const int chunk = (int)(id % chunks), group = (int)(id / chunks % groups);
-    const int64_t b = id / chunks / groups;
+    const int chunk = (int)(id % chunks), g = (int)(id / chunks % a.P);
+    const int64_t b = id / chunks / a.P;
+    const int n = verify_length(a, b);
+    if (g > n) return;
+    const SplitRow row = split_row(ws, a, b);
+    const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)g * a.lp;
+    const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
+    const bool both = !PROBS && g < n;
+    Sum p = {-__builtin_inff(), 0.f, 0.0}, q = p;
+    const int tiles = (a.V + kTile - 1) / kTile, last = (chunk + 1) * kChunk < tiles ? (chunk + 1) * kChunk : tiles;
+    constexpr int N = kChunk / kSplitWaves;                      // this wave's tiles, all asked for at once
+    Raw<T> x[N];
+    Raw<D> y[N];
+    int at[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int i = chunk * kChunk + wave + k * kSplitWaves;
+        at[k] = verify_base(true, (i < tiles ? i : tiles - 1) * kTile, a.V) + 8 * lane;
+        x[k].load(lr + at[k]);
+    }
+    if (both)
+#pragma unroll
+        for (int k = 0; k < N; ++k) y[k].load(dr + at[k]);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int i = chunk * kChunk + wave + k * kSplitWaves;
+        if (i >= last) continue;
+        sum_raw(p, x[k], i * kTile - at[k]);
+        if (both) sum_raw(q, y[k], i * kTile - at[k]);
+    }
+    p = sum_wave(p);
+    if (both) q = sum_wave(q);
+    if (lane == 0) { parts[0][wave] = p; parts[1][wave] = q; }
+    __syncthreads();
+    if (wave == 0) {
+        p = sum_parts(parts[0], kSplitWaves);
+        q = sum_parts(parts[1], kSplitWaves);
+        if (lane == 0) {
+            row.p[g * chunks + chunk] = p;
+            if (both) row.q[g * chunks + chunk] = q;
+        }
+    }
+}
+
+// Codes that do not lie side by side: the test sums of one tile of all positions, one wave per position in turns.  The
+// positions of a code share cache lines; where they are all that lies between a code and the next (the prior's forward), the
+// tile of all positions is one piece of memory and is copied into LDS (t_staged, d_staged) instead of fetched anew by every
+// position.
+constexpr int kCellWaves = 8;
+template <typename T>
+__device__ __forceinline__ Sum verify_cell_sum(const T* row, int64_t sv, const T* staged, int codes, int lane) {
+    float x[8];
+    Sum s = {-__builtin_inff(), 0.f, 0.0};
+    if (staged) verify_tile(staged, sv, false, 0, codes, lane, -__builtin_inff(), x);
+    else verify_tile(row, sv, false, 0, codes, lane, -__builtin_inff(), x);
+    sum_add(s, x);
+    return sum_wave(s);
+}
+template <typename T, typename D, bool PROBS>
+__global__ __launch_bounds__(kCellWaves * 64) void verify_cells_kernel(VerifyArgs a, char* ws, int tiles, bool t_staged, bool d_staged) {
+    extern __shared__ __align__(16) char block[];
+    const int wave = verify_wave(), lane = threadIdx.x & 63;
+    const int tile = (int)((int64_t)blockIdx.x % tiles);
+    const int64_t b = (int64_t)blockIdx.x / tiles;
+    const int codes = a.V - tile * kTile < kTile ? a.V - tile * kTile : kTile;
+    const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)tile * kTile * a.lv;
+    const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)tile * kTile * a.dv;
+    T* const t = reinterpret_cast<T*>(block);
+    D* const d = reinterpret_cast<D*>(block + (t_staged ? kTile * a.P * sizeof(T) : 0));
+    if (t_staged) verify_copy(lr, codes * a.P, t);
+    if (d_staged) verify_copy(dr, codes * a.G, d);
     const int n = verify_length(a, b);
     const SplitRow row = split_row(ws, a, b);
-    const int first = groups == 1 ? 0 : group, end = groups == 1 ? a.P : group + 1;
-    for (int g = first; g < end && g <= n; ++g) {
-        const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)g * a.lp;
-        const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)g * a.dg;
-        const bool both = !PROBS && g < n;
-        Sum p = {-__builtin_inff(), 0.f, 0.0}, q = p;
-        const int tiles = (a.V + kTile - 1) / kTile, last = (chunk + 1) * kChunk < tiles ? (chunk + 1) * kChunk : tiles;
-        if (a.unit) {
-            constexpr int N = kChunk / kSplitWaves;              // this wave's tiles, all asked for at once
-            Raw<T> x[N];
-            Raw<D> y[N];
-            int at[N];
-#pragma unroll
-            for (int k = 0; k < N; ++k) {
-                const int i = chunk * kChunk + wave + k * kSplitWaves;
-                at[k] = verify_base(true, (i < tiles ? i : tiles - 1) * kTile, a.V) + 8 * lane;
-                x[k].load(lr + at[k]);
-            }
-            if (both)
-#pragma unroll
-                for (int k = 0; k < N; ++k) y[k].load(dr + at[k]);
-#pragma unroll
-            for (int k = 0; k < N; ++k) {
-                const int i = chunk * kChunk + wave + k * kSplitWaves;
-                if (i >= last) continue;
-                sum_raw(p, x[k], i * kTile - at[k]);
-                if (both) sum_raw(q, y[k], i * kTile - at[k]);
-            }
-        }
-        else
-            for (int i = chunk * kChunk + wave; i < last; i += kSplitWaves) {
-                float x[8];
-                verify_tile(lr, a.lv, false, i * kTile, a.V, lane, -__builtin_inff(), x);
-                sum_add(p, x);
-                if (both) {
-                    verify_tile(dr, a.dv, false, i * kTile, a.V, lane, -__builtin_inff(), x);
-                    sum_add(q, x);
-                }
-            }
-        p = sum_wave(p);
-        if (both) q = sum_wave(q);
-        __syncthreads();
-        if (lane == 0) { parts[0][wave] = p; parts[1][wave] = q; }
-        __syncthreads();
-        if (wave == 0) {
-            p = sum_parts(parts[0], kSplitWaves);
-            q = sum_parts(parts[1], kSplitWaves);
-            if (lane == 0) {
-                row.p[g * chunks + chunk] = p;
-                if (both) row.q[g * chunks + chunk] = q;
-            }
+    __syncthreads();
+    for (int g = wave; g < a.P && g <= n; g += kCellWaves) {
+        const Sum p = verify_cell_sum(lr + (int64_t)g * a.lp, a.lv, t_staged ? t + g : nullptr, codes, lane);
+        if (lane == 0) row.p[(int64_t)g * tiles + tile] = p;
+        if (!PROBS && g < n) {
+            const Sum q = verify_cell_sum(dr + (int64_t)g * a.dg, a.dv, d_staged ? d + g : nullptr, codes, lane);
+            if (lane == 0) row.q[(int64_t)g * tiles + tile] = q;
         }
     }
 }
@@ -1078,21 +1112,28 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_draw_kernel(VerifyArg
 
 // Rows that the workgroup-per-row form takes; fewer, or codes that do not lie side by side, are cut among workgroups.
 constexpr int kRowsMin = 192;
-constexpr int kShortWaves = 16384;
+// Short rows, positions at a time: all at once for few rows, so that the call takes one position's time; with more rows a wave
+// behind the first rejection is work in vain.  So many waves in all (us with 1024 / 2048 / 4096 / 16384, logits side by side: 1050 rows of
+// 8 x 223 bf16 21 / 16 / 15 / 20, 719 of 13 x 1005 fp32 19 / 18 / 20 / 31, 300 of 12 x 300 14 / 14 / 17 / 17, 4096 of 9 x 512 26 / 26 / 27 / 35), and
+// of a row whose block is staged one for so many bytes at least (2000 rows of 7 x 1000, codes of all positions side by side: 3500 / 4608 /
+// 6144 bytes 66 / 67 / 46; 4096 of 9 x 512 53 / 41 / 38).
+constexpr int kShortWaves = 2048;
+constexpr int kShortStage = 6144;
+constexpr size_t kCellBytes = 65536;                         // LDS of a tile of all positions
 static bool verify_split(int64_t B, int V, bool unit) { return V > 2 * kTile && (!unit || B < kRowsMin); }
 
 template <typename T, typename D, bool PROBS>
 static int verify_launch(const VerifyArgs& a, char* ws, hipStream_t st) {
     const dim3 grid((unsigned)a.B);
     if (a.V <= 2 * kTile) {
-        // positions at a time: all at once for few rows, few where the rows alone fill the card
-        int64_t waves = kShortWaves / a.B;
+        const size_t block = (size_t)a.V * a.P * sizeof(T), room = (kTile + kTile / 8) * sizeof(double);
+        const bool staged = a.P > 1 && a.lp == 1 && a.lv == a.P && block <= 32768;
+        int64_t waves = (kShortWaves + a.B - 1) / a.B;
+        if (staged && waves < (int64_t)(block / kShortStage)) waves = block / kShortStage;
         if (waves > a.G + 1) waves = a.G + 1;
         if (waves > 16) waves = 16;
         if (waves < 1) waves = 1;
         const dim3 blk((unsigned)waves * 64);
-        const size_t block = (size_t)a.V * a.P * sizeof(T), room = (kTile + kTile / 8) * sizeof(double);
-        const bool staged = a.P > 1 && a.lp == 1 && a.lv == a.P && block <= 32768;
         const size_t lds = staged && block > room ? block : room;
         if (a.V <= kTile) {
             if (staged) hipLaunchKernelGGL((verify_short_kernel<1, true, T, D, PROBS>), grid, blk, lds, st, a);
@@ -1105,9 +1146,19 @@ static int verify_launch(const VerifyArgs& a, char* ws, hipStream_t st) {
     }
     const int tiles = (a.V + kTile - 1) / kTile;
     if (verify_split(a.B, a.V, a.unit)) {
-        const int chunks = (tiles + kChunk - 1) / kChunk, groups = a.unit ? a.P : 1, per = (tiles + kSplitWaves - 1) / kSplitWaves;
+        const int chunks = (int)split_parts(a.V, a.unit), per = (tiles + kSplitWaves - 1) / kSplitWaves;
         const dim3 blk(kSplitWaves * 64);
-        hipLaunchKernelGGL((verify_stats_kernel<T, D, PROBS>), dim3((unsigned)(a.B * groups * chunks)), blk, 0, st, a, ws, chunks, groups);
+        if (a.unit) hipLaunchKernelGGL((verify_stats_kernel<T, D, PROBS>), dim3((unsigned)(a.B * a.P * chunks)), blk, 0, st, a, ws, chunks);
+        else {
+            size_t lds = 0;
+            const size_t t_bytes = kTile * sizeof(T) * a.P, d_bytes = kTile * sizeof(D) * a.G;
+            const bool t_staged = a.P > 1 && a.lp == 1 && a.lv == a.P && t_bytes <= kCellBytes;
+            if (t_staged) lds += t_bytes;
+            const bool d_staged = !PROBS && a.G > 1 && a.dg == 1 && a.dv == a.G && lds + d_bytes <= kCellBytes;
+            if (d_staged) lds += d_bytes;
+            hipLaunchKernelGGL((verify_cells_kernel<T, D, PROBS>), dim3((unsigned)(a.B * tiles)), dim3(kCellWaves * 64), lds, st, a, ws, tiles,
+                               t_staged, d_staged);
+        }
         hipLaunchKernelGGL((verify_pass_kernel<T, D, PROBS>), dim3((unsigned)(a.B * per)), blk, 0, st, a, ws, chunks, per);
         hipLaunchKernelGGL((verify_draw_kernel<T, D, PROBS>), grid, blk, (size_t)tiles * 17, st, a, ws);
         return check_launch("prior_verify");
@@ -1124,8 +1175,9 @@ using namespace dvq;
 
 extern "C" size_t dvq_prior_verify_workspace_bytes(const DvqPriorVerify* v) {
     if (!v || v->B < 1 || v->V < 1 || v->P < 1 || v->G < 0) return 0;
-    if (!verify_split(v->B, v->V, v->logits_v == 1 && (v->draft_v == 1 || v->G == 0))) return 0;
-    return (size_t)v->B * (size_t)((split_bytes(v->P, v->G, v->V) + 15) / 16 * 16);
+    const bool unit = v->logits_v == 1 && (v->draft_v == 1 || v->G == 0);
+    if (!verify_split(v->B, v->V, unit)) return 0;
+    return (size_t)v->B * (size_t)((split_bytes(v->P, v->G, v->V, unit) + 15) / 16 * 16);
 }
 
 extern "C" int dvq_prior_verify(const DvqPriorVerify* v, void* workspace, size_t workspace_bytes, void* stream) {
@@ -1138,11 +1190,12 @@ extern "C" int dvq_prior_verify(const DvqPriorVerify* v, void* workspace, size_t
     if (v->B == 0) return DVQ_OK;
     if (!v->logits || !v->u_draw || !v->accepted || !v->next || (v->G > 0 && (!v->draft || !v->tokens || !v->u_accept)))
         return fail(DVQ_EINVAL, "prior_verify: null pointer");
-    // (threads of the largest launch: a wave or more per row, four waves or more, or four per row, position and chunk)
-    const bool short_rows = v->V <= 2 * kTile, split = verify_split(v->B, v->V, v->logits_v == 1 && (v->draft_v == 1 || v->G == 0));
-    const int64_t chunks = (v->V + kTile * kChunk - 1) / (kTile * kChunk), per = (v->V + kTile * kSplitWaves - 1) / (kTile * kSplitWaves);
-    const int64_t groups = !split ? 1 : v->P * chunks > per ? v->P * chunks : per;
-    if (!launch_fits(v->B * groups, short_rows ? 64 : kSplitWaves * 64)) return fail(DVQ_EINVAL, "prior_verify: B x P x V too large");
+    // (threads of the largest launch: a wave or more per short row, a workgroup per row, or per row and part of it)
+    const bool unit = v->logits_v == 1 && (v->draft_v == 1 || v->G == 0);
+    const bool short_rows = v->V <= 2 * kTile, split = verify_split(v->B, v->V, unit);
+    const int64_t parts = split_parts(v->V, unit) * (unit ? v->P : 1), per = (v->V + kTile * kSplitWaves - 1) / (kTile * kSplitWaves);
+    const int64_t groups = !split ? 1 : parts > per ? parts : per;
+    if (!launch_fits(v->B * groups, short_rows ? 64 : kCellWaves * 64)) return fail(DVQ_EINVAL, "prior_verify: B x P x V too large");
     const size_t need = dvq_prior_verify_workspace_bytes(v);
     if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
         return fail(DVQ_EINVAL, "prior_verify: needs a 16-byte aligned workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : 0);

@@ -409,3 +409,33 @@ def test_logits_with_all_positions_of_a_code_side_by_side(V, P, dtype):
     for B in (1, 40, 5000 if V * P < 400 else 60):
         check(make(B, P - 1, P, V, dtype, sigma=0.3, seed=V), place=place)
         check(make(B, P, P, V, dtype, probs=True, sigma=0.3, seed=V), probs=True, place=place)
+
+
+@pytest.mark.parametrize("tdt,ddt", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16)])
+@pytest.mark.parametrize("G,P,V", [(1, 1, 1100), (1, 2, 1300), (2, 2, 1025), (9, 10, 1537), (10, 10, 2600), (17, 18, 1111), (31, 32, 1500), (40, 41, 1200),
+                                   (3, 4, 40000)])
+def test_long_rows_with_all_positions_of_a_code_side_by_side(G, P, V, tdt, ddt):
+    """Tiles of all positions in LDS as far as it reaches: target and draft, the target alone, neither; every second code of a wider
+    buffer, and positions padded to more than there are, which are read in place."""
+    B = 5
+    cells = lambda k, v: v.transpose(1, 2).contiguous().transpose(1, 2) if k in ("logits", "draft") else v
+
+    def padded(k, v):
+        if k not in ("logits", "draft"):
+            return v
+        wide = torch.full((v.shape[0], 2 * v.shape[2], v.shape[1] + 3), 9, dtype=v.dtype, device=DEV)
+        wide[:, ::2, 1:1 + v.shape[1]] = v.transpose(1, 2)
+        return wide[:, ::2, 1:1 + v.shape[1]].transpose(1, 2)
+    for place in (cells, padded):
+        check(make(B, G, P, V, tdt, ddt, sigma=0.05, seed=V), place=place)
+        check(make(B, G, P, V, tdt, ddt, probs=True, sigma=0.05, seed=V), lengths=torch.arange(B) * G // 4, probs=True, place=place)
+    c = make(B, G, P, V, sigma=0.05, seed=V)
+    c["draft"] = c["logits"][:, :G].clone()
+    c["draft"][:, G - 1] += torch.randn(B, V, generator=torch.Generator().manual_seed(V))
+    p, q = (np.stack([S.distribution(c[k][b, G - 1].numpy()) for b in range(B)]) for k in ("logits", "draft"))
+    for b in range(B):                                           # an unsure test at the last draft
+        x = int(np.argmin(p[b] / q[b]))
+        c["tokens"][b, G - 1] = x
+        c["u_accept"][b, G - 1] = p[b, x] / q[b, x] * (1 - 1e-12 if b % 2 else 1 + 1e-12)
+    a, _ = check(c, place=cells)
+    assert a.tolist() == [G if b % 2 else G - 1 for b in range(B)]
