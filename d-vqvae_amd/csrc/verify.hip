@@ -463,18 +463,25 @@ static __device__ __noinline__ double verify_row_sum64(Exp ex, const T* row, int
     return all;
 }
 
-// Copies elements that lie side by side into LDS; the whole workgroup.
+// Copies elements that lie side by side into LDS; the whole workgroup.  Four loads of a thread are under way at a time (one
+// behind the end reads the last 16 bytes once more: left out, it would make the others wait).
 template <typename T>
 __device__ __forceinline__ void verify_copy(const T* from, int total, T* to) {
-    constexpr int N = 16 / sizeof(T);
-    int i = threadIdx.x * N;
-#pragma unroll 4
-    for (; i + N <= total; i += blockDim.x * N) {
-        u32x4 v;
-        __builtin_memcpy(&v, from + i, 16);
-        *reinterpret_cast<u32x4*>(to + i) = v;
+    constexpr int N = 16 / sizeof(T), U = 4;
+    const int step = blockDim.x * N, whole = total / N * N;
+    for (int i0 = 0; i0 < whole; i0 += U * step) {
+        u32x4 v[U];
+        int at[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            at[k] = i0 + k * step + (int)threadIdx.x * N;
+            __builtin_memcpy(&v[k], from + (at[k] < whole ? at[k] : whole - N), 16);
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+            if (at[k] < whole) *reinterpret_cast<u32x4*>(to + at[k]) = v[k];
     }
-    for (; i < total; ++i) to[i] = from[i];                      // (at most one thread has a rest)
+    for (int i = whole + (int)threadIdx.x; i < total; i += blockDim.x) to[i] = from[i];
 }
 
 // ------------------------------------------------------------------------------------------------ rows of up to 1024 codes
@@ -937,7 +944,7 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_stats_kernel(VerifyAr
     }
 }
 
-// Codes that do not lie side by side: the test sums of one tile of all positions, one wave per position in turns.  The
+// Codes that do not lie side by side: the test sums of `per` tiles of all positions, one wave per tile and position in turns.  The
 // positions of a code share cache lines; where they are all that lies between a code and the next (the prior's forward), the
 // tile of all positions is one piece of memory and is copied into LDS (t_staged, d_staged) instead of fetched anew by every
 // position.
@@ -952,27 +959,33 @@ __device__ __forceinline__ Sum verify_cell_sum(const T* row, int64_t sv, const T
     return sum_wave(s);
 }
 template <typename T, typename D, bool PROBS>
-__global__ __launch_bounds__(kCellWaves * 64) void verify_cells_kernel(VerifyArgs a, char* ws, int tiles, bool t_staged, bool d_staged) {
+__global__ __launch_bounds__(kCellWaves * 64) void verify_cells_kernel(VerifyArgs a, char* ws, int per, int groups, bool t_staged, bool d_staged) {
     extern __shared__ __align__(16) char block[];
     const int wave = verify_wave(), lane = threadIdx.x & 63;
-    const int tile = (int)((int64_t)blockIdx.x % tiles);
-    const int64_t b = (int64_t)blockIdx.x / tiles;
-    const int codes = a.V - tile * kTile < kTile ? a.V - tile * kTile : kTile;
-    const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)tile * kTile * a.lv;
-    const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)tile * kTile * a.dv;
+    const int tiles = (a.V + kTile - 1) / kTile, first = (int)((int64_t)blockIdx.x % groups) * per;
+    const int64_t b = (int64_t)blockIdx.x / groups;
+    const int codes = a.V - first * kTile < per * kTile ? a.V - first * kTile : per * kTile;
+    const T* lr = reinterpret_cast<const T*>(a.logits) + b * a.lb + (int64_t)first * kTile * a.lv;
+    const D* dr = reinterpret_cast<const D*>(a.draft) + b * a.db + (int64_t)first * kTile * a.dv;
     T* const t = reinterpret_cast<T*>(block);
-    D* const d = reinterpret_cast<D*>(block + (t_staged ? kTile * a.P * sizeof(T) : 0));
+    D* const d = reinterpret_cast<D*>(block + (t_staged ? per * kTile * a.P * sizeof(T) : 0));
     if (t_staged) verify_copy(lr, codes * a.P, t);
     if (d_staged) verify_copy(dr, codes * a.G, d);
     const int n = verify_length(a, b);
     const SplitRow row = split_row(ws, a, b);
     __syncthreads();
-    for (int g = wave; g < a.P && g <= n; g += kCellWaves) {
-        const Sum p = verify_cell_sum(lr + (int64_t)g * a.lp, a.lv, t_staged ? t + g : nullptr, codes, lane);
-        if (lane == 0) row.p[(int64_t)g * tiles + tile] = p;
-        if (!PROBS && g < n) {
-            const Sum q = verify_cell_sum(dr + (int64_t)g * a.dg, a.dv, d_staged ? d + g : nullptr, codes, lane);
-            if (lane == 0) row.q[(int64_t)g * tiles + tile] = q;
+    const int rows = PROBS ? a.P : a.P + a.G;
+    for (int i = wave; i < per * rows; i += kCellWaves) {
+        const int k = i / rows, g = i % rows, off = k * kTile, rest = codes - off < kTile ? codes - off : kTile;
+        if (rest <= 0) break;
+        if (g < a.P) {
+            if (g > n) continue;
+            const Sum p = verify_cell_sum(lr + (int64_t)g * a.lp + off * a.lv, a.lv, t_staged ? t + (off * a.P + g) : nullptr, rest, lane);
+            if (lane == 0) row.p[(int64_t)g * tiles + first + k] = p;
+        } else if (!PROBS && g - a.P < n) {
+            const int m = g - a.P;
+            const Sum q = verify_cell_sum(dr + (int64_t)m * a.dg + off * a.dv, a.dv, d_staged ? d + (off * a.G + m) : nullptr, rest, lane);
+            if (lane == 0) row.q[(int64_t)m * tiles + first + k] = q;
         }
     }
 }
@@ -1150,13 +1163,14 @@ static int verify_launch(const VerifyArgs& a, char* ws, hipStream_t st) {
         const dim3 blk(kSplitWaves * 64);
         if (a.unit) hipLaunchKernelGGL((verify_stats_kernel<T, D, PROBS>), dim3((unsigned)(a.B * a.P * chunks)), blk, 0, st, a, ws, chunks);
         else {
+            const int rows = PROBS ? a.P : a.P + a.G, each = rows < kCellWaves ? kCellWaves / rows : 1, groups = (tiles + each - 1) / each;
             size_t lds = 0;
-            const size_t t_bytes = kTile * sizeof(T) * a.P, d_bytes = kTile * sizeof(D) * a.G;
+            const size_t t_bytes = each * kTile * sizeof(T) * a.P, d_bytes = each * kTile * sizeof(D) * a.G;
             const bool t_staged = a.P > 1 && a.lp == 1 && a.lv == a.P && t_bytes <= kCellBytes;
             if (t_staged) lds += t_bytes;
             const bool d_staged = !PROBS && a.G > 1 && a.dg == 1 && a.dv == a.G && lds + d_bytes <= kCellBytes;
             if (d_staged) lds += d_bytes;
-            hipLaunchKernelGGL((verify_cells_kernel<T, D, PROBS>), dim3((unsigned)(a.B * tiles)), dim3(kCellWaves * 64), lds, st, a, ws, tiles,
+            hipLaunchKernelGGL((verify_cells_kernel<T, D, PROBS>), dim3((unsigned)(a.B * groups)), dim3(kCellWaves * 64), lds, st, a, ws, each, groups,
                                t_staged, d_staged);
         }
         hipLaunchKernelGGL((verify_pass_kernel<T, D, PROBS>), dim3((unsigned)(a.B * per)), blk, 0, st, a, ws, chunks, per);
