@@ -1123,17 +1123,23 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_draw_kernel(VerifyArg
     verify_finish<T, D, PROBS>(ex, a, b, at_draw, lr, dr, w, a.unit, sp, sq, tile_a, tile_c, tile_near, tiles, lds);
 }
 
-// Rows that the workgroup-per-row form takes; fewer, or codes that do not lie side by side, are cut among workgroups.
-constexpr int kRowsMin = 192;
+// Long rows whose codes lie side by side have a workgroup each, and are cut among workgroups -- three launches -- only where they
+// are few and long.  us of a call, cut / one workgroup of 8 waves, 4 drafts, fp32 logits: 8 rows x 4096 20 / 17, x 8192 20 / 21, x 40000 21 /
+// 50; 64 rows x 8192 22 / 21, x 16384 25 / 29; 128 x 16384 36 / 31, x 40000 63 / 66; 190 x 16384 42 / 33, x 40000 85 / 72.
+constexpr int kRowsMin = 128, kRowsTo = 8192;
+// Its waves: eight for long rows as long as there is a CU for each, else four, which leave less of the card idle when a row stops.
+// Eight / four, 4 drafts, fp32 logits: 256 rows x 30000 62 / 71 us, x 8192 25.0 / 25.5, x 4096 20 / 19, x 1100 18 / 16; 500 rows x 30000
+// 105 / 108, x 8192 40 / 37, x 1100 22 / 18; 760 rows x 8192 60 / 52.
+constexpr int kRows8 = 256, kRows8From = 4096;
 // Short rows, positions at a time: all at once for few rows, so that the call takes one position's time; with more rows a wave
 // behind the first rejection is work in vain.  So many waves in all (us with 1024 / 2048 / 4096 / 16384, logits side by side: 1050 rows of
 // 8 x 223 bf16 21 / 16 / 15 / 20, 719 of 13 x 1005 fp32 19 / 18 / 20 / 31, 300 of 12 x 300 14 / 14 / 17 / 17, 4096 of 9 x 512 26 / 26 / 27 / 35), and
-// of a row whose block is staged one for so many bytes at least (2000 rows of 7 x 1000, codes of all positions side by side: 3500 / 4608 /
-// 6144 bytes 66 / 67 / 46; 4096 of 9 x 512 53 / 41 / 38).
+// of a row whose block is staged one for so many bytes at least (2000 rows of 7 x 1000, codes of all positions side by side: 4608 /
+// 6144 / 20000 bytes 65 / 44 / 49; 4096 of 9 x 512 39 / 35 / 43).
 constexpr int kShortWaves = 2048;
 constexpr int kShortStage = 6144;
 constexpr size_t kCellBytes = 65536;                         // LDS of a tile of all positions
-static bool verify_split(int64_t B, int V, bool unit) { return V > 2 * kTile && (!unit || B < kRowsMin); }
+static bool verify_split(int64_t B, int V, bool unit) { return V > 2 * kTile && (!unit || (B < kRowsMin && V > kRowsTo)); }
 
 template <typename T, typename D, bool PROBS>
 static int verify_launch(const VerifyArgs& a, char* ws, hipStream_t st) {
@@ -1178,8 +1184,8 @@ static int verify_launch(const VerifyArgs& a, char* ws, hipStream_t st) {
         return check_launch("prior_verify");
     }
     const size_t lds = (size_t)tiles * 17;
-    if (a.B >= 768) hipLaunchKernelGGL((verify_row_kernel<4, T, D, PROBS>), grid, dim3(256), lds, st, a);
-    else hipLaunchKernelGGL((verify_row_kernel<8, T, D, PROBS>), grid, dim3(512), lds, st, a);
+    if (a.B <= kRows8 && a.V > kRows8From) hipLaunchKernelGGL((verify_row_kernel<8, T, D, PROBS>), grid, dim3(512), lds, st, a);
+    else hipLaunchKernelGGL((verify_row_kernel<4, T, D, PROBS>), grid, dim3(256), lds, st, a);
     return check_launch("prior_verify");
 }
 

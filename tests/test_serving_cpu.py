@@ -117,14 +117,15 @@ def test_verify_refusals(bad):
 def test_verify_refuses_a_workspace_too_small():
     """Long rows whose codes lie apart, and few long rows, need one."""
     lib = _lib.load()
-    for kw in (dict(V=5000, logits_v=9, draft_v=1), dict(V=5000, logits_v=1, draft_v=1)):
+    for kw in (dict(V=5000, logits_v=9, draft_v=1), dict(V=50000, logits_v=1, draft_v=1)):
         a = _verify_args(**kw)
         need = lib.dvq_prior_verify_workspace_bytes(ctypes.byref(a))
         assert need > 0
         for ws, size in ((None, need), (16, need - 1), (24, need)):
             assert lib.dvq_prior_verify(ctypes.byref(a), ws, size, None) == -1
     assert lib.dvq_prior_verify_workspace_bytes(ctypes.byref(_verify_args(V=1000, logits_v=1, draft_v=1))) == 0
-    assert lib.dvq_prior_verify_workspace_bytes(ctypes.byref(_verify_args(V=5000, logits_v=1, draft_v=1, B=5000))) == 0
+    assert lib.dvq_prior_verify_workspace_bytes(ctypes.byref(_verify_args(V=5000, logits_v=1, draft_v=1))) == 0
+    assert lib.dvq_prior_verify_workspace_bytes(ctypes.byref(_verify_args(V=50000, logits_v=1, draft_v=1, B=5000))) == 0
 
 
 def test_empty_calls_return_without_a_launch():
@@ -160,5 +161,5 @@ def test_sizes_that_no_launch_holds_are_refused():
     for bad in (dict(M=1 << 26, N=1 << 10, ldy=1 << 10), dict(M=(1 << 30) + 1), dict(N=(1 << 30) + 1, ldy=1 << 31), dict(N=1 << 28, ldy=1 << 28),
                 dict(M=100, N=1 << 26, ldy=1 << 26, ldw=17)):
         assert _product(lib, **bad) == -1 and lib.dvq_last_error()
-    for bad in (dict(B=1 << 26, V=8), dict(B=1 << 24, V=5000, logits_v=1, draft_v=1), dict(B=1 << 20, V=1 << 20, logits_v=9, draft_v=9)):
+    for bad in (dict(B=1 << 26, V=8), dict(B=1 << 24, V=5000, logits_v=1, draft_v=1), dict(B=1 << 24, V=5000, logits_v=4, draft_v=4), dict(B=1 << 20, V=1 << 20, logits_v=9, draft_v=9)):
         assert lib.dvq_prior_verify(ctypes.byref(_verify_args(**bad)), 16, 1 << 60, None) == -1 and b"too large" in lib.dvq_last_error()
