@@ -1127,10 +1127,11 @@ __global__ __launch_bounds__(kSplitWaves * 64) void verify_draw_kernel(VerifyArg
 // are few and long.  us of a call, cut / one workgroup of 8 waves, 4 drafts, fp32 logits: 8 rows x 4096 20 / 17, x 8192 20 / 21, x 40000 21 /
 // 50; 64 rows x 8192 22 / 21, x 16384 25 / 29; 128 x 16384 36 / 31, x 40000 63 / 66; 190 x 16384 42 / 33, x 40000 85 / 72.
 constexpr int kRowsMin = 128, kRowsTo = 8192;
-// Its waves: eight for long rows as long as there is a CU for each, else four, which leave less of the card idle when a row stops.
-// Eight / four, 4 drafts, fp32 logits: 256 rows x 30000 62 / 71 us, x 8192 25.0 / 25.5, x 4096 20 / 19, x 1100 18 / 16; 500 rows x 30000
-// 105 / 108, x 8192 40 / 37, x 1100 22 / 18; 760 rows x 8192 60 / 52.
-constexpr int kRows8 = 256, kRows8From = 4096;
+// Its waves: eight for long rows as long as there is a CU for each, two for many rows of a few tiles, else four: more leave more of
+// the card idle when a row stops.  us of eight / four / two, 4 drafts, fp32 logits: 256 rows x 30000 62 / 71 / -, x 8192 25.0 / 25.5 / -,
+// x 4096 20 / 19 / -; 500 rows x 8192 40 / 37 / -, x 1100 22 / 18 / 21; 700 x 4096 - / 31.4 / 31.5; 1000 x 4096 - / 40 / 37, x 8192
+// - / 65 / 66; 4096 x 1100 - / 84 / 61, x 4096 - / 121 / 114, x 8192 - / 197 / 204.
+constexpr int kRows8 = 256, kRows2 = 512, kRowsShort = 4096;
 // Short rows, positions at a time: all at once for few rows, so that the call takes one position's time; with more rows a wave
 // behind the first rejection is work in vain.  So many waves in all (us with 1024 / 2048 / 4096 / 16384, logits side by side: 1050 rows of
 // 8 x 223 bf16 21 / 16 / 15 / 20, 719 of 13 x 1005 fp32 19 / 18 / 20 / 31, 300 of 12 x 300 14 / 14 / 17 / 17, 4096 of 9 x 512 26 / 26 / 27 / 35), and
@@ -1184,7 +1185,8 @@ static int verify_launch(const VerifyArgs& a, char* ws, hipStream_t st) {
         return check_launch("prior_verify");
     }
     const size_t lds = (size_t)tiles * 17;
-    if (a.B <= kRows8 && a.V > kRows8From) hipLaunchKernelGGL((verify_row_kernel<8, T, D, PROBS>), grid, dim3(512), lds, st, a);
+    if (a.B <= kRows8 && a.V > kRowsShort) hipLaunchKernelGGL((verify_row_kernel<8, T, D, PROBS>), grid, dim3(512), lds, st, a);
+    else if (a.B > kRows2 && a.V <= kRowsShort) hipLaunchKernelGGL((verify_row_kernel<2, T, D, PROBS>), grid, dim3(128), lds, st, a);
     else hipLaunchKernelGGL((verify_row_kernel<4, T, D, PROBS>), grid, dim3(256), lds, st, a);
     return check_launch("prior_verify");
 }
