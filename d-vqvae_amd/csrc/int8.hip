@@ -17,6 +17,11 @@ constexpr int kInt8MaxBatch = 8;
 // Tiles against split, int8 operands in place: 64 tiles (128 x 2048 x 2048) 9.1 / 8.4 us, 32 (100 x 1000 x 512) 6.0 / 4.9;
 // 80 tiles (128 x 2560 x 1024) 6.8 / 8.7, 96 (200 x 1536 x 4096) 13.8 / 21.5.
 constexpr int kInt8SplitTo = 64;
+// Floats are quantised by every workgroup of 16 x 16 outputs for itself -- one launch, no workspace, the rows read once per 16
+// channels -- as long as the workgroups fit the chip in a round: two launches / one, us of a call, fp32: 64 x 4096 -> 1024 (256 workgroups)
+// 22 / 15, 128 x 2560 -> 1024 (512) 17 / 17, 256 x 2560 -> 1024 (1024) 17 / 29; up to 1024 features, where four fit a CU, 256 x 1024 ->
+// 1024 16 / 14.
+constexpr int kInt8OneLaunch = 256, kInt8OneLaunchShort = 1024;
 struct Int8Prepare {
     const void* x[kInt8MaxBatch];
     const int8_t* W[kInt8MaxBatch];
@@ -206,12 +211,12 @@ __global__ __launch_bounds__(512) void int8_rows16_kernel(Int8Batch p, int64_t l
     __shared__ unsigned tops[8][16];
     __shared__ float sc[16];
     __shared__ __align__(16) int red[8 * 256];
-    const int bz = blockIdx.y, n0 = (int)blockIdx.x * 16;
+    const int bz = blockIdx.y, n0 = (int)blockIdx.x * 16, m0 = (int)blockIdx.z * 16;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int r = lane & 15, kl = 64 * wave + 16 * (lane >> 4);
     const int wr = n0 + r < N ? n0 + r : N - 1;
     const int8_t* w = p.W[bz] + (int64_t)wr * ldw;
-    const T* x = reinterpret_cast<const T*>(p.x[bz]) + (int64_t)(r < M ? r : M - 1) * ldx;
+    const T* x = reinterpret_cast<const T*>(p.x[bz]) + (int64_t)(m0 + r < M ? m0 + r : M - 1) * ldx;
     const bool wide = (reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T))) == 0;
     i32x4 wf[STEPS];
     f32x4 v[STEPS][4];
@@ -263,16 +268,16 @@ __global__ __launch_bounds__(512) void int8_rows16_kernel(Int8Batch p, int64_t l
     __syncthreads();
     if (tid >= 256) return;
     const int m = tid >> 4, n = tid & 15;
-    if (m >= M || n0 + n >= N) return;
+    if (m0 + m >= M || n0 + n >= N) return;
     int sum = 0;
 #pragma unroll
     for (int g = 0; g < 8; ++g) sum += red[g * 256 + (m + 16 * (n >> 2)) * 4 + (n & 3)];
-    int8_store(reinterpret_cast<Y*>(p.y[bz]) + m * ldy + n0 + n,
+    int8_store(reinterpret_cast<Y*>(p.y[bz]) + (int64_t)(m0 + m) * ldy + n0 + n,
                int8_scale(sum, sc[m], p.ws[bz][n0 + n], p.b[bz] ? p.b[bz][n0 + n] : 0.f, relu));
 }
 template <typename T, typename Y>
 static int int8_rows16(const Int8Batch& p, int n_batch, int64_t ldx, int64_t ldw, int M, int K, int N, int relu, int64_t ldy, hipStream_t st) {
-    const dim3 grid((unsigned)((N + 15) / 16), (unsigned)n_batch), blk(512);
+    const dim3 grid((unsigned)((N + 15) / 16), (unsigned)n_batch, (unsigned)((M + 15) / 16)), blk(512);
     if (K <= 1024) hipLaunchKernelGGL((int8_rows16_kernel<2, T, Y>), grid, blk, 0, st, p, ldx, ldw, M, K, N, relu, ldy);
     else if (K <= 2560) hipLaunchKernelGGL((int8_rows16_kernel<5, T, Y>), grid, blk, 0, st, p, ldx, ldw, M, K, N, relu, ldy);
     else hipLaunchKernelGGL((int8_rows16_kernel<8, T, Y>), grid, blk, 0, st, p, ldx, ldw, M, K, N, relu, ldy);
@@ -532,8 +537,10 @@ static inline int64_t int8_each(int rows, int K) { return rows * int8_ld(K) + (r
 
 using namespace dvq;
 
-// Rows of a float matrix at a time quantised by each workgroup for itself: no workspace, one launch.
-static bool int8_one_launch(int M, int K) { return M <= 16 && K <= kInt8Held; }
+// Rows of a float matrix quantised by each workgroup for itself: no workspace, one launch.
+static bool int8_one_launch(int n_batch, int M, int K, int N) {
+    return K <= kInt8Held && (M <= 16 || tile_count(M, N, 16, n_batch) <= (K <= 1024 ? kInt8OneLaunchShort : kInt8OneLaunch));
+}
 
 extern "C" size_t dvq_linear_int8_workspace_bytes(int n_batch, int M, int K, int N) {
     if (n_batch < 1 || M < 1 || K < 1 || N < 1) return 0;
@@ -577,7 +584,7 @@ extern "C" int dvq_linear_int8_batched(int n_batch, const void* const* x, int x_
     }
     hipStream_t st = as_stream(stream);
     const bool f32 = y_dtype == DVQ_F32;
-    if (!codes && int8_one_launch(M, K)) {
+    if (!codes && int8_one_launch(n_batch, M, K, N)) {
         if (!launch_fits((N + 15) / 16, 512)) return fail(DVQ_EINVAL, "linear_int8: N too large");
         typedef unsigned short u16;
         if (x_dtype == DVQ_F32)

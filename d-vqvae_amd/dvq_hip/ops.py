@@ -420,9 +420,10 @@ def linear_int8(x, W: torch.Tensor, w_scale: torch.Tensor, b: Optional[torch.Ten
     if M == 0 or N == 0:
         return out
     lib = _lib.load()
-    ws, nbytes = _int8_workspace(lib, 1, M, K, N, sx is not None, dev)
-    _launch(lib.dvq_linear_int8, "dvq_linear_int8", dev, x.data_ptr(), _CODES[x.dtype], None if sx is None else sx.data_ptr(), ldx,
-            W.data_ptr(), w_scale.data_ptr(), ldw, None if b is None else b.data_ptr(), M, K, N, int(relu), out.data_ptr(),
+    xp, wp = x.data_ptr(), W.data_ptr()
+    ws, nbytes = _int8_workspace(lib, 1, M, K, N, sx is not None, (xp | wp | ldx | ldw | K) % 16 == 0, dev)
+    _launch(lib.dvq_linear_int8, "dvq_linear_int8", dev, xp, _CODES[x.dtype], None if sx is None else sx.data_ptr(), ldx,
+            wp, w_scale.data_ptr(), ldw, None if b is None else b.data_ptr(), M, K, N, int(relu), out.data_ptr(),
             _CODES[out.dtype], ldy, None if ws is None else ws.data_ptr(), nbytes)
     return out
 
@@ -462,10 +463,11 @@ def linear_int8_batched(xs, Ws, w_scales, bs, relu: bool = False, out_dtype: tor
     if M == 0 or N == 0:
         return outs
     lib = _lib.load()
-    ws, nbytes = _int8_workspace(lib, n, M, K, N, pairs, dev)
     step, base = M * N * y.element_size(), y.data_ptr()
+    reads = [x.data_ptr() for x in feats] + [W.data_ptr() for W in Ws]
+    ws, nbytes = _int8_workspace(lib, n, M, K, N, pairs, pairs and (ldx | ldw | K) % 16 == 0 and all(p % 16 == 0 for p in reads), dev)
     # the six lists of n addresses behind one another
-    lists = (ctypes.c_void_p * (6 * n))(*[x.data_ptr() for x in feats], *[W.data_ptr() for W in Ws], *[s.data_ptr() for s in w_scales],
+    lists = (ctypes.c_void_p * (6 * n))(*reads, *[s.data_ptr() for s in w_scales],
                                         *[None if b is None else b.data_ptr() for b in bs], *range(base, base + n * step, step),
                                         *([s.data_ptr() for _, s in xs] if pairs else [None] * n))
     at = ctypes.addressof(lists)
@@ -493,8 +495,12 @@ def _int8_out(M, N, dtype, dev, what):
     return torch.empty((M, N), dtype=dtype, device=dev)
 
 
-def _int8_workspace(lib, n, M, K, N, pairs, dev):
-    if M <= 16 and K <= 4096 and not pairs:              # few rows of floats: one launch that needs none
+def _int8_workspace(lib, n, M, K, N, pairs, aligned, dev):
+    """The workspace of n products and its size; none where dvq_linear_int8 touches none."""
+    if pairs:
+        if aligned or n * ((M + 63) // 64) * ((N + 63) // 64) <= 64:
+            return None, 0
+    elif K <= 4096 and (M <= 16 or n * ((M + 15) // 16) * ((N + 15) // 16) <= (1024 if K <= 1024 else 256)):
         return None, 0
     nbytes = lib.dvq_linear_int8_workspace_bytes(n, M, K, N)
     return torch.empty(nbytes, dtype=torch.uint8, device=dev), nbytes

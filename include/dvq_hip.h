@@ -375,8 +375,9 @@ int dvq_prior_uniforms(int64_t first_id, int64_t n, int n_cells, uint64_t seed, 
  *   K < 2^17.  act: relu keeps a NaN.  y must not overlap x.
  * dvq_linear_int8_batched: products of ONE shape in the same launches; x, xs, W, ws, b, y: host arrays of n_batch (1..8) device
  *   pointers.
- *   workspace: dvq_linear_int8_workspace_bytes() bytes (n_batch = 1 for a single product), 16-byte aligned; not touched (may be NULL) for M <= 16 rows of floats
- *   with K <= 4096, and for DVQ_I8 with rows of x and W at multiples of 16 bytes and K % 16 == 0. */
+ *   workspace: dvq_linear_int8_workspace_bytes() bytes (n_batch = 1 for a single product), 16-byte aligned; not touched (may be
+ *   NULL) for floats with K <= 4096 and M <= 16 or at most 256 (K <= 1024: 1024) blocks of 16 x 16 outputs in all products
+ *   together, and for DVQ_I8 with rows of x and W at multiples of 16 bytes and K % 16 == 0, or at most 64 blocks of 64 x 64 outputs. */
 int dvq_int8_quantize_rows(const void* x, int dtype, int64_t ldx, int M, int K, void* codes, int64_t ldc, float* scale, void* stream);
 size_t dvq_linear_int8_workspace_bytes(int n_batch, int M, int K, int N);
 int dvq_linear_int8(const void* x, int x_dtype, const float* xs, int64_t ldx, const void* W, const float* ws, int64_t ldw,

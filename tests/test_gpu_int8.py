@@ -321,3 +321,20 @@ def test_single_rows_and_features_of_any_stride_together():
     layers = [one[0].to(DEV)] * 2, [one[1].to(DEV)] * 2, [one[2].to(DEV)] * 2
     for y, x in zip(ops.linear_int8_batched([cols[0], cols[2]], *layers), (cols[0], cols[2])):
         assert torch.equal(y, ops.linear_int8(x.contiguous(), one[0].to(DEV), one[1].to(DEV), one[2].to(DEV)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,K,N", [(17, 4096, 33), (250, 4096, 250), (255, 2571, 241), (257, 2560, 240), (512, 1024, 512), (511, 1009, 497), (528, 1024, 512),
+                                   (1000, 70, 256), (4000, 300, 16), (100, 4097, 40)])
+def test_rows_quantised_by_every_workgroup_and_once_before(M, K, N, dtype):
+    """At, below and above the sizes where a layer of floats is one launch."""
+    x = rows(M, K, dtype, M + N)
+    x[M // 2] = 0
+    x[M - 1, 0] = float("inf")
+    W, t, b = layer(N, K, N)
+    y = ops.linear_int8(x.to(DEV), W.to(DEV), t.to(DEV), b.to(DEV), relu=True)
+    codes, scale = S.int8_codes(x)
+    check_output(y, codes, scale, W, t, b, True)
+    xs = [x.to(DEV), x.to(DEV).flip(0)]
+    for z, want in zip(ops.linear_int8_batched(xs, [W.to(DEV)] * 2, [t.to(DEV)] * 2, [b.to(DEV)] * 2, relu=True), (y, y.flip(0))):
+        assert torch.equal(z.nan_to_num(7.0), want.nan_to_num(7.0)) and torch.equal(z.isnan(), want.isnan())

@@ -72,8 +72,8 @@ def test_quantize_refusals(bad):
 
 @pytest.mark.parametrize("bad", [dict(n=0), dict(n=9), dict(K=0), dict(K=1 << 17), dict(M=-1), dict(N=0), dict(x_dtype=3), dict(y_dtype=2), dict(ldy=3),
                                  dict(ldx=-1), dict(ldw=-1), dict(ptr=None), dict(x_dtype=2, xs=False), dict(M=0x7FFFFFFF),
-                                 dict(M=20, ws=None), dict(M=20, ws=8), dict(M=20, nbytes=20 * 64 + 80 + 4 * 64 - 1), dict(K=4097, ws=None),
-                                 dict(n=2, M=20, nbytes=20 * 64 + 80 + 4 * 64)])
+                                 dict(M=20000, ws=None), dict(M=20000, ws=8), dict(M=20000, nbytes=20000 * 64 + 80000 + 4 * 64 - 1), dict(K=4097, ws=None),
+                                 dict(n=2, M=20000, nbytes=20000 * 64 + 80000 + 4 * 64)])
 def test_product_refusals(bad):
     lib = _lib.load()
     assert _product(lib, **bad) == -1 and lib.dvq_last_error()
@@ -84,7 +84,7 @@ def test_single_product_refusals():
     call = lambda x=16, W=16, y=16, x_dtype=0, xs=16, N=4, ws=16, M=4: lib.dvq_linear_int8(x, x_dtype, xs, 16, W, 16, 16, None, M, 16, N, 0, y, 0, 4,
                                                                                         ws, 1 << 40, None)
     assert call(M=0) == 0
-    for bad in (dict(x=None), dict(W=None), dict(y=None), dict(x_dtype=2, xs=None), dict(N=0), dict(M=20, ws=None)):
+    for bad in (dict(x=None), dict(W=None), dict(y=None), dict(x_dtype=2, xs=None), dict(N=0), dict(M=20000, ws=None)):
         assert call(**bad) == -1 and lib.dvq_last_error()
 
 
