@@ -557,7 +557,7 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(TILES == 1
                 }
             } else if (!sum_ok(p)) st = VERIFY_BAD;
         }
-        int stop = st == VERIFY_KEEP ? waves : 0;                // first wave of this round whose position stops the row
+        int stop = st == VERIFY_KEEP ? waves : 0;                // first wave of these whose position stops the row
         if (waves > 1) {
             __syncthreads();
             if (lane == 0) state[wave] = st;

@@ -36,7 +36,7 @@ extern "C" {
 #define DVQ_BF16 1
 #define DVQ_I8 2      /* 8-bit codes with a scale per row (dvq_linear_int8) */
 
-#define DVQ_VERSION 114   /* major*10000 + minor*100 + patch */
+#define DVQ_VERSION 113   /* major*10000 + minor*100 + patch */
 
 int dvq_version(void);
 const char* dvq_last_error(void);
