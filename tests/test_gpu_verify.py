@@ -439,3 +439,22 @@ def test_long_rows_with_all_positions_of_a_code_side_by_side(G, P, V, tdt, ddt):
         c["u_accept"][b, G - 1] = p[b, x] / q[b, x] * (1 - 1e-12 if b % 2 else 1 + 1e-12)
     a, _ = check(c, place=cells)
     assert a.tolist() == [G if b % 2 else G - 1 for b in range(B)]
+
+
+@pytest.mark.parametrize("V", [600, 1500, 3000, 20000])
+@pytest.mark.parametrize("layout", ["rows", "cells"])
+@pytest.mark.parametrize("B", [4, 600])
+def test_a_nan_among_masked_codes(B, V, layout):
+    """Whole tiles of -inf with one NaN in them, in target and draft: a distribution that is none, wherever the NaN lies."""
+    if B * V > 2000000:
+        B = 64
+    c = make(B, 2, 3, V, sigma=0.1, seed=V)
+    lo, hi = (0, 512) if V < 1024 else (512, min(V, 1536))
+    for b in range(0, B, 2):
+        which = "logits" if b % 4 else "draft"
+        g = b // 4 % c[which].shape[1]
+        c[which][b, g, lo:hi] = -INF
+        c[which][b, g, lo + (b * 37) % (hi - lo)] = float("nan")
+    place = (lambda k, v: v) if layout == "rows" else lambda k, v: v.transpose(1, 2).contiguous().transpose(1, 2) if k in ("logits", "draft") else v
+    _, n = check(c, place=place)
+    assert (n == -1).any() and (n >= 0).any()
