@@ -410,7 +410,7 @@ def linear_int8(x, W: torch.Tensor, w_scale: torch.Tensor, b: Optional[torch.Ten
     if sx is not None:
         _vector(sx, M, dev, what, "the scale of x")
     if out is None:
-        out = _int8_out(M, N, out_dtype, dev, what)
+        out = _int8_out(x, M, N, out_dtype, what)
         ldy = N
     else:
         ldy = _rows(out, _FLOATS, dev, what, "out")
@@ -459,7 +459,7 @@ def linear_int8_batched(xs, Ws, w_scales, bs, relu: bool = False, out_dtype: tor
         for _, s in xs:
             _vector(s, M, dev, what, "the scale of x")
     # (n outputs cut from one buffer)
-    y = _int8_out(n * M, N, out_dtype, dev, what)
+    y = _int8_out(first, n * M, N, out_dtype, what)
     outs = list(y.view(n, M, N).unbind(0)) if M > 0 else [y] * n
     if M == 0 or N == 0:
         return outs
@@ -489,10 +489,10 @@ def _int8_layer(W, w_scale, b, K, dev, what):
     return ldw, N
 
 
-def _int8_out(M, N, dtype, dev, what):
+def _int8_out(like, M, N, dtype, what):
     if dtype not in _FLOATS:
         raise RuntimeError(f"{what}: output of float32 or bfloat16, not {dtype}")
-    return torch.empty((M, N), dtype=dtype, device=dev)
+    return like.new_empty((M, N), dtype=dtype)
 
 
 def _int8_workspace(lib, n, M, K, N, pairs, aligned, dev):
@@ -749,12 +749,13 @@ def prior_verify(logits: torch.Tensor, draft: torch.Tensor, tokens: torch.Tensor
                                "None" if t is None else f"{t.dtype} {tuple(t.shape)}" for t in (logits, draft, tokens, u_accept, u_draw, lengths)))
     if not logits.is_cuda:
         raise RuntimeError("dvq_hip kernels need tensors on a HIP device (got a CPU tensor); there is no CPU fallback")
-    if draft.device != dev or tokens.device != dev or u_accept.device != dev or u_draw.device != dev or (
-            lengths is not None and lengths.device != dev):
+    index = dev.index
+    if draft.get_device() != index or tokens.get_device() != index or u_accept.get_device() != index or u_draw.get_device() != index or (
+            lengths is not None and lengths.get_device() != index):
         raise RuntimeError(f"prior_verify: all tensors must be on {dev}, where the logits are")
     if (P != G and P != G + 1) or P < 1 or V < 1:
         raise RuntimeError(f"prior_verify: {P} positions of logits for {G} drafted codes (as many, or one more) of {V}")
-    accepted, nxt = torch.empty((2, B), dtype=torch.int64, device=dev).unbind(0)
+    accepted, nxt = tokens.new_empty((2, B)).unbind(0)
     if B == 0:
         return accepted, nxt
     a = _VERIFY_ARGS.pack(logits.data_ptr(), *logits.stride(), draft.data_ptr(), *draft.stride(), tokens.data_ptr(), *tokens.stride(),
