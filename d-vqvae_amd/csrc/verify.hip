@@ -759,9 +759,9 @@ __device__ __forceinline__ void verify_sums(Ring<T, D, Q>& ring, const Share& w,
     if (Q) ring.ty.load(nd + (nboth ? V - kTile + 8 * lane : 8 * lane));
 }
 
-// Codes side by side (a.unit).  Bound by the vector instructions (exponentials in the tests, 64-bit ones in the draw) and by rows that
-// stop at different positions: what a CU's rows need in all differs by a factor of two.  1024 rows of 4 drafts x 16381 bf16 84 us
-// (41 of memory), 1000 of up to 5 x 8192 46 us (14).
+// Codes side by side (a.unit).  The tests run at 86 % of a copy's rate (1024 rows x 16381 bf16, all drafts kept, no draw: 60 us for 268 MB);
+// the draw, 64-bit exponentials of the whole row once more, takes 45 us where every row ends in one, 24 without a residual.  With rows
+// that stop at different positions 84 us (41 of memory); 1000 of up to 5 x 8192 46 us (14).
 template <int WAVES, typename T, typename D, bool PROBS>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(4))) void verify_row_kernel(VerifyArgs a) {
     extern __shared__ double tile_a[];                           // per tile of the row: a, c, near
