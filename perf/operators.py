@@ -5,7 +5,6 @@ distribution (`dvq_hip.ops.prior_verify`).
 `run` computes them in elementary torch operations, or through the framework's entry points where `own` is true; `exact`
 says in 64 bits what the outputs are.
 """
-import importlib
 import math
 import os
 import sys
@@ -19,11 +18,11 @@ TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16}
 
 
 def _ops():
-    """The framework's entry points, imported once as a user's program does."""
-    if "dvq_hip.ops" not in sys.modules:
-        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "d-vqvae_amd"))
-        importlib.import_module("dvq_hip.ops")
-    return sys.modules["dvq_hip.ops"]
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "d-vqvae_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    from dvq_hip import ops
+    return ops
 
 
 def listed():
@@ -210,11 +209,9 @@ def work(case):
     a = math.erfc(case["sigma"] / math.sqrt(8.0))
     tests = [sum(a ** g for g in range(n)) for n in (range(G + 1) if case["ragged"] else [G])]
     ends = [a ** n if n < P else 0.0 for n in (range(G + 1) if case["ragged"] else [G])]
-    lost = [1.0 - a ** n for n in (range(G + 1) if case["ragged"] else [G])]
-    tests, ends, lost = (sum(v) / len(v) for v in (tests, ends, lost))
-    # Of a draft given as probabilities a test needs the one of its code, and only a rejection the whole row.
-    dread = V * size * tests if case["draft"] == "logits" else 4 * tests + 4 * V * lost
-    read = V * size * (tests + ends) + dread + tests * 16 + 8
+    tests, ends = sum(tests) / len(tests), sum(ends) / len(ends)
+    dsize = 4 if case["draft"] == "probs" else size
+    read = tests * V * (size + dsize) + ends * V * size + tests * 16 + 8
     return {"bytes": int(B * (read + 16)), "flops": int(B * V * (tests * 2 + ends) * 4)}
 
 
