@@ -41,11 +41,10 @@ class _HostStagedGather:
     queued on the CURRENT stream right behind the producer, one event after it; wait() blocks the host on that event
     alone (not on the device), runs the collective on the pinned buffers and queues the copy back.
 
-    torch's own gloo path for device tensors stages through a fresh HIGH-PRIORITY pool stream per collective.  On
-    this ROCm stack such a stream, made to wait for an event of a stream that is still busy with the generation
-    step's work (when first seen: the prior's replayed graph beside an encoder on a second stream), sometimes never drains -- reproducible
-    in one process without any process group (tools/gloo_hang_probe.py emu1); the same wait on a normal-priority
-    pool stream (what the RCCL backend uses), or on a high-priority stream that has been used before, completes.
+    torch's own gloo path for device tensors stages through a fresh HIGH-PRIORITY pool stream per collective.  On this
+    ROCm stack such a stream, made to wait for an event of a stream that is still busy with the generation step's work
+    (when first seen: the prior's replayed graph beside an encoder on a second stream), sometimes never drains, without
+    any process group as well; the same wait on a normal-priority pool stream (what the RCCL backend uses) completes.
     Staging on the caller's stream takes that stream out of the picture."""
 
     def __init__(self, t: torch.Tensor, ws: int):
