@@ -55,7 +55,9 @@ def set_compute_dtype(model, dtype):
 def set_head_dtype(model, dtype):
     """Operand type of the MLP heads (`Encoder`, `Decoder`) inside `model` alone: torch.float32, torch.bfloat16, or torch.int8
     -- 8-bit integers with a scale per activation row and per output channel, sums exact, results fp32 (ops.linear_int8) --
-    for every batch size.  The PointNet encoders and the prior keep theirs; set_compute_dtype sets the heads again."""
+    for every batch size.  The PointNet encoders and the prior keep theirs; set_compute_dtype sets the heads again.
+    Eager calls read an 8-bit copy of each weight that is made anew when the weight changes; a recorded graph quantises the weights
+    in every replay, so edits of weights and biases count from the next replay on."""
     if dtype not in (torch.float32, torch.bfloat16, torch.int8):
         raise ValueError("dtype must be torch.float32, torch.bfloat16 or torch.int8")
     for m in model.modules():

@@ -41,15 +41,16 @@ class _Int8Copy:
 
 
 def _int8_weight(layer):
-    """8-bit codes and per-channel scales of an nn.Linear's weight, kept on the layer and refreshed when the weight changes --
-    in place, where recorded graphs read them.  While a graph is recorded nothing is kept: the graph quantises for itself."""
+    """8-bit codes and per-channel scales of an nn.Linear's weight, kept on the layer and refreshed in place when the weight
+    changes.  A graph that is being recorded quantises for itself and reads nothing that is kept: it follows the weight, as it
+    does in fp32 (one more launch, the weight's bytes, a replay)."""
     W = layer.weight.detach()
+    if torch.cuda.is_current_stream_capturing():
+        return ops.quantize_rows(W.float())
     key = (W.data_ptr(), W._version, dvq_hip.weights_epoch())
     kept = layer.__dict__.setdefault("_dvq_int8", _Int8Copy())
     if kept.key != key:
         codes, scale = ops.quantize_rows(W.float())
-        if torch.cuda.is_current_stream_capturing():
-            return codes, scale
         if kept.key is not None and kept.codes.shape == codes.shape and kept.codes.device == codes.device:
             kept.codes.copy_(codes)
             kept.scale.copy_(scale)

@@ -214,3 +214,39 @@ def test_8_bit_heads_in_recorded_graphs():
             second.replay()                                           # reads the copy that the call above refreshed
             assert torch.equal(b, want)
             torch.cuda.synchronize()
+
+
+def test_recorded_graphs_follow_edited_weights_without_an_eager_call():
+    """A graph recorded after an eager call quantises for itself as well: weights and biases that are edited in place or loaded
+    count at the next replay, as they do for heads in fp32."""
+    e = set_head_dtype(head(Encoder, [64, 32], 16, 10), torch.int8)
+    d = set_head_dtype(head(Decoder, [48, 6], 64, 11), torch.int8)
+    twins = [copy.deepcopy(m) for m in (e, d)]
+    x = torch.randn(40, 64, generator=torch.Generator().manual_seed(2)).to(DEV)
+    for m in (e, d, *twins):
+        m(x)                                                          # eager calls first: copies of the weights are kept
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    with torch.no_grad():
+        for m in (e, d):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1]):
+                outs.append(m(x))
+        for step in range(4):
+            for m, t in zip((e, d), twins):
+                if step == 1:
+                    for p, q in zip(m.parameters(), t.parameters()):
+                        p.mul_(1.5)
+                        q.mul_(1.5)
+                if step == 2:
+                    state = {k: v + 0.25 for k, v in t.state_dict().items()}
+                    m.load_state_dict(state)
+                    t.load_state_dict(state)
+                if step == 3:
+                    m(x)                                              # an eager call in between
+            for g in graphs:
+                g.replay()
+            got = [o.clone() for o in outs]
+            for m, t, y in zip((e, d), twins, got):
+                assert torch.equal(y, t(x))
+            torch.cuda.synchronize()
