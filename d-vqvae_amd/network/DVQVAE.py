@@ -31,10 +31,11 @@ def _bf16_weight(layer):
 
 
 class _Int8Copy:
-    """8-bit copy of a layer's weight and the version it was made of; deep copies and pickles carry an empty one."""
+    """8-bit copy of a layer's weight and the version it was made of; deep copies and pickles carry an empty one.  The weight's
+    memory is held with it: as long as the copy stands for that address no other weight can take it."""
 
     def __init__(self):
-        self.key = self.codes = self.scale = None
+        self.key = self.source = self.codes = self.scale = None
 
     def __reduce__(self):
         return _Int8Copy, ()
@@ -57,7 +58,7 @@ def _int8_weight(layer):
         else:
             kept.codes, kept.scale = codes, scale
         torch.cuda.current_stream(W.device).synchronize()        # other streams read them from now on
-        kept.key = key
+        kept.key, kept.source = key, W
     return kept.codes, kept.scale
 
 

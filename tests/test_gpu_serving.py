@@ -250,3 +250,16 @@ def test_recorded_graphs_follow_edited_weights_without_an_eager_call():
             for m, t, y in zip((e, d), twins, got):
                 assert torch.equal(y, t(x))
             torch.cuda.synchronize()
+
+
+def test_a_replaced_weight_at_an_earlier_address_is_quantised_anew():
+    """Replaced twice between two calls, a weight can lie where the first one lay, at the same version."""
+    e = set_head_dtype(head(Encoder, [64, 32], 16, 12), torch.int8)
+    x = torch.randn(5, 64, generator=torch.Generator().manual_seed(3)).to(DEV)
+    for seed in range(12):
+        g = torch.Generator().manual_seed(seed)
+        e.linear_means.weight = torch.nn.Parameter(torch.randn(16, 32, generator=g).to(DEV))
+        if seed % 2:                                                  # (the call comes after every second replacement)
+            fresh = copy.deepcopy(e)
+            assert torch.equal(e(x), fresh(x))
+            del fresh
