@@ -107,7 +107,7 @@ class _PackedTaps:
 
 
 class GatedPixelCNN(dvq_hip.DropsPackedCopies, nn.Module):
-    _packed_defaults = {"_packed_key": lambda: None, "_packed": lambda: None, "_bufs": dict, "_cls": lambda: None}
+    _packed_defaults = {"_packed_key": lambda: None, "_packed": lambda: None, "_bufs": dict, "_cls": lambda: None, "_recorded": list}
 
     def __init__(self, input_dim=256, dim=128, n_layers=15, n_classes=128):
         super().__init__()
@@ -124,6 +124,7 @@ class GatedPixelCNN(dvq_hip.DropsPackedCopies, nn.Module):
         self._bufs = {}
         self.class_row1 = True                 # grid row 1: the taps on grid row 0 per class as well
         self._cls = None                       # per-class constants of the weights (see _class_rows)
+        self._recorded = []                    # what graphs recorded over forward() read
         self.use_graph = True                  # replay generate() as a captured HIP graph
         self.split = 1                         # sub-batches evaluated side by side (own streams and graphs)
         self.split_min_rows = 2048             # ... for batches of at least this many rows
@@ -160,22 +161,34 @@ class GatedPixelCNN(dvq_hip.DropsPackedCopies, nn.Module):
         B, H, W = x.shape
         dev = x.device
         self._prepared_hip()
-        bufs = self._act_buffers(B, H, W, dev, part=("forward", 0))      # own buffers: a recorded generate() graph stays
+        recording = torch.cuda.is_current_stream_capturing()
+        # own buffers: a recorded generate() graph stays; a graph that is being recorded here has some of its own as well, since
+        # a later call may drop the kept ones
+        bufs = self._new_buffers(B, H, W, dev) if recording else self._act_buffers(B, H, W, dev, part=("forward", 0))
         bufs["label"].copy_(label.reshape(-1).to(torch.int64))
         if self._by_class(B):
             self._class_rows((H, W), B >= self.vrow_min_rows)
         out = torch.empty(B, self.output_conv[2].out_channels, H, W, dtype=torch.float32, device=dev)
         self._run_hip(bufs, (H, W), B, None, False, None, forced=x.to(torch.int64).contiguous(), collect=out)
+        if recording:
+            self._recorded.append((self._packed, self._cls, bufs["emb"]))  # the graph reads them by address: they stay
         return out
+
+    def _tables_ready(self, B, H, W, dev):
+        """Whether the packed weights and class tables that _forward_hip reads are made already."""
+        return (self._weights_key() == self._packed_key
+                and (not self._by_class(B) or ((H, W), B >= self.vrow_min_rows, str(dev)) in (self._cls or {})))
 
     @torch.no_grad()
     def verify(self, x, label, draft, u_accept, u_draw, lengths=None, draft_probs=False):
         """Verify drafted grids x (int64 [B,H,W], raster order) against this prior: one forward with x as the history, then
         ops.prior_verify.  draft [B, H*W, input_dim]: the logits (draft_probs: probabilities, as generate(return_probs=True)
         of a drafting prior returns them) the codes were drawn from; u_accept float64 [B, H*W], u_draw float64 [B];
-        lengths int64 [B]: only the first so many cells of a grid are drafts (the rest may hold anything).  Returns (accepted [B], next [B]): the first
-        accepted cells of a grid and the code after them, where there is a cell for it (-1 where not), are distributed as
-        generate()'s."""
+        lengths int64 [B]: only the first so many cells of a grid are drafts (the rest may hold anything).  Returns
+        (accepted [B], next [B]): the first accepted cells of a grid and the code after them, where there is a cell for it
+        (-1 where not), are distributed as generate()'s.
+        It may be recorded into a graph once it has run eagerly (refused before); the graph keeps the packed weights of that
+        time: record it again when the weights have changed."""
         if x.dim() != 3:
             raise RuntimeError(f"GatedPixelCNN.verify: x must be int64 [B,H,W], got {tuple(x.shape)}")
         B, H, W = x.shape
@@ -184,6 +197,9 @@ class GatedPixelCNN(dvq_hip.DropsPackedCopies, nn.Module):
             return empty, empty.clone()
         if draft.dim() != 3 or draft.shape[:2] != (B, H * W):
             raise RuntimeError(f"GatedPixelCNN.verify: draft must be [{B},{H * W},codes], got {tuple(draft.shape)}")
+        if x.is_cuda and torch.cuda.is_current_stream_capturing() and not self.training and not self._tables_ready(B, H, W, x.device):
+            # (made while recording they would hold nothing before the first replay, and eager calls would read them)
+            raise RuntimeError("GatedPixelCNN.verify: call it once before recording: its packed weights and class tables are not made yet")
         # (cells behind a grid's drafts may hold anything, and a code outside the table is rejected: neither is looked up)
         cells = self.forward(x.clamp(0, self.embedding.num_embeddings - 1), label).flatten(2).transpose(1, 2)     # [B, H*W, codes], a view
         return ops.prior_verify(cells, draft, x.reshape(B, H * W), u_accept, u_draw, lengths, draft_probs)

@@ -263,3 +263,55 @@ def test_a_replaced_weight_at_an_earlier_address_is_quantised_anew():
             fresh = copy.deepcopy(e)
             assert torch.equal(e(x), fresh(x))
             del fresh
+
+
+def test_verify_is_recorded_once_its_tables_are_made(monkeypatch):
+    """Packed weights and class tables that a first call makes would hold nothing until the graph's first replay, and eager calls
+    would read them: refused.  A recorded graph has buffers of its own: calls of other batch sizes, which drop the kept ones,
+    other graphs and changed weights leave it what it is."""
+    target = prior(5)
+    g = torch.Generator().manual_seed(9)
+    u = lambda *s: torch.rand(*s, generator=g, dtype=torch.float64).to(DEV)
+
+    def inputs(B):
+        return [torch.randint(0, 128, (B, 3, 3), generator=g).to(DEV), torch.randint(0, 16, (B,), generator=g).to(DEV),
+                torch.randn(B, 9, 128, generator=g).to(DEV), u(B, 9), u(B)]
+    a, b, other = inputs(6), inputs(6), inputs(11)
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="once before"):
+            target.verify(*a)
+    assert not target._bufs and target._packed_key is None
+    target.verify(*a)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for args in (a, b):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(target.verify(*args))
+    for i in range(4):
+        for args in (a, b):
+            for t, v in zip(args, inputs(6)):
+                t.copy_(v)
+        want = [[t.clone() for t in target.verify(*args)] for args in (a, b)]
+        target.generate(None, other[1], batch_size=11, uniforms=other[3])         # (drops the buffers of other batch sizes)
+        spoil = [torch.full((1 << 18,), float("nan"), device=DEV) for _ in range(64)]
+        for j in ((0, 1), (1, 0))[i % 2]:
+            graphs[j].replay()
+        for got, w in zip(outs, want):
+            assert torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])
+        assert all(t.isnan().all() for t in spoil)
+        del spoil
+        torch.cuda.synchronize()
+    with torch.no_grad():
+        target.embedding.weight.add_(0.0)                                         # (another version of the same weights)
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="once before"):
+            target.verify(*a)
+    target.verify(*other)                                                         # packs them anew
+    spoil = [torch.full((1 << 18,), float("nan"), device=DEV) for _ in range(64)]
+    graphs[0].replay()
+    assert torch.equal(outs[0][0], want[0][0]) and torch.equal(outs[0][1], want[0][1]) and all(t.isnan().all() for t in spoil)
+    twin = copy.deepcopy(target)
+    assert not twin._recorded and target._recorded
