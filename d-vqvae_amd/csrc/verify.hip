@@ -1150,19 +1150,24 @@ constexpr int kShortWaves = 2048;
 constexpr int kShortStage = 6144;
 constexpr size_t kCellBytes = 65536;                         // LDS of a tile of all positions
 static bool verify_split(int64_t B, int V, bool unit) { return V > 2 * kTile && (!unit || (B < kRowsMin && V > kRowsTo)); }
+// Short rows: whether the row's block of `size`-byte logits is staged, and the waves of a workgroup.
+static bool verify_staged(int V, int P, int64_t lp, int64_t lv, size_t size) { return P > 1 && lp == 1 && lv == P && (size_t)V * P * size <= 32768; }
+static int verify_short_waves(int64_t B, int V, int G, int P, bool staged, size_t size) {
+    int64_t waves = (kShortWaves + B - 1) / B;
+    const int64_t least = staged ? (int64_t)((size_t)V * P * size / kShortStage) : 0;
+    if (waves < least) waves = least;
+    if (waves > G + 1) waves = G + 1;
+    if (waves > 16) waves = 16;
+    return waves < 1 ? 1 : (int)waves;
+}
 
 template <typename T, typename D, bool PROBS>
 static int verify_launch(const VerifyArgs& a, char* ws, hipStream_t st) {
     const dim3 grid((unsigned)a.B);
     if (a.V <= 2 * kTile) {
         const size_t block = (size_t)a.V * a.P * sizeof(T), room = (kTile + kTile / 8) * sizeof(double);
-        const bool staged = a.P > 1 && a.lp == 1 && a.lv == a.P && block <= 32768;
-        int64_t waves = (kShortWaves + a.B - 1) / a.B;
-        if (staged && waves < (int64_t)(block / kShortStage)) waves = block / kShortStage;
-        if (waves > a.G + 1) waves = a.G + 1;
-        if (waves > 16) waves = 16;
-        if (waves < 1) waves = 1;
-        const dim3 blk((unsigned)waves * 64);
+        const bool staged = verify_staged(a.V, a.P, a.lp, a.lv, sizeof(T));
+        const dim3 blk((unsigned)verify_short_waves(a.B, a.V, a.G, a.P, staged, sizeof(T)) * 64);
         const size_t lds = staged && block > room ? block : room;
         if (a.V <= kTile) {
             if (staged) hipLaunchKernelGGL((verify_short_kernel<1, true, T, D, PROBS>), grid, blk, lds, st, a);
@@ -1224,12 +1229,14 @@ extern "C" int dvq_prior_verify(const DvqPriorVerify* v, void* workspace, size_t
     if (v->B == 0) return DVQ_OK;
     if (!v->logits || !v->u_draw || !v->accepted || !v->next || (v->G > 0 && (!v->draft || !v->tokens || !v->u_accept)))
         return fail(DVQ_EINVAL, "prior_verify: null pointer");
-    // (threads of the largest launch: a wave or more per short row, a workgroup per row, or per row and part of it)
+    // (threads of the largest launch: the waves of a short row, a workgroup per row, or per row and part of it)
     const bool unit = v->logits_v == 1 && (v->draft_v == 1 || v->G == 0);
     const bool short_rows = v->V <= 2 * kTile, split = verify_split(v->B, v->V, unit);
     const int64_t parts = split_parts(v->V, unit) * (unit ? v->P : 1), per = (v->V + kTile * kSplitWaves - 1) / (kTile * kSplitWaves);
     const int64_t groups = !split ? 1 : parts > per ? parts : per;
-    if (!launch_fits(v->B * groups, short_rows ? 64 : kCellWaves * 64)) return fail(DVQ_EINVAL, "prior_verify: B x P x V too large");
+    const size_t size = v->logits_dtype == DVQ_F32 ? 4 : 2;
+    const int short_waves = verify_short_waves(v->B, v->V, v->G, v->P, verify_staged(v->V, v->P, v->logits_p, v->logits_v, size), size);
+    if (!launch_fits(v->B * groups, (short_rows ? short_waves : kCellWaves) * 64)) return fail(DVQ_EINVAL, "prior_verify: B x P x V too large");
     const size_t need = dvq_prior_verify_workspace_bytes(v);
     if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
         return fail(DVQ_EINVAL, "prior_verify: needs a 16-byte aligned workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : 0);

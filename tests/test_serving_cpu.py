@@ -163,3 +163,12 @@ def test_sizes_that_no_launch_holds_are_refused():
         assert _product(lib, **bad) == -1 and lib.dvq_last_error()
     for bad in (dict(B=1 << 26, V=8), dict(B=1 << 24, V=5000, logits_v=1, draft_v=1), dict(B=1 << 24, V=5000, logits_v=4, draft_v=4), dict(B=1 << 20, V=1 << 20, logits_v=9, draft_v=9)):
         assert lib.dvq_prior_verify(ctypes.byref(_verify_args(**bad)), 16, 1 << 60, None) == -1 and b"too large" in lib.dvq_last_error()
+
+
+@pytest.mark.parametrize("logits_dtype,V,P,waves", [(0, 1000, 8, 5), (1, 1000, 16, 5), (0, 500, 7, 2), (0, 900, 9, 5)])
+def test_short_rows_of_several_waves_that_no_launch_holds_are_refused(logits_dtype, V, P, waves):
+    """Staged rows have up to five waves whatever their number: counted as launched, not as one."""
+    lib = _lib.load()
+    for B in (((1 << 32) - 1) // (64 * waves) + 1, 1 << 26):
+        a = _verify_args(B=B, V=V, P=P, G=P - 1, logits_dtype=logits_dtype, logits_p=1, logits_v=P, draft_v=1)
+        assert lib.dvq_prior_verify(ctypes.byref(a), 16, 1 << 60, None) == -1 and b"too large" in lib.dvq_last_error()
