@@ -179,19 +179,23 @@ __global__ __launch_bounds__(64) void int8_prepare_kernel(Int8Prepare p, int64_t
     }
 }
 
-// Scaled in 64 bits, rounded once: no intermediate leaves the range of 32 bits where the result does not (s is up to 2^121,
-// the sum up to 2^31), at four 64-bit instructions per output.
-__device__ __forceinline__ float int8_scale(int acc, double s, double t, double b, int relu) {
-    const float v = (float)__builtin_fma((double)acc, s * t, b);
-    return relu && v < 0.f ? 0.f : v;
+// Scaled in 64 bits: no intermediate leaves the range of 32 bits where the result does not (s is up to 2^121, the sum up to
+// 2^31), at four 64-bit instructions per output, seven for 16 bits.  Stored with one rounding to the output's type: on its way to 16 bits through
+// 32, a value next to the border of two 16-bit values would be rounded onto the border and then to the even side.
+__device__ __forceinline__ double int8_scale(int acc, double s, double t, double b, int relu) {
+    const double v = __builtin_fma((double)acc, s * t, b);
+    return relu && v < 0.0 ? 0.0 : v;
 }
-__device__ __forceinline__ void int8_store(float* y, float v) { *y = v; }
-__device__ __forceinline__ void int8_store(unsigned short* y, float v) { *y = f32_to_bf16_bits(v); }
-__device__ __forceinline__ void int8_store4(float* y, const float (&v)[4]) { *reinterpret_cast<f32x4*>(y) = f32x4{v[0], v[1], v[2], v[3]}; }
-__device__ __forceinline__ void int8_store4(unsigned short* y, const float (&v)[4]) {
+__device__ __forceinline__ unsigned short int8_to_bf16(double v) { return __builtin_bit_cast(unsigned short, static_cast<__bf16>(v)); }
+__device__ __forceinline__ void int8_store(float* y, double v) { *y = (float)v; }
+__device__ __forceinline__ void int8_store(unsigned short* y, double v) { *y = int8_to_bf16(v); }
+__device__ __forceinline__ void int8_store4(float* y, const double (&v)[4]) {
+    *reinterpret_cast<f32x4*>(y) = f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+}
+__device__ __forceinline__ void int8_store4(unsigned short* y, const double (&v)[4]) {
     uint2 o;
-    o.x = f32_to_bf16_bits(v[0]) | (unsigned)f32_to_bf16_bits(v[1]) << 16;
-    o.y = f32_to_bf16_bits(v[2]) | (unsigned)f32_to_bf16_bits(v[3]) << 16;
+    o.x = int8_to_bf16(v[0]) | (unsigned)int8_to_bf16(v[1]) << 16;
+    o.y = int8_to_bf16(v[2]) | (unsigned)int8_to_bf16(v[3]) << 16;
     *reinterpret_cast<uint2*>(y) = o;
 }
 
@@ -470,7 +474,7 @@ __global__ __launch_bounds__(WVM * WVN * 64) void int8_tile_kernel(Int8Batch p, 
             for (int q = 0; q < 4; ++q) {
                 const int n = 32 * j + 8 * q + 4 * h;
                 const double* t = tb + wn + n;
-                float v[4];
+                double v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = int8_scale(acc[i][j][4 * q + e], s, t[e], t[BN + e], relu);
                 int8_store4(reinterpret_cast<Y*>(slab + r * RS) + n, v);

@@ -338,3 +338,40 @@ def test_rows_quantised_by_every_workgroup_and_once_before(M, K, N, dtype):
     xs = [x.to(DEV), x.to(DEV).flip(0)]
     for z, want in zip(ops.linear_int8_batched(xs, [W.to(DEV)] * 2, [t.to(DEV)] * 2, [b.to(DEV)] * 2, relu=True), (y, y.flip(0))):
         assert torch.equal(z.nan_to_num(7.0), want.nan_to_num(7.0)) and torch.equal(z.isnan(), want.isnan())
+
+
+# ------------------------------------------------------------- rounded once
+def to_bf16_exactly(v):
+    """float64 -> the nearest bfloat16 (ties to even) as float64, in one rounding."""
+    m, e = np.frexp(v)
+    q = np.exp2(np.maximum(e - 8, -133).astype(np.float64))        # 8 significant bits, no finer than the smallest subnormal
+    return np.rint(v / q) * q
+
+
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("M,N", [(3, 70), (30, 100), (70, 200), (700, 650), (1500, 1400), (2048, 4096)])
+def test_bf16_outputs_are_rounded_once(M, N, relu):
+    """Biases on the border of two bfloat16 values, sums that move them off it by less than 32 bits hold: rounded to 32 bits in
+    between they would lie on the border again.  Everything up to the rounding is exact in 64 bits."""
+    K = 64
+    W = torch.zeros(N, K, dtype=torch.int8)
+    W[:, 5] = 1
+    b = (1 + (2 * (torch.arange(N) % 128) + 1) * 2.0 ** -8) * torch.exp2((torch.arange(N) % 7 - 3).float())
+    b[::3] *= -1
+    b[1::11] = 5 * 2.0 ** -134                                      # (a border of subnormals)
+    t = torch.where(b.abs() < 1e-30, 2.0 ** -120, 1.0)              # (there the sums are a part of the subnormals' step as well)
+    codes = torch.zeros(M, K, dtype=torch.int8)
+    codes[:, 5] = torch.tensor([1, -1, 0, 1, 1, -1])[torch.arange(M) % 6].to(torch.int8) * 127
+    s = torch.full((M,), 2.0 ** -40)
+    x = codes.float() * 2.0 ** -40                                  # quantised in the call: the same codes and scales
+    want = to_bf16_exactly(codes[:, 5].double().numpy()[:, None] * (s.double().numpy()[:, None] * t.double().numpy()[None, :]) + b.double().numpy()[None, :])
+    want = np.where(want < 0, 0.0, want) if relu else want
+    dev = [v.to(DEV) for v in (W, t, b)]
+    for xs in (x.to(DEV), x.to(torch.bfloat16).to(DEV), (codes.to(DEV), s.to(DEV))):
+        y = ops.linear_int8(xs, *dev, relu=relu, out_dtype=torch.bfloat16)
+        assert np.array_equal(y.float().cpu().numpy().astype(np.float64), want)
+        wide = torch.zeros(M, N + 7, dtype=torch.bfloat16, device=DEV)
+        ops.linear_int8(xs, *dev, relu=relu, out=wide[:, 3:3 + N])
+        assert torch.equal(wide[:, 3:3 + N], y)
+    for y in ops.linear_int8_batched([x.to(DEV)] * 2, [dev[0]] * 2, [dev[1]] * 2, [dev[2]] * 2, relu=relu, out_dtype=torch.bfloat16):
+        assert np.array_equal(y.float().cpu().numpy().astype(np.float64), want)
