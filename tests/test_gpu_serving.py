@@ -315,3 +315,26 @@ def test_verify_is_recorded_once_its_tables_are_made(monkeypatch):
     assert torch.equal(outs[0][0], want[0][0]) and torch.equal(outs[0][1], want[0][1]) and all(t.isnan().all() for t in spoil)
     twin = copy.deepcopy(target)
     assert not twin._recorded and target._recorded
+
+
+def test_generated_parameters_are_those_of_the_8_bit_layers_one_by_one():
+    """Generation with 8-bit heads: what both decoders make of the pieces they are given equals their layers on the 64-bit oracle,
+    and the parameter vector is made of that."""
+    from dvq_hip.pipeline import GraspGenerator, assemble_param
+    gen = GraspGenerator.synthetic(torch.device(DEV), seed=0, with_prior=True)
+    objs = synth.object_clouds(5, 300, seed=4).to(DEV)
+    xt = torch.randint(0, 128, (5, 3, 3), generator=torch.Generator().manual_seed(0)).to(DEV)
+    set_head_dtype(gen.model, torch.int8)
+    seen = {}
+    for name in ("decoder", "pos_decoder"):
+        def record(pieces, name=name, run=getattr(gen.model, name).forward_pieces):
+            y = run(pieces)
+            seen[name] = (torch.cat([p[1][p[0]] if isinstance(p, tuple) else p for p in pieces], 1).cpu(), y.clone())
+            return y
+        getattr(gen.model, name).forward_pieces = record
+    param = gen.generate(objs, x_tilde=xt)["recon_param"]
+    for name in ("decoder", "pos_decoder"):
+        x, y = seen[name]
+        ref = oracle_mlp([m for m in getattr(gen.model, name).MLP if isinstance(m, torch.nn.Linear)], x, False)
+        assert np.all(np.abs(y.cpu().double().numpy() - ref) <= 2.0 ** -24 * np.abs(ref) * (1 + 1e-6) + 2.0 ** -50)
+    assert torch.equal(param, assemble_param(seen["decoder"][1], seen["pos_decoder"][1]))
