@@ -26,13 +26,15 @@ namespace dvq {
 // Residual mass below this is rounding (p and q equal up to 64-bit noise): the draw is then from p itself.
 constexpr double kVerifyNoMass = 9.094947017729282e-13;   // 2^-40
 constexpr int kTile = 512;                                // codes of a tile: 8 per lane
-// Relative error of u q / p from sums taken in 32 bits.  A term exp2((x - ref) log2 e) carries |x - ref| 1.5 * 2^-23 from its
-// argument (difference, constant and product rounded) and 2^-23 from the exponential; eight of them are added in 32 bits
-// (3 * 2^-24), the eights in 64.  ref lies at most kVerifySlack below the largest logit and the mean of |x - ref| under the
-// distribution is at most kVerifySlack + ln V <= 8 + 13.9, so a lane's sum is off by less than 22 * 1.5 * 2^-23 + 2^-23 + 3 *
-// 2^-24 = 4.3e-6 relative.  Joining lanes, waves and workgroups moves sums by the difference of two such reference points,
-// counted in the mean above, at 2^-23 + 7 * 2^-24 = 5.4e-7 each of three times.  A sum is off by less than 6e-6, the quotient
-// of two by less than 1.2e-5.  More than three times that:
+// Relative error of u q / p from sums taken in 32 bits, in units of e = 2^-23.  A term exp2((x - r) log2 e) carries |x - r| 1.5 e from
+// its argument (difference, constant and product rounded) and e from the exponential; eight of them are added in 32 bits
+// (1.5 e), the eights in 64.  When the lane's reference r moves up by D > kVerifySlack, what is summed takes a factor with an
+// error of D 1.5 e + e: at most (R - r) 1.625 e over all moves up to the last reference R (at most (R - r) / 8 of them).  A term
+// lies at most kVerifySlack above the reference it was summed with, so it carries at most (R - x) 1.625 e where x <= r, and
+// (R - x + 8) 1.625 e + 8 * 1.5 e where x > r: (R - x) 1.625 e + 25 e + e in all cases.  Joining lanes, waves and workgroups
+// moves sums to larger references, counted in R, at e + 3.5 e for the exponential and seven roundings each of three times.
+// R is at most the largest logit, from which the mean distance under the distribution is at most ln V <= 13.9: a sum is off by
+// less than (22.6 + 26 + 1.5 + 13.5) e = 7.6e-6, the quotient of two by less than 1.6e-5.  Two and a half times that:
 constexpr double kVerifyMargin = 4e-5;
 constexpr float kVerifySlack = 8.f;
 
@@ -202,8 +204,8 @@ __device__ __forceinline__ double sum_moved(const Exp& ex, const Sum& a, float r
     return a.ref > -__builtin_inff() && a.ref < ref ? a.s * ex((double)a.ref - (double)ref) : a.s;
 }
 
-// The reference moves up only where the next eight codes of some lane exceed it by more than kVerifySlack: what that lane has
-// summed is then less than e^-8 of what it sums now, and 32 bits are enough to move it.
+// The reference moves up only where the next eight codes of some lane exceed it by more than kVerifySlack.  What the lane has summed
+// may be most of its mass then (many codes just within the slack): the factor's error counts in kVerifyMargin.
 __device__ __forceinline__ void sum_add(Sum& a, const float (&x)[8]) {
     float m = x[0];
 #pragma unroll
@@ -335,7 +337,7 @@ __device__ __forceinline__ double verify_sum8(const double (&w)[8]) {
 // a code whose sign that k does not settle.
 struct Tile { double mass, c; bool near; };
 
-// One wave.  w.k is within kVerifyMargin / 3 of the true one.
+// One wave.  w.k is within kVerifyMargin / 2 of the true one.
 template <bool PROBS, typename T, typename D>
 __device__ __forceinline__ Tile verify_pass(const Exp& ex, const Weights& w, const T& t, const D& q, double& sp, double& sq) {
     double mass[2] = {0.0, 0.0}, c[2] = {0.0, 0.0}, p2[2] = {0.0, 0.0}, q2[2] = {0.0, 0.0};

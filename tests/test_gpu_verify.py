@@ -458,3 +458,47 @@ def test_a_nan_among_masked_codes(B, V, layout):
     place = (lambda k, v: v) if layout == "rows" else lambda k, v: v.transpose(1, 2).contiguous().transpose(1, 2) if k in ("logits", "draft") else v
     _, n = check(c, place=place)
     assert (n == -1).any() and (n >= 0).any()
+
+
+def rising(V, kind, g):
+    """Logits whose running reference point has to move: levels just below and above the slack of 8, slow and fast ascents."""
+    at = torch.arange(V).float() / V
+    tile = torch.arange(V) // 512
+    if kind == "below":                                          # 7.9 above the first level for most of the row
+        x = torch.where(at < 0.1, 0.0, 7.9)
+    elif kind == "steps":                                        # most of the mass lies 7.9 above, then one tile 8.1 above moves it
+        x = torch.where(at < 0.1, 0.0, 7.9)
+        x[-600:] = 8.1
+    elif kind == "stairs":                                       # every tile 8.1 above the one in front of it, up to the last six
+        x = 8.1 * (tile - tile.max()).clamp_min(-6).float()
+    elif kind == "gentle":                                       # moves in most tiles, each of them with mass
+        x = 40.0 * at
+    else:
+        x = torch.sort(12.0 * torch.randn(V, generator=g)).values
+    return x + 0.01 * torch.randn(V, generator=g)
+
+
+@pytest.mark.parametrize("kind", ["below", "steps", "stairs", "gentle", "sorted"])
+@pytest.mark.parametrize("B,V", [(8, 6000), (24, 20000), (130, 9000)])
+def test_ascending_logits_and_uniforms_next_to_the_border(B, V, kind):
+    """Rows whose reference point moves while its lane holds most of the mass: the test sums are joined over moves, and tests from
+    1e-12 to 1e-4 next to the border have to come out as in 64 bits."""
+    g = torch.Generator().manual_seed(V + B)
+    c = make(B, 1, 2, V, seed=V)
+    want = []
+    for b in range(B):
+        up = rising(V, kind, g)
+        c["logits"][b, 0] = up
+        c["draft"][b, 0] = up.flip(0) if b % 3 == 0 else up + 0.3 * torch.randn(V, generator=g)
+        p, q = S.distribution(c["logits"][b, 0].numpy()), S.distribution(c["draft"][b, 0].numpy())
+        x = int(np.argmin(np.where(q > 1e-9, p / np.maximum(q, 1e-300), np.inf)))
+        if not p[x] > 1e-12:
+            x = int(np.argmax(np.where(p < q, p, 0.0)))          # (flipped: a code that both have)
+        assert 0 < p[x] < q[x]
+        c["tokens"][b, 0] = x
+        off = (1e-12, 1e-9, 1e-7, 1e-6, 5e-6, 1.5e-5, 3e-5, 1e-4)[b // 2 % 8]
+        c["u_accept"][b, 0] = p[x] / q[x] * (1 - off if b % 2 else 1 + off)
+        want.append(b % 2)
+    for place in (lambda k, v: v, lambda k, v: v.transpose(1, 2).contiguous().transpose(1, 2) if k in ("logits", "draft") else v):
+        a, _ = check(c, place=place)
+        assert a.tolist() == want
