@@ -46,7 +46,7 @@ def _int8_weight(layer):
     changes.  A graph that is being recorded quantises for itself and reads nothing that is kept: it follows the weight, as it
     does in fp32 (one more launch, the weight's bytes, a replay)."""
     W = layer.weight.detach()
-    if torch.cuda.is_current_stream_capturing():
+    if W.is_cuda and torch.cuda.is_current_stream_capturing():
         return ops.quantize_rows(W.float())
     key = (W.data_ptr(), W._version, dvq_hip.weights_epoch())
     kept = layer.__dict__.setdefault("_dvq_int8", _Int8Copy())

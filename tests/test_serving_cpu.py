@@ -172,3 +172,10 @@ def test_short_rows_of_several_waves_that_no_launch_holds_are_refused(logits_dty
     for B in (((1 << 32) - 1) // (64 * waves) + 1, 1 << 26):
         a = _verify_args(B=B, V=V, P=P, G=P - 1, logits_dtype=logits_dtype, logits_p=1, logits_v=P, draft_v=1)
         assert lib.dvq_prior_verify(ctypes.byref(a), 16, 1 << 60, None) == -1 and b"too large" in lib.dvq_last_error()
+
+
+def test_8_bit_heads_on_the_cpu_are_refused():
+    from network.DVQVAE import Decoder, Encoder
+    for head in (Encoder([8, 6], 4), Decoder([6, 4], 8)):
+        with pytest.raises(RuntimeError, match="HIP device"):
+            set_head_dtype(head, torch.int8)(torch.zeros(2, 8))
