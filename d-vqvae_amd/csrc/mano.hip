@@ -328,7 +328,7 @@ __global__ __launch_bounds__(WAVES * 64) void mano_lbs_kernel(
         constexpr int VP = TABLE ? 2 : 1;
 #pragma unroll
         for (int i0 = 0; i0 < 4; i0 += VP) {
-        // (kept as pairs of neighbours within a row, the order the LDS reads deliver: one packed multiply-add per pair)
+        // (kept as pairs of neighbours within a row, the order the LDS reads deliver)
         f32x2 T2[VP][6];
 #pragma unroll
         for (int u = 0; u < VP; ++u)

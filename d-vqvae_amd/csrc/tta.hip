@@ -33,7 +33,7 @@ __device__ __forceinline__ int wave_sum_i(int v) {
 }
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-constexpr int kTtaPts = 4;   // object points per thread and pass (two packed-fp32 pairs)
+constexpr int kTtaPts = 4;   // object points per thread and pass, kept as two pairs (the operations are scalar ones)
 // 768 threads x 4 points cover a 3000-point cloud in one pass, and twelve waves per workgroup (two workgroups
 // per CU) give each SIMD six waves to hide the LDS latency of the vertex reads behind other waves' arithmetic.
 constexpr int kCgThreads = 768;
@@ -42,7 +42,7 @@ constexpr int kCgGroup = 8;    // hand vertices per scan step (one compare-selec
 
 // Vertices are searched in `order`: the n_contact vertices of the contact set first, then the others.
 // The nearest contact-set vertex is then simply the running minimum at the end of the first group, and
-// every (point, vertex) pair costs three packed subtract/multiply-add pairs and one compare-select, not two.
+// every (point, vertex) pair costs six fp32 subtractions and multiply-adds and one minimum, not two.
 // Exact distance ties resolve to the lowest vertex id (both parts of `order` must list their vertices ascending).
 __global__ __launch_bounds__(kCgThreads, 6) void tta_contact_grad_kernel(
     const float* __restrict__ obj, int64_t sb, int64_t sc, int64_t sp, int N, const float* __restrict__ verts, int V, int nC,

@@ -7,7 +7,7 @@
 //   mode 4  as 3, but the consumer's loads carry the device-scope bit (sc1) instead
 // Every phase each workgroup rewrites its 16-KiB slice of the group's buffer and, after the barrier, checks the slice
 // of its neighbour in the group (which it also read in the phase before, so a stale L1 line shows).
-// Build: hipcc --offload-arch=gfx950 -O3 -o group_barrier group_barrier.hip
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o group_barrier group_barrier.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -1,5 +1,5 @@
 // Read-bandwidth ceiling of one MI355X for a once-read stream: every lane loads 16 bytes per instruction, UNROLL
-// instructions in flight, persistent grid.  Build: hipcc --offload-arch=gfx950 -O3 -o hbm_stream hbm_stream.hip
+// instructions in flight, persistent grid.  Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o hbm_stream hbm_stream.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -10,7 +10,7 @@
 // and prints, per mode, the time and the fraction of the nominal 2.5 PFLOP/s.  Work = the search of 1 Mi x 256-d latents
 // against 8192 codes (4.4 TFLOP).  Under `rocprofv3 --pmc SQ_VALU_MFMA_BUSY_CYCLES SQ_BUSY_CU_CYCLES GRBM_GUI_ACTIVE` the
 // same launches give the matrix pipe's busy share and the clock held.
-// Build: hipcc --offload-arch=gfx950 -O3 -o mfma_ceiling mfma_ceiling.hip ; run: ./mfma_ceiling [mode|-1] [reps]
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o mfma_ceiling mfma_ceiling.hip ; run: ./mfma_ceiling [mode|-1] [reps]
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

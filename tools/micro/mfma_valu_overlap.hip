@@ -1,6 +1,6 @@
 // Do fp32 MFMAs of one wave run under the vector multiply-adds of another wave on the same SIMD?  One workgroup of 8 waves
 // per CU (two waves per SIMD); waves 0-3 run a chain of v_mfma_f32_16x16x4_f32 over three accumulators, waves 4-7 a chain of
-// packed fp32 multiply-adds (or LDS reads), each alone and both together.  Build: hipcc --offload-arch=gfx950 -O3 -o
+// fp32 multiply-adds (or LDS reads), each alone and both together.  Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o
 // mfma_valu_overlap mfma_valu_overlap.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
