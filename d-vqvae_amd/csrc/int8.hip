@@ -160,7 +160,8 @@ __device__ __forceinline__ void int8_quantize_row(const T* x, int K, bool wide, 
 
 // Rows 0 .. M-1 of every matrix of the batch are quantised; T = int8_t: copied to rows that start at multiples of 16 bytes.
 // The N rows behind them (if any) are weights, copied alike.  One wave per row: the maximum needs no barrier, and a row's 16-byte
-// loads are all under way at once.  Bound by memory: 4096 x 2560 fp32 (42 MB read, 10.5 written) 10.3 us, 5.1 TB/s -- a copy's rate.
+// loads are all under way at once.  Bound by memory: 4096 x 2560 fp32 (42 MB read, 10.5 written) 12.6 us, 4.2 TB/s -- four fifths of a
+// copy's rate (median of traced launches over three sets of operands, as all times of kernels here; 12.0 over one).
 template <typename T>
 __global__ __launch_bounds__(64) void int8_prepare_kernel(Int8Prepare p, int64_t ldx, int64_t ldw, int M, int K, int64_t ldc) {
     const int bz = blockIdx.y;
@@ -180,8 +181,9 @@ __global__ __launch_bounds__(64) void int8_prepare_kernel(Int8Prepare p, int64_t
 }
 
 // Scaled in 64 bits: no intermediate leaves the range of 32 bits where the result does not (s is up to 2^121, the sum up to
-// 2^31), at four 64-bit instructions per output, seven for 16 bits.  Stored with one rounding to the output's type: on its way to 16 bits through
-// 32, a value next to the border of two 16-bit values would be rounded onto the border and then to the even side.
+// 2^31), at four 64-bit instructions per output, seven for 16 bits.  Stored with one rounding to the output's type: on its way
+// to 16 bits through 32, a value next to the border of two 16-bit values would be rounded onto the border and then to the
+// even side.
 __device__ __forceinline__ double int8_scale(int acc, double s, double t, double b, int relu) {
     const double v = __builtin_fma((double)acc, s * t, b);
     return relu && v < 0.0 ? 0.0 : v;
@@ -211,7 +213,8 @@ __device__ __forceinline__ void int8_load16(const T* x, int k, int K, bool wide,
 // reads weights and activations of its own share of k straight in the operand layout of the 16x16x64 instruction (lane l: 16
 // consecutive k of row l % 16) and quantises in registers; all that the waves exchange before the products is the rows'
 // maxima.  STEPS: blocks of 64 k per wave; K <= 512 STEPS.  Bound by latency (loads, maxima, codes, products, sums one after the
-// other): 1 x 2560 -> 1024 fp32 7.0 us, 16 x 2048 -> 1024 bf16 9.4 us for 2.6 MB, where two launches took 26.
+// other): 1 x 2560 -> 1024 fp32 6.9 us, 16 x 2048 -> 1024 bf16 9.2 us for 2.6 MB, where two launches took 26.  2048 features run
+// the instance of up to 2560: a fifth of its loads and products there is for nothing.
 template <int STEPS, typename T, typename Y>
 __global__ __launch_bounds__(512) void int8_rows16_kernel(Int8Batch p, int64_t ldx, int64_t ldw, int M, int K, int N, int relu, int64_t ldy) {
     __shared__ unsigned tops[8][16];
@@ -349,13 +352,15 @@ __device__ __attribute__((aligned(16))) const int int8_zeros[4] = {0, 0, 0, 0};
 // Tiles of BM x BN outputs, WVM x WVN waves, k in stages of BK bytes through a ring of R buffers in LDS: the copies of R
 // stages go straight from memory into LDS while the products of the stage in front of them run, one barrier a stage.  Rows
 // of both operands start at multiples of 16 bytes and K is a multiple of 16 (zeros behind the features); stages behind K
-// are copied from a line of zeros, so that every stage is the same number of loads.  The 16-byte pieces of a row are swapped by
-// its number, so that 32 rows' pieces of one k lie in all 64 banks.  The 256 x 256 tile is bound by the matrix instructions: 8192 x 4096 x 4096 145 us, 1.9 POP/s; the others by filling and emptying the
-// ring, with one or two tiles a CU: 4096 x 2560 -> 1024 20 us, six of 512 x 1024 -> 512 9.6.  No fence keeps the fragments' reads in
-// front of the products (170 us with one: the scheduler interleaves them better).
+// are copied from a line of zeros, so that every stage is the same number of loads.
 // LDS serves 16 lanes of a 16-byte read at a time from 64 banks (256 bytes): with rows of 128 (64) bytes those are 16 rows, of
 // which every second (fourth) falls on the same banks.  16-byte piece c of a row lies at place c ^ (row / 2 % 8) (c ^ (row / 4
 // % 4)), which spreads them over all banks; the copies stay linear in LDS, each lane picks its source.
+// 256 x 256: 8192 x 4096 x 4096 149 us, 1.85 POP/s; the matrix pipes are busy 54 % of the cycles (131 k of 243 k per SIMD, at
+// 1.85 GHz), 29 % of the waves' cycles are waits, in 43 % an instruction is held back.  128 x 128: 4096 x 2560 -> 1024 19.4 us; matrix
+// pipes 30 %, waits 45 %: one tile a CU, so that neither the ring's filling and emptying nor the 168 MB from L2 into LDS
+// (8.7 TB/s) run behind another tile; the two were not measured apart.  64 x 64: six of 512 x 1024 -> 512 9.8 us.  No fence keeps
+// the fragments' reads in front of the products (170 us with one: the scheduler interleaves them better).
 template <int BM, int BN, int WVM, int WVN, int BK, int R, typename Y>
 __global__ __launch_bounds__(WVM * WVN * 64) void int8_tile_kernel(Int8Batch p, int64_t ldx, int64_t ldw, int M, int K, int N, int relu, int64_t ldy) {
     constexpr int WV = WVM * WVN, TM = BM / WVM / 32, TN = BN / WVN / 32;

@@ -493,7 +493,8 @@ __device__ __forceinline__ void verify_copy(const T* from, int total, T* to) {
 //
 // STAGED: the prior's forward hands its logits over as [B, V, cells], all positions of a code side by side.  Read position
 // by position, every position fetches every cache line of the row again (from L2: 4096 grids of 9 x 512 took 38 us, bound
-// by that); the row's block is copied into LDS once instead: 25 us, 16 of them the memory's.  One grid takes 3.9 us of kernel.
+// by that); the row's block is copied into LDS once instead: 25 us a call, 16 of them the memory's.  One grid takes 4.0 us of kernel
+// over one set of operands, 5.2 over three in turns (medians of traced launches).
 template <int TILES, bool STAGED, typename T, typename D, bool PROBS>
 __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(TILES == 1 && PROBS ? 8 : 4))) void verify_short_kernel(VerifyArgs a) {
     extern __shared__ __align__(16) char block[];                // the staged block, later room for verify_locate
@@ -635,8 +636,9 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(TILES == 1
 // The draw of a row whose tiles have been passed over: mass, c and near of every tile in LDS, sp and sq the sums of e_p and e_q.
 // Every wave calls it.
 template <typename T, typename D, bool PROBS>
-__device__ __forceinline__ void verify_finish(const Exp& ex, const VerifyArgs& args, int64_t b, double at_draw, const T* lr, const D* dr, Weights w, bool unit, double sp,
-                                              double sq, double* a, const double* c, const unsigned char* near, int tiles, double* lds) {
+__device__ __forceinline__ void verify_finish(const Exp& ex, const VerifyArgs& args, int64_t b, double at_draw, const T* lr, const D* dr,
+                                              Weights w, bool unit, double sp, double sq, double* a, const double* c,
+                                              const unsigned char* near, int tiles, double* lds) {
     const int wave = verify_wave(), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     double total = 0.0;
     if (w.residual) {
@@ -763,7 +765,8 @@ __device__ __forceinline__ void verify_sums(Ring<T, D, Q>& ring, const Share& w,
 
 // Codes side by side (a.unit).  The tests run at 86 % of a copy's rate (1024 rows x 16381 bf16, all drafts kept, no draw: 60 us for 268 MB);
 // the draw, 64-bit exponentials of the whole row once more, takes 45 us where every row ends in one, 24 without a residual.  With rows
-// that stop at different positions 84 us (41 of memory); 1000 of up to 5 x 8192 46 us (14).
+// that stop at different positions 86 us over three sets of operands in turns, 78 over one that fits the last cache (41 of memory); 1000 of
+// up to 5 x 8192 46 to 48 us (14), where a draw in 32 bits saved 1 to 3: what holds it is that rows of 0 to 5 positions end apart.
 template <int WAVES, typename T, typename D, bool PROBS>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(4))) void verify_row_kernel(VerifyArgs a) {
     extern __shared__ double tile_a[];                           // per tile of the row: a, c, near
